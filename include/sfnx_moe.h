@@ -41,6 +41,9 @@ extern "C" {
 
 enum { SFNX_Q4_0 = 2, SFNX_Q5_1 = 7, SFNX_Q8_0 = 8, SFNX_Q4_K = 12, SFNX_Q5_K = 13 }; /* GgmlType ids (src/gguf.hpp:22-25; the others ggml's) */
 
+/* types of activations and outputs (ggml's ids) where a call lets the caller choose */
+enum { SFNX_F32 = 0, SFNX_F16 = 1, SFNX_BF16 = 30 };
+
 /* src/kernels.hpp:18-23: one expert's matrix applied to up to SFNX_MAXT activation rows */
 typedef struct sfnx_job {
     int w;                    /* expert */
@@ -179,6 +182,50 @@ int sfnx_q8s_swiglu_gemv(const sfnx_q8s* W, int rows, int ffs, const float* gu, 
  * the reference calls cublasGemmEx; the C rows are taken 64 at a time.  rows % 256 == 0, cols % 512 == 0. */
 int sfnx_pf_dense(const sfnx_q8s* W, int rows, int cols, const uint16_t* xh, int C, float* out, int ldo, void* wk,
                   size_t wk_bytes, void* st);
+
+/* ---------------------------------------------------------------------------------------------- 8-bit floating point
+ * No counterpart in the reference, whose experts are GGUF block types: experts and dense matrices as e4m3 (the 8-bit type of
+ * 4 exponent and 3 mantissa bits without infinities, largest value 448) with an f32 scale for each block of 128.  A matrix
+ * [rows][cols] of the 8-bit store is its values, row-major, then the scales of its 128 x 128 blocks
+ * [ceil(rows / 128)][ceil(cols / 128)] (the last blocks of a row or column may be shorter); an activation row has a scale for
+ * each 128 values, [rows][ceil(cols / 128)].  A product is the
+ * sum over b of (xs_b ws_b) (sum over the block's k of xq[k] wq[k]), on the matrix cores: in fp32 where the result is kept
+ * in 32 bits or quantized again, and for jobs of up to 16 rows; where it is rounded to 16 bits (more than 16 rows), sums of
+ * 8 consecutive products keep 13 bits of the largest, 1.5e-5 of the result's norm, and the rest is fp32.
+ * cols % 16 == 0; pointers 16-byte aligned (outputs and scales to their type); expert strides a multiple of 16, or 0 for a
+ * table of expert pointers; out_type SFNX_F32, SFNX_F16 or SFNX_BF16.  Rows that no job names are left as they were.
+ * A matrix's values and the activation rows are read as they are: a NaN reaches every output it belongs to. */
+/* bytes of a matrix of the 8-bit store, rounded up to 16 */
+size_t sfnx_f8_matrix_bytes(int rows, int cols);
+/* rows of x (type SFNX_F32, SFNX_F16 or SFNX_BF16, ldx values apart) as 8-bit rows: per 128 values
+ * s = max(max |x| c, 2^-126) over the finite ones with c = 1 / 448 in fp32, q = e4m3(x / s); values that are not finite
+ * become NaN */
+int sfnx_quantize_f8(uint32_t type, const void* x, int64_t ldx, int rows, int cols, uint8_t* q, float* s, void* st);
+/* out[c][n] (rows ldo values apart) = row n of the matrix W times 8-bit row c, c < C */
+int sfnx_f8_gemm(const void* W, int rows, int cols, const uint8_t* xq, const float* xs, int C, uint32_t out_type, void* out,
+                 int ldo, void* st);
+/* A decode window's routed gate|up: per job, h[out[j]] = silu(gate) * up of 8-bit row y[j], the expert's rows
+ * [gate (ff) | up (ff)] as in sfnx_moe_gate_up; ff % 16 == 0 */
+int sfnx_moe_gate_up_swiglu_f8(const void* A, size_t sa, int n_in, int ff, const sfnx_job* jobs, const int* njobs,
+                               int njobs_max, const uint8_t* xq, const float* xs, float* h, void* st);
+/* A window's down: out[out[j]] = the expert's rows times h[y[j]], h's rows quantized in the call as sfnx_quantize_f8 does
+ * (out rows n_out values apart); n_in <= 8192 */
+int sfnx_moe_down_f8(const void* A, size_t sa, int n_in, int n_out, const sfnx_job* jobs, const int* njobs, int njobs_max,
+                     const float* h, uint32_t out_type, void* out, void* st);
+/* The same over a prompt chunk's BigJobs, h as 8-bit rows (hq [pairs][ff], hs [pairs][ceil(ff / 128)]) */
+int sfnx_moe_gate_up_swiglu_f8_big(const void* A, size_t sa, int n_in, int ff, const sfnx_bigjob* jobs, const int* njobs,
+                                   int njobs_cap, const uint8_t* xq, const float* xs, uint8_t* hq, float* hs, void* st);
+int sfnx_moe_down_f8_big(const void* A, size_t sa, int n_in, int n_out, const sfnx_bigjob* jobs, const int* njobs,
+                         int njobs_cap, const uint8_t* hq, const float* hs, uint32_t out_type, void* out, void* st);
+
+/* ---------------------------------------------------------------------------------------------- 16-bit experts
+ * No counterpart in the reference: experts that are not quantized, matrices [n_out][n_in] of f16 or bf16 (type SFNX_F16 or
+ * SFNX_BF16) sa bytes apart (a multiple of 16, or 0 for a table of pointers), over a window's jobs or a chunk's BigJobs:
+ * out[out[j]] = the expert's rows times row y[j] of x (the same type), summed in fp32.  n_in % 8 == 0. */
+int sfnx_moe_mm_16(const void* A, size_t sa, uint32_t type, int n_in, int n_out, const sfnx_job* jobs, const int* njobs,
+                   int njobs_max, const uint16_t* x, uint32_t out_type, void* out, void* st);
+int sfnx_moe_mm_16_big(const void* A, size_t sa, uint32_t type, int n_in, int n_out, const sfnx_bigjob* jobs,
+                       const int* njobs, int njobs_cap, const uint16_t* x, uint32_t out_type, void* out, void* st);
 
 /* ---------------------------------------------------------------------------------------------- fused decode */
 /* one layer's weights: router W [E + 1][H] fp32 (row E gates the shared expert), planar gate|up experts (E + 1 of

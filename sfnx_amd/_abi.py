@@ -14,6 +14,7 @@ LIB_PATH = Path(os.environ.get("SFNX_LIB", PKG / "libsfnx_moe.so"))   # SFNX_LIB
 HEADER = PKG.parent / "include" / "sfnx_moe.h"
 
 Q4_0, Q5_1, Q8_0, Q4_K, Q5_K = 2, 7, 8, 12, 13
+F32, F16, BF16 = 0, 1, 30      # activation and output types (ggml's ids)
 MAXT, PF_JOB = 16, 64
 JOB_INTS = 2 + 2 * MAXT        # sfnx_job: w, n, y[16], out[16]
 BIGJOB_INTS = 2 + 2 * PF_JOB   # sfnx_bigjob
@@ -55,6 +56,15 @@ SIGNATURES = {
     "sfnx_moe_decode_q8s": (i32, [vp, vp, i32, u32, u32, i32, i32, i32, i32, vp, i32, i32, f32, vp, sz, i32, vp]),
     "sfnx_q8s_gemv": (i32, [vp, i32, i32, vp, vp, i32, i32, vp]),
     "sfnx_q8s_split": (i32, [vp, i32, i32, vp, vp]),
+    "sfnx_f8_matrix_bytes": (sz, [i32, i32]),
+    "sfnx_quantize_f8": (i32, [u32, vp, i64, i32, i32, vp, vp, vp]),
+    "sfnx_f8_gemm": (i32, [vp, i32, i32, vp, vp, i32, u32, vp, i32, vp]),
+    "sfnx_moe_gate_up_swiglu_f8": (i32, [vp, sz, i32, i32, vp, vp, i32, vp, vp, vp, vp]),
+    "sfnx_moe_down_f8": (i32, [vp, sz, i32, i32, vp, vp, i32, vp, u32, vp, vp]),
+    "sfnx_moe_gate_up_swiglu_f8_big": (i32, [vp, sz, i32, i32, vp, vp, i32, vp, vp, vp, vp, vp]),
+    "sfnx_moe_down_f8_big": (i32, [vp, sz, i32, i32, vp, vp, i32, vp, vp, u32, vp, vp]),
+    "sfnx_moe_mm_16": (i32, [vp, sz, u32, i32, i32, vp, vp, i32, vp, u32, vp, vp]),
+    "sfnx_moe_mm_16_big": (i32, [vp, sz, u32, i32, i32, vp, vp, i32, vp, u32, vp, vp]),
     "sfnx_hc_workspace": (sz, [i32, i32, i32, vp]),
     "sfnx_pf_dense": (i32, [vp, i32, i32, vp, i32, vp, i32, vp, sz, vp]),
     "sfnx_hc_read": (i32, [vp, vp, vp, vp, vp, vp, vp, vp, vp, f32, vp, vp, vp, i32, i32, i32, i32, vp, sz, vp]),

@@ -217,6 +217,41 @@ inline void hc_read(float* R, const float* bo, const float* inj_prev, const floa
                     LR, scratch, scratch_bytes, st));
 }
 
+// ------------------------------------------------------------------------------------------------ 8- and 16-bit experts
+// No counterpart in the reference (see sfnx_moe.h): a DW's p / ep hold matrices of the 8-bit store, or f16 / bf16 matrices
+// (type SFNX_F16 or SFNX_BF16 for the latter; unused for the former)
+inline void quantize_f8(uint32_t type, const void* x, int64_t ldx, int rows, int cols, uint8_t* q, float* s, void* st) {
+    ck(sfnx_quantize_f8(type, x, ldx, rows, cols, q, s, st));
+}
+inline void f8_gemm(const DW& W, const uint8_t* xq, const float* xs, int C, uint32_t out_type, void* out, int ldo, void* st) {
+    ck(sfnx_f8_gemm(W.p, W.n_out, W.n_in, xq, xs, C, out_type, out, ldo, st));
+}
+inline void moe_gate_up_swiglu_f8(const DW& A, size_t sa, const Job* jobs, const int* njobs, int njobs_max, const uint8_t* xq,
+                                  const float* xs, float* h, void* st) {
+    ck(sfnx_moe_gate_up_swiglu_f8(detail::base_of(A), detail::stride_of(A, sa), A.n_in, A.n_out / 2, jobs, njobs, njobs_max, xq, xs, h, st));
+}
+inline void moe_down_f8(const DW& A, size_t sa, const Job* jobs, const int* njobs, int njobs_max, const float* h,
+                        uint32_t out_type, void* out, void* st) {
+    ck(sfnx_moe_down_f8(detail::base_of(A), detail::stride_of(A, sa), A.n_in, A.n_out, jobs, njobs, njobs_max, h, out_type, out, st));
+}
+inline void moe_gate_up_swiglu_f8_big(const DW& A, size_t sa, const BigJob* jobs, const int* njobs, int njobs_cap,
+                                      const uint8_t* xq, const float* xs, uint8_t* hq, float* hs, void* st) {
+    ck(sfnx_moe_gate_up_swiglu_f8_big(detail::base_of(A), detail::stride_of(A, sa), A.n_in, A.n_out / 2, jobs, njobs, njobs_cap, xq, xs,
+                                      hq, hs, st));
+}
+inline void moe_down_f8_big(const DW& A, size_t sa, const BigJob* jobs, const int* njobs, int njobs_cap, const uint8_t* hq,
+                            const float* hs, uint32_t out_type, void* out, void* st) {
+    ck(sfnx_moe_down_f8_big(detail::base_of(A), detail::stride_of(A, sa), A.n_in, A.n_out, jobs, njobs, njobs_cap, hq, hs, out_type, out, st));
+}
+inline void moe_mm_16(const DW& A, size_t sa, const Job* jobs, const int* njobs, int njobs_max, const uint16_t* x,
+                      uint32_t out_type, void* out, void* st) {
+    ck(sfnx_moe_mm_16(detail::base_of(A), detail::stride_of(A, sa), A.type, A.n_in, A.n_out, jobs, njobs, njobs_max, x, out_type, out, st));
+}
+inline void moe_mm_16_big(const DW& A, size_t sa, const BigJob* jobs, const int* njobs, int njobs_cap, const uint16_t* x,
+                          uint32_t out_type, void* out, void* st) {
+    ck(sfnx_moe_mm_16_big(detail::base_of(A), detail::stride_of(A, sa), A.type, A.n_in, A.n_out, jobs, njobs, njobs_cap, x, out_type, out, st));
+}
+
 static_assert(sizeof(Job) == 136 && sizeof(BigJob) == 520, "job layouts match the reference's");
 
 }  // namespace sfnx

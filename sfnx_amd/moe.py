@@ -196,6 +196,116 @@ def kernel_clock_read() -> list:
     return list(us)
 
 
+# ---------------------------------------------------------------------------------------------------- 8-bit and 16-bit experts
+_TYPE_ID = {torch.float32: _abi.F32, torch.float16: _abi.F16, torch.bfloat16: _abi.BF16}
+
+
+def _need(t, name: str, dtypes, shape=None, rows_strided: bool = False) -> None:
+    """a tensor argument: its type, its size (entries None: any), contiguous, on the current GPU"""
+    if t.dtype not in dtypes:
+        raise ValueError(f"{name}: type {t.dtype}, expected {' or '.join(str(d) for d in dtypes)}")
+    if shape is not None and (t.dim() != len(shape) or any(w is not None and w != g for g, w in zip(t.shape, shape))):
+        raise ValueError(f"{name}: shape {tuple(t.shape)}, expected {tuple('any' if w is None else w for w in shape)}")
+    if not t.is_contiguous() and not (rows_strided and t.dim() == 2 and (t.stride(1) == 1 or t.shape[1] == 1)):
+        raise ValueError(f"{name}: not contiguous")
+    if not t.is_cuda or t.get_device() != torch.cuda.current_device():
+        raise ValueError(f"{name}: not on the current GPU")
+
+
+_F8_BYTES = (torch.uint8, torch.float8_e4m3fn)
+
+
+def _need_rows(q, s, qn: str, sn: str, cols: int) -> None:
+    """8-bit rows and their scales"""
+    _need(q, qn, _F8_BYTES, (None, cols))
+    _need(s, sn, (torch.float32,), (q.shape[0], (cols + 127) // 128))
+
+
+def _need_jobs(jobs, njobs, n: int, ints: int) -> None:
+    _need(jobs, "jobs", (torch.int32,))
+    _need(njobs, "njobs", (torch.int32,))
+    if n < 0 or jobs.numel() < n * ints or njobs.numel() < 1:
+        raise ValueError("jobs: smaller than the jobs announced, or njobs empty")
+
+
+def f8_matrix_bytes(rows: int, cols: int) -> int:
+    """bytes of a matrix of the 8-bit store: e4m3 values [rows][cols], the f32 scales of its 128 x 128 blocks"""
+    return lib().sfnx_f8_matrix_bytes(rows, cols)
+
+
+def quantize_f8(x, q, s) -> None:
+    """rows of x (f32, f16 or bf16; rows may be strided) as e4m3 rows q with a scale s for each 128 values"""
+    _need(x, "x", tuple(_TYPE_ID), (None, None), rows_strided=True)
+    rows, cols = x.shape
+    _need(q, "q", _F8_BYTES, (rows, cols))
+    _need(s, "s", (torch.float32,), (rows, (cols + 127) // 128))
+    check(lib().sfnx_quantize_f8(_TYPE_ID[x.dtype], _p(x), x.stride(0) if rows > 1 else cols, rows, cols, _p(q), _p(s), _st()))
+
+
+def f8_gemm(W, rows: int, cols: int, xq, xs, out) -> None:
+    """out [C][rows] (f32, f16 or bf16; rows may be strided) = the 8-bit rows xq, xs [C][cols] times the 8-bit matrix W"""
+    _need(W, "W", (torch.uint8,))
+    if W.numel() < rows * cols + 4 * ((rows + 127) // 128) * ((cols + 127) // 128):
+        raise ValueError("W: smaller than the matrix")
+    _need_rows(xq, xs, "xq", "xs", cols)
+    _need(out, "out", tuple(_TYPE_ID), (xq.shape[0], rows), rows_strided=True)
+    check(lib().sfnx_f8_gemm(_p(W), rows, cols, _p(xq), _p(xs), xq.shape[0], _TYPE_ID[out.dtype], _p(out),
+                             out.stride(0) if out.shape[0] > 1 else rows, _st()))
+
+
+def moe_gate_up_swiglu_f8(A, sa, n_in, ff, jobs, njobs, njobs_max, xq, xs, h) -> None:
+    """a window's h rows (f32) = silu(gate) * up of the 8-bit rows xq, xs, over jobs"""
+    _need_jobs(jobs, njobs, njobs_max, JOB_INTS)
+    _need_rows(xq, xs, "xq", "xs", n_in)
+    _need(h, "h", (torch.float32,), (None, ff))
+    check(lib().sfnx_moe_gate_up_swiglu_f8(_p(A), sa, n_in, ff, _p(jobs), _p(njobs), njobs_max, _p(xq), _p(xs), _p(h), _st()))
+
+
+def moe_down_f8(A, sa, n_in, n_out, jobs, njobs, njobs_max, h, out) -> None:
+    """a window's out rows = the experts' rows times h's (f32, quantized in the call), over jobs"""
+    _need_jobs(jobs, njobs, njobs_max, JOB_INTS)
+    _need(h, "h", (torch.float32,), (None, n_in))
+    _need(out, "out", tuple(_TYPE_ID), (None, n_out))
+    check(lib().sfnx_moe_down_f8(_p(A), sa, n_in, n_out, _p(jobs), _p(njobs), njobs_max, _p(h), _TYPE_ID[out.dtype], _p(out), _st()))
+
+
+def moe_gate_up_swiglu_f8_big(A, sa, n_in, ff, jobs, njobs, njobs_cap, xq, xs, hq, hs) -> None:
+    """a chunk's 8-bit h rows hq, hs = silu(gate) * up of the 8-bit rows xq, xs, over BigJobs"""
+    _need_jobs(jobs, njobs, njobs_cap, BIGJOB_INTS)
+    _need_rows(xq, xs, "xq", "xs", n_in)
+    _need_rows(hq, hs, "hq", "hs", ff)
+    check(lib().sfnx_moe_gate_up_swiglu_f8_big(_p(A), sa, n_in, ff, _p(jobs), _p(njobs), njobs_cap, _p(xq), _p(xs), _p(hq),
+                                               _p(hs), _st()))
+
+
+def moe_down_f8_big(A, sa, n_in, n_out, jobs, njobs, njobs_cap, hq, hs, out) -> None:
+    """a chunk's out rows = the experts' rows times the 8-bit rows hq, hs, over BigJobs"""
+    _need_jobs(jobs, njobs, njobs_cap, BIGJOB_INTS)
+    _need_rows(hq, hs, "hq", "hs", n_in)
+    _need(out, "out", tuple(_TYPE_ID), (None, n_out))
+    check(lib().sfnx_moe_down_f8_big(_p(A), sa, n_in, n_out, _p(jobs), _p(njobs), njobs_cap, _p(hq), _p(hs),
+                                     _TYPE_ID[out.dtype], _p(out), _st()))
+
+
+def _mm_16(fn, ints, A, sa, n_in, n_out, jobs, njobs, n, x, out) -> None:
+    _need_jobs(jobs, njobs, n, ints)
+    _need(x, "x", (torch.float16, torch.bfloat16), (None, n_in))
+    _need(out, "out", tuple(_TYPE_ID), (None, n_out))
+    if sa != 0 and A.dtype != x.dtype:
+        raise ValueError("A: another type than x")
+    check(fn(_p(A), sa, _TYPE_ID[x.dtype], n_in, n_out, _p(jobs), _p(njobs), n, _p(x), _TYPE_ID[out.dtype], _p(out), _st()))
+
+
+def moe_mm_16(A, sa, n_in, n_out, jobs, njobs, njobs_max, x, out) -> None:
+    """a window's out rows = the f16 or bf16 experts' rows times x's (of their type), over jobs"""
+    _mm_16(lib().sfnx_moe_mm_16, JOB_INTS, A, sa, n_in, n_out, jobs, njobs, njobs_max, x, out)
+
+
+def moe_mm_16_big(A, sa, n_in, n_out, jobs, njobs, njobs_cap, x, out) -> None:
+    """a chunk's out rows = the f16 or bf16 experts' rows times x's (of their type), over BigJobs"""
+    _mm_16(lib().sfnx_moe_mm_16_big, BIGJOB_INTS, A, sa, n_in, n_out, jobs, njobs, njobs_cap, x, out)
+
+
 # ---------------------------------------------------------------------------------------------------- a layer
 @dataclass
 class LayerShape:
@@ -478,6 +588,119 @@ def prefill_layer_q8(L: MoeLayer, x: torch.Tensor, y: torch.Tensor, b: PrefillBu
     if s.sh_q8s:   # the reference's shared expert is the f16 dense path on this path too (src/prefill.cu:1173-1177)
         to_f16(x, b.xh)
         prefill_shared(L, b)
+    moe_combine(b.part, b.topw, b.topi, b.logits, y, s.E, s.K, s.shared)
+
+
+# ---------------------------------------------------------------------------------------------------- layers of 8- and 16-bit experts
+class MoeLayerF8:
+    """One MoE layer whose experts are block-scaled 8-bit floating point, resident in HBM: gu_w [experts][stride] the
+    matrices of [gate ; up] rows [2 ff][H], dn_w the down matrices [H][ff], both in the 8-bit store's form
+    (f8_matrix_bytes); W the router [E + 1][H].  The shared expert, when there is one, is expert E of the stores.  Of the
+    shape, H, E, K, ff and shared count."""
+
+    def __init__(self, shape: LayerShape, W: torch.Tensor, gu_w: torch.Tensor, dn_w: torch.Tensor):
+        s, n = shape, shape.E + (1 if shape.shared else 0)
+        _need(W, "W", (torch.float32,), (s.E + 1, s.H))
+        for name, t, rows, cols in (("gu_w", gu_w, 2 * s.ff, s.H), ("dn_w", dn_w, s.H, s.ff)):
+            _need(t, name, (torch.uint8,), (n, None))
+            if t.shape[1] < f8_matrix_bytes(rows, cols) or t.shape[1] % 16:
+                raise ValueError(f"{name}: rows of {t.shape[1]} bytes, expected at least {f8_matrix_bytes(rows, cols)}, a multiple of 16")
+        self.s, self.W, self.gu_w, self.dn_w = s, W, gu_w, dn_w
+        self.gu_stride, self.dn_stride = gu_w.shape[1], dn_w.shape[1]
+
+    @staticmethod
+    def store(q: torch.Tensor, scales: torch.Tensor) -> torch.Tensor:
+        """the 8-bit store of matrices as model files hold them: e4m3 values [n][rows][cols] and the f32 scales of their
+        128 x 128 blocks [n][ceil(rows / 128)][ceil(cols / 128)]"""
+        n, rows, cols = q.shape
+        if q.dtype not in _F8_BYTES or scales.dtype != torch.float32 or scales.shape != (n, (rows + 127) // 128, (cols + 127) // 128):
+            raise ValueError("store: e4m3 values [n][rows][cols] and f32 scales [n][ceil(rows / 128)][ceil(cols / 128)]")
+        out = torch.zeros((n, f8_matrix_bytes(rows, cols)), dtype=torch.uint8, device=q.device)
+        out[:, : rows * cols] = q.reshape(n, -1).view(torch.uint8)
+        out[:, rows * cols: rows * cols + 4 * scales[0].numel()] = scales.contiguous().view(n, -1).view(torch.uint8)
+        return out
+
+
+class MoeLayer16:
+    """One MoE layer whose experts are f16 matrices: gu_w [experts][2 ff][H], dn_w [experts][H][ff]; the rest as MoeLayerF8"""
+
+    def __init__(self, shape: LayerShape, W: torch.Tensor, gu_w: torch.Tensor, dn_w: torch.Tensor):
+        s, n = shape, shape.E + (1 if shape.shared else 0)
+        _need(W, "W", (torch.float32,), (s.E + 1, s.H))
+        _need(gu_w, "gu_w", (torch.float16,), (n, 2 * s.ff, s.H))
+        _need(dn_w, "dn_w", (torch.float16,), (n, s.H, s.ff))
+        self.s, self.W, self.gu_w, self.dn_w = s, W, gu_w, dn_w
+        self.gu_stride, self.dn_stride = 4 * s.ff * s.H, 2 * s.H * s.ff
+
+
+class FloatBuffers:
+    """What a window (T <= 16) or a prompt chunk of T tokens needs beside a layer of 8-bit or f16 experts"""
+
+    def __init__(self, shape: LayerShape, T: int, device="cuda"):
+        s, big = shape, T > _abi.MAXT
+        P = T * s.K
+        NP = P + (T if s.shared else 0)
+        self.T, self.big = T, big
+        self.cap = P // PF_JOB + s.E + (T + PF_JOB - 1) // PF_JOB + 1 if big else P + 1
+        i32 = dict(dtype=torch.int32, device=device)
+        f32 = dict(dtype=torch.float32, device=device)
+        u8 = dict(dtype=torch.uint8, device=device)
+        f16 = dict(dtype=torch.float16, device=device)
+        self.logits = torch.empty((T, s.E + 1), **f32)
+        self.topi, self.topw = torch.empty((T, s.K), **i32), torch.empty((T, s.K), **f32)
+        self.cnt, self.jbase = torch.zeros(s.E, **i32), torch.zeros(s.E, **i32)
+        ints = BIGJOB_INTS if big else JOB_INTS
+        self.jobs_gu, self.jobs_dn = torch.zeros(self.cap * ints, **i32), torch.zeros(self.cap * ints, **i32)
+        self.njobs = torch.zeros(2, **i32)
+        self.xq, self.xs = torch.empty((T, s.H), **u8), torch.empty((T, (s.H + 127) // 128), **f32)
+        self.hq, self.hs = torch.empty((NP, s.ff), **u8), torch.empty((NP, (s.ff + 127) // 128), **f32)
+        self.h = torch.zeros((NP, s.ff), **f32)
+        self.xh, self.h16 = torch.empty((T, s.H), **f16), torch.zeros((NP, s.ff), **f16)
+        self.gu = torch.zeros((NP, 2 * s.ff), **f32)
+        self.part = torch.zeros((NP, s.H), **f32)
+
+
+def _route(L, x, b) -> None:
+    s = L.s
+    if b.big:
+        router_logits(L.W, x, b.logits)
+        pf_route(b.logits, b.topi, b.topw, b.cnt, b.jbase, b.jobs_gu, b.jobs_dn, b.njobs, s.E, s.K, s.shared)
+    else:
+        router_route(L.W, x, b.logits, b.topi, b.topw, b.jobs_gu, b.jobs_dn, b.njobs, s.E, s.K, s.shared)
+
+
+def _need_call(L, x, y, b) -> None:
+    _need(x, "x", (torch.float32,), (b.T, L.s.H))
+    _need(y, "y", (torch.float32,), (b.T, L.s.H))
+
+
+def layer_f8(L: MoeLayerF8, x: torch.Tensor, y: torch.Tensor, b: FloatBuffers) -> None:
+    """A decode window or a prompt chunk (b's tokens) through a layer of 8-bit experts: routing, the activations quantized,
+    gate|up with SwiGLU, down, the combine"""
+    s = L.s
+    _need_call(L, x, y, b)
+    _route(L, x, b)
+    quantize_f8(x, b.xq, b.xs)
+    if b.big:
+        moe_gate_up_swiglu_f8_big(L.gu_w, L.gu_stride, s.H, s.ff, b.jobs_gu, b.njobs, b.cap, b.xq, b.xs, b.hq, b.hs)
+        moe_down_f8_big(L.dn_w, L.dn_stride, s.ff, s.H, b.jobs_dn, b.njobs, b.cap, b.hq, b.hs, b.part)
+    else:
+        moe_gate_up_swiglu_f8(L.gu_w, L.gu_stride, s.H, s.ff, b.jobs_gu, b.njobs, b.cap, b.xq, b.xs, b.h)
+        moe_down_f8(L.dn_w, L.dn_stride, s.ff, s.H, b.jobs_dn, b.njobs, b.cap, b.h, b.part)
+    moe_combine(b.part, b.topw, b.topi, b.logits, y, s.E, s.K, s.shared)
+
+
+def layer_16(L: MoeLayer16, x: torch.Tensor, y: torch.Tensor, b: FloatBuffers) -> None:
+    """A decode window or a prompt chunk through a layer of f16 experts: routing, f16 activations, gate|up, SwiGLU to f16,
+    down, the combine"""
+    s = L.s
+    _need_call(L, x, y, b)
+    _route(L, x, b)
+    to_f16(x, b.xh)
+    mm = moe_mm_16_big if b.big else moe_mm_16
+    mm(L.gu_w, L.gu_stride, s.H, 2 * s.ff, b.jobs_gu, b.njobs, b.cap, b.xh, b.gu)
+    swiglu_h16(b.gu, b.h16, s.ff)
+    mm(L.dn_w, L.dn_stride, s.ff, s.H, b.jobs_dn, b.njobs, b.cap, b.h16, b.part)
     moe_combine(b.part, b.topw, b.topi, b.logits, y, s.E, s.K, s.shared)
 
 
