@@ -1,11 +1,8 @@
 // Experts and dense matrices in block-scaled 8-bit floating point (e4m3 values, an f32 scale for each 128 x 128 block of a
 // matrix and for each 128 values of an activation row): the activation quantizer, the dense product, and the products
 // grouped by expert over the routers' jobs.
-#include <algorithm>
-#include <type_traits>
-
 #include "mm_few.hpp"
-#include "mm_tile.hpp"
+#include "mm_tiles.hpp"
 
 namespace sfnx {
 namespace {
@@ -113,8 +110,8 @@ extern "C" int sfnx_f8_gemm(const void* W, int rows, int cols, const uint8_t* xq
         Args a{(const uint8_t*) W, sfnx_f8_matrix_bytes(rows, cols), cols, rows, nullptr, nullptr, C, xq, xs, out, nullptr, out_type, ldo,
                vec_ok(out, out_type, ldo)};
         if (C <= FEW_M) launch_few<F8X, STORE, false>(a, 1, stream_of(st));
-        else if (out_type == SFNX_F32) launch_tile<F8X, STORE>(a, (C + TL_BM - 1) / TL_BM, stream_of(st));
-        else launch_tile<F8, STORE>(a, (C + TL_BM - 1) / TL_BM, stream_of(st));
+        else if (out_type == SFNX_F32) launch_tiles<F8X, STORE>(a, (C + BM1 - 1) / BM1, stream_of(st));
+        else launch_tiles<F8, STORE>(a, (C + BM1 - 1) / BM1, stream_of(st));
     });
 }
 
@@ -159,7 +156,7 @@ extern "C" int sfnx_moe_gate_up_swiglu_f8_big(const void* A, size_t sa, int n_in
         check_f8_rows(xq, xs);
         check_f8_rows(hq, hs);
         Args a{(const uint8_t*) A, sa, n_in, 2 * ff, jobs, njobs, 0, xq, xs, hq, hs, SFNX_F32, ff, 1};
-        launch_tile<F8X, SWIGLU>(a, njobs_cap, stream_of(st));
+        launch_tiles<F8X, SWIGLU>(a, njobs_cap, stream_of(st));
     });
 }
 
@@ -172,7 +169,7 @@ extern "C" int sfnx_moe_down_f8_big(const void* A, size_t sa, int n_in, int n_ou
         check_f8_rows(hq, hs);
         check_out(out, out_type);
         Args a{(const uint8_t*) A, sa, n_in, n_out, jobs, njobs, 0, hq, hs, out, nullptr, out_type, n_out, vec_ok(out, out_type, n_out)};
-        if (out_type == SFNX_F32) launch_tile<F8X, STORE>(a, njobs_cap, stream_of(st));
-        else launch_tile<F8, STORE>(a, njobs_cap, stream_of(st));
+        if (out_type == SFNX_F32) launch_tiles<F8X, STORE>(a, njobs_cap, stream_of(st));
+        else launch_tiles<F8, STORE>(a, njobs_cap, stream_of(st));
     });
 }

@@ -14,6 +14,9 @@
 // serves outputs kept in 32 bits, the scales of quantized ones, and products of few rows, which wait for the weights anyway.
 #pragma once
 
+#include <algorithm>
+#include <type_traits>
+
 #include "common.hpp"
 
 namespace sfnx {
@@ -29,6 +32,7 @@ typedef _Float16 half2f __attribute__((ext_vector_type(2)));
 enum Elem { F8, F8X, F16, BF16 };
 template <Elem EL> constexpr bool IS8 = EL == F8 || EL == F8X;
 template <Elem EL> constexpr int ESZ = IS8<EL> ? 1 : 2;   // bytes of a weight or activation
+constexpr int CUS = 256;                                   // compute units
 constexpr int STEP = 128;                                  // bytes of a row in a K step
 constexpr int BLK = 128;                                   // values of a scale block
 constexpr float F8_MAX = 448.f, F8_INV = 1.f / 448.f, S_MIN = 0x1p-126f;
@@ -153,6 +157,7 @@ struct Args {
     uint32_t out_type;
     int ldo;
     int vec;                 // four consecutive outputs at a multiple of 4 are aligned to their size
+    int slices = 0;          // of a matrix, 256 rows each
 };
 
 // workgroups of a launch: a job's slices for each job; a launch holds fewer than 2^32 threads
@@ -163,6 +168,20 @@ inline unsigned grid_of(int slices, int jobs, int threads) {
 
 // an address that is always readable, for the lanes past a row's end
 static __device__ const uint4 ZERO16 = {0, 0, 0, 0};
+
+// a pointer that all lanes share, in scalar registers
+__device__ __forceinline__ const uint8_t* uniform_ptr(const uint8_t* p) {
+    const uint64_t u = (uint64_t) p;
+    const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t) u), hi = __builtin_amdgcn_readfirstlane((uint32_t) (u >> 32));
+    return (const uint8_t*) ((uint64_t) hi << 32 | lo);
+}
+
+// lane l's 16 bytes at base + off to lds + 16 l (lds_copy_async with a uniform base and a 32-bit offset)
+__device__ __forceinline__ void lds_copy_async16(const uint8_t* base, uint32_t off, const void* lds) {
+    const uint32_t m0 = __builtin_amdgcn_readfirstlane(
+        (uint32_t) reinterpret_cast<uintptr_t>((const __attribute__((address_space(3))) void*) lds));
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(m0) : "memory", "m0");
+}
 
 enum Mode { STORE, SWIGLU };
 

@@ -88,7 +88,7 @@ def test_quantize_strided_rows_and_nothing():
 
 # ------------------------------------------------------------------------------------------------ dense
 GEMM = [(1, 16, 1), (1, 2048, 1024), (2, 128, 17), (5, 144, 130), (16, 2000, 257), (17, 256, 33), (63, 640, 300), (64, 1024, 256),
-        (65, 1040, 513), (130, 2048, 129), (200, 4096, 640), (300, 48, 1301)]
+        (65, 1040, 513), (130, 2048, 129), (200, 4096, 640), (300, 48, 1301), (2000, 272, 4357)]
 
 
 @pytest.mark.parametrize("t", sorted(OUT))
