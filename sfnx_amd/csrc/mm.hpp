@@ -59,21 +59,29 @@ template <Elem EL> __device__ __forceinline__ Operand<EL> operand(const Frag& f)
     else return f;
 }
 
+// the product of a K step of e4m3 values, without its scales
+template <Elem EL> __device__ __forceinline__ float4v step_dot(const Operand<EL>& w, const Operand<EL>& x) {
+    float4v d = {};
+    if constexpr (EL == F8) {
+        const int8v a = {(int) w.lo.x, (int) w.lo.y, (int) w.lo.z, (int) w.lo.w, (int) w.hi.x, (int) w.hi.y, (int) w.hi.z, (int) w.hi.w};
+        const int8v b = {(int) x.lo.x, (int) x.lo.y, (int) x.lo.z, (int) x.lo.w, (int) x.hi.x, (int) x.hi.y, (int) x.hi.z, (int) x.hi.w};
+        d = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, d, 0, 0, 0, 0, 0, 0);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) d = __builtin_amdgcn_mfma_f32_16x16x32_f16(w.h[i], x.h[i], d, 0, 0, 0);
+    }
+    return d;
+}
+__device__ __forceinline__ float4v scaled_add(float4v d, float s, float4v acc) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) acc[i] = fmaf(d[i], s, acc[i]);
+    return acc;
+}
+
 // acc += W . x over one K step; s: the product of the step's scales (e4m3 only)
 template <Elem EL> __device__ __forceinline__ float4v step_mma(const Operand<EL>& w, const Operand<EL>& x, float4v acc, float s) {
     if constexpr (IS8<EL>) {
-        float4v d = {};
-        if constexpr (EL == F8) {
-            const int8v a = {(int) w.lo.x, (int) w.lo.y, (int) w.lo.z, (int) w.lo.w, (int) w.hi.x, (int) w.hi.y, (int) w.hi.z, (int) w.hi.w};
-            const int8v b = {(int) x.lo.x, (int) x.lo.y, (int) x.lo.z, (int) x.lo.w, (int) x.hi.x, (int) x.hi.y, (int) x.hi.z, (int) x.hi.w};
-            d = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, d, 0, 0, 0, 0, 0, 0);
-        } else {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) d = __builtin_amdgcn_mfma_f32_16x16x32_f16(w.h[i], x.h[i], d, 0, 0, 0);
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) acc[i] = fmaf(d[i], s, acc[i]);
-        return acc;
+        return scaled_add(step_dot<EL>(w, x), s, acc);
     } else if constexpr (EL == F16) {
         acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8v, w.lo), __builtin_bit_cast(half8v, x.lo), acc, 0, 0, 0);
         return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8v, w.hi), __builtin_bit_cast(half8v, x.hi), acc, 0, 0, 0);
@@ -176,11 +184,21 @@ __device__ __forceinline__ const uint8_t* uniform_ptr(const uint8_t* p) {
     return (const uint8_t*) ((uint64_t) hi << 32 | lo);
 }
 
-// lane l's 16 bytes at base + off to lds + 16 l (lds_copy_async with a uniform base and a 32-bit offset)
-__device__ __forceinline__ void lds_copy_async16(const uint8_t* base, uint32_t off, const void* lds) {
-    const uint32_t m0 = __builtin_amdgcn_readfirstlane(
-        (uint32_t) reinterpret_cast<uintptr_t>((const __attribute__((address_space(3))) void*) lds));
-    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(m0) : "memory", "m0");
+// Copies to LDS that a caller spreads among its matrix instructions: issued all at once they hold up the wavefront until the
+// address unit has taken them (about 35 cycles each).  As lds_copy_async, but no compiler barrier, so LDS reads of other
+// places move across them; the order against vm_wait and lds_barrier stays.  lds: wave-uniform; lane l's bytes land at lds + 16 l
+// (copy4: 4 l).  copy16's address is a uniform base and a lane's 32-bit offset, or a lane's pointer.
+__device__ __forceinline__ uint32_t lds_address(const void* lds) {
+    return __builtin_amdgcn_readfirstlane((uint32_t) reinterpret_cast<uintptr_t>((const __attribute__((address_space(3))) void*) lds));
+}
+__device__ __forceinline__ void copy16(const uint8_t* base, uint32_t off, const void* lds) {
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(lds_address(lds)) : "m0");
+}
+__device__ __forceinline__ void copy16(const uint8_t* p, const void* lds) {
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(p), "s"(lds_address(lds)) : "m0");
+}
+__device__ __forceinline__ void copy4(const void* p, const void* lds) {
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(p), "s"(lds_address(lds)) : "m0");
 }
 
 enum Mode { STORE, SWIGLU };

@@ -32,7 +32,7 @@ static_assert(T_LDS + 64 <= 160 * 1024 && 4 * WINDOW <= SG_LIST && 2 * BMG * 4 +
 // an expert's weights come from HBM once for them; xg = 4, or 1 where there are too few to use all XCDs evenly.  false: no
 // such group
 __device__ __forceinline__ bool tile_at(int b, int nsl, int n, int& sl, int& i) {
-    const int xg = n >= 256 ? 4 : 1;
+    const int xg = n >= 64 ? 4 : 1;
     const int x = b % XCDS, k = b / XCDS, m = k / nsl;
     sl = k % nsl;
     i = xg * (XCDS * (m / xg) + x) + m % xg;
@@ -167,18 +167,17 @@ template <Elem EL, Mode MODE> __device__ __forceinline__ void stream_tiles(const
         const uint8_t* x = xsrc + k;
         if (k + STEP <= rb) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) lds_copy_async16(uniform_ptr(wbase + k), woff[i], buf + (32 * wave + 8 * i) * STEP);
+            for (int i = 0; i < 4; ++i) copy16(uniform_ptr(wbase + k), woff[i], buf + (32 * wave + 8 * i) * STEP);
         } else {   // zero past the rows' end
             const bool in = k + 16 * p8 < rb;
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-                lds_copy_async<16>(in ? wbase + k + woff[i] : (const uint8_t*) &ZERO16, buf + (32 * wave + 8 * i) * STEP);
+            for (int i = 0; i < 4; ++i) copy16(in ? wbase + k + woff[i] : (const uint8_t*) &ZERO16, buf + (32 * wave + 8 * i) * STEP);
             if (!in) x = (const uint8_t*) &ZERO16;
         }
-        lds_copy_async<16>(x, buf + S::X + 8 * wave * STEP);
+        copy16(x, buf + S::X + 8 * wave * STEP);
         if constexpr (IS8<EL>) {   // every wavefront copies them all: the same values, and each counts the same requests
-            lds_copy_async<4>(xs_src + ps, buf + S::XS);
-            lds_copy_async<4>(ws_src + ps, buf + S::WS);
+            copy4(xs_src + ps, buf + S::XS);
+            copy4(ws_src + ps, buf + S::WS);
         }
         ++ps;
         return true;
@@ -265,7 +264,7 @@ template <Elem EL, Mode MODE> __device__ __forceinline__ void group_tile(const A
     };
     auto act_row = [&](int m) {
         const int n = rows_of(m / BM1);
-        if (n == 0) return dense ? 0 : -1;
+        if (n == 0) return 0;   // some row: a job that the group does not have
         const int mm = min(m % BM1, n - 1);
         return dense ? BM1 * (j0 + m / BM1) + mm : jobs[m / BM1].y[mm];
     };
@@ -281,56 +280,104 @@ template <Elem EL, Mode MODE> __device__ __forceinline__ void group_tile(const A
     const float *xs_src = nullptr, *ws_src = nullptr;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        woff[i] = (uint32_t) weight_row<MODE, 8>(a, sl, 32 * wave + 8 * i + r8) * (uint32_t) rb + 16 * p8;
-        const int y = act_row(32 * wave + 8 * i + r8);
-        xsrc[i] = y < 0 ? nullptr : a.x + (size_t) y * rb + 16 * p8;   // null: a job that the group does not have
+        woff[i] = (uint32_t) weight_row<MODE, 8>(a, sl, 32 * wave + 8 * i + r8) * (uint32_t) rb;
+        xsrc[i] = a.x + (size_t) act_row(32 * wave + 8 * i + r8) * rb;
     }
     if constexpr (IS8<EL>) {
-        xs_src = a.xs + (size_t) max(0, act_row(64 * wm + lane)) * nb;
+        xs_src = a.xs + (size_t) act_row(64 * wm + lane) * nb;
         ws_src = scales_of(mat, a.n_out, a.n_in) + (size_t) (weight_row<MODE, 8>(a, sl, 16 * r) / BLK) * nb;
     }
-    auto request = [&](int s, uint8_t* buf) {
-        const int k = s * STEP;
-        const bool whole = k + STEP <= rb, in = k + 16 * p8 < rb;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            if (whole) lds_copy_async16(uniform_ptr(mat + k), woff[i], buf + (32 * wave + 8 * i) * STEP);
-            else lds_copy_async<16>(in ? mat + k + woff[i] : (const uint8_t*) &ZERO16, buf + (32 * wave + 8 * i) * STEP);
-        }
-        if (n > 0)   // wavefronts 2 w and 2 w + 1 copy job w's rows
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                lds_copy_async<16>(in ? xsrc[i] + k : (const uint8_t*) &ZERO16, buf + S::X + (32 * wave + 8 * i) * STEP);
+    // the u-th eighth of step s into a stage; past the rows' end their last piece (see below), past the last step that again
+    auto copy = [&](int u, int s, uint8_t* buf) {
+        s = min(s, steps - 1);
+        const uint32_t k = (uint32_t) min(s * STEP + 16 * p8, rb - 16);
+        const int i = u % 4;
+        if (u < 4) copy16(mat, woff[i] + k, buf + (32 * wave + 8 * i) * STEP);
+        else copy16(xsrc[i] + k, buf + S::X + (32 * wave + 8 * i) * STEP);
         if constexpr (IS8<EL>) {
-            lds_copy_async<4>(xs_src + s, buf + S::XS + 256 * wm);
-            lds_copy_async<4>(ws_src + s, buf + S::WS);
+            if (u == 2) copy4(xs_src + s, buf + S::XS + 256 * wm);
+            if (u == 3) copy4(ws_src + s, buf + S::WS);
         }
+        asm volatile("" ::: "memory");   // the LDS reads stay where they are: all at once they would not fit the registers
     };
     float4v acc[8][4] = {};
     lds_barrier();   // the tile before is done with LDS
-    request(0, lds);
+#pragma unroll
+    for (int u = 0; u < 8; ++u) copy(u, 0, lds);
     for (int s = 0; s < steps; ++s) {
-        const uint8_t* buf = lds + (s & 1) * S::SIZE;
+        uint8_t* buf = lds + (s & 1) * S::SIZE;
+        uint8_t* to = lds + ((s + 1) & 1) * S::SIZE;
         vm_wait<0>();
-        lds_barrier();   // every wavefront's copies of this stage landed, and every wavefront is past the one before
-        if (s + 1 < steps) request(s + 1, lds + ((s + 1) & 1) * S::SIZE);
-        if (n == 0) continue;
-        Operand<EL> x[4];
-        float xs[4];
+        if (s == steps - 1 && rb % STEP) {   // zero past the rows' end, whatever lies there: each wavefront in what it copied
+            const int k = s * STEP + 16 * p8;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            x[j] = operand<EL>(lds_frag(buf + S::X, 64 * wm + 16 * j + r, q));
-            if constexpr (IS8<EL>) xs[j] = reinterpret_cast<const float*>(buf + S::XS)[64 * wm + 16 * j + r];
+            for (int i = 0; i < 4; ++i)
+                if (k >= rb) {
+                    *reinterpret_cast<uint4*>(buf + (32 * wave + 8 * i) * STEP + 16 * lane) = uint4{};
+                    *reinterpret_cast<uint4*>(buf + S::X + (32 * wave + 8 * i) * STEP + 16 * lane) = uint4{};
+                }
         }
+        lds_barrier();   // every wavefront's copies of this stage landed, and every wavefront is past the one before
+        if constexpr (EL == F8) {
+            // the products of a weight tile are added while the next tile's are made
+            Frag x[4];
+            float xs[4];
 #pragma unroll
-        for (int u = 0; u < 8; ++u) {
-            const Operand<EL> w = operand<EL>(lds_frag(buf, 128 * wn + 16 * u + r, q));
-            float ws = 1.f;
-            if constexpr (IS8<EL>) ws = reinterpret_cast<const float*>(buf + S::WS)[8 * wn + u];
+            for (int j = 0; j < 4; ++j) {
+                x[j] = lds_frag(buf + S::X, 64 * wm + 16 * j + r, q);
+                xs[j] = reinterpret_cast<const float*>(buf + S::XS)[64 * wm + 16 * j + r];
+            }
+            Frag w = lds_frag(buf, 128 * wn + r, q);
+            float ws = reinterpret_cast<const float*>(buf + S::WS)[8 * wn];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) acc[u][j] = step_mma<EL>(w, x[j], acc[u][j], IS8<EL> ? xs[j] * ws : 1.f);
+            for (int u = 0; u < 8; ++u) {
+                float4v d[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) d[j] = step_dot<EL>(w, x[j]);
+                const float sc = ws;
+                if (u < 7) {
+                    w = lds_frag(buf, 128 * wn + 16 * (u + 1) + r, q);
+                    ws = reinterpret_cast<const float*>(buf + S::WS)[8 * wn + u + 1];
+                }
+                copy(u, s + 1, to);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) acc[u][j] = scaled_add(d[j], xs[j] * sc, acc[u][j]);
+            }
+        } else if constexpr (EL == F8X) {
+            // converted, 64 activation rows are too many registers beside the sums: half of them at a time
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                FragX x[2];
+                float xs[2];
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    x[j] = operand<EL>(lds_frag(buf + S::X, 64 * wm + 32 * h + 16 * j + r, q));
+                    xs[j] = reinterpret_cast<const float*>(buf + S::XS)[64 * wm + 32 * h + 16 * j + r];
+                }
+#pragma unroll
+                for (int u = 0; u < 8; ++u) {
+                    const FragX w = operand<EL>(lds_frag(buf, 128 * wn + 16 * u + r, q));
+                    const float ws = reinterpret_cast<const float*>(buf + S::WS)[8 * wn + u];
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) acc[u][2 * h + j] = step_mma<EL>(w, x[j], acc[u][2 * h + j], xs[j] * ws);
+                    if (u % 2 == 0) copy(4 * h + u / 2, s + 1, to);
+                    else asm volatile("" ::: "memory");
+                }
+            }
+        } else {
+            Frag x[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) x[j] = lds_frag(buf + S::X, 64 * wm + 16 * j + r, q);
+#pragma unroll
+            for (int u = 0; u < 8; ++u) {
+                const Frag w = lds_frag(buf, 128 * wn + 16 * u + r, q);
+                copy(u, s + 1, to);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) acc[u][j] = step_mma<EL>(w, x[j], acc[u][j], 1.f);
+            }
         }
     }
+    vm_wait<0>();   // the copies past the end
     if constexpr (MODE == STORE) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
