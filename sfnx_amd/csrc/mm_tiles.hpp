@@ -298,7 +298,16 @@ template <Elem EL, Mode MODE> __device__ __forceinline__ void group_tile(const A
             if (u == 2) copy4(xs_src + s, buf + S::XS + 256 * wm);
             if (u == 3) copy4(ws_src + s, buf + S::WS);
         }
-        asm volatile("" ::: "memory");   // the LDS reads stay where they are: all at once they would not fit the registers
+    };
+    auto fence = [] { asm volatile("" ::: "memory"); };   // LDS reads stay where they are: all at once they would not fit the registers
+    // what a wavefront copies of the next step beside its u-th weight tile (of 8): all of it in the first half of the step, so
+    // that it is there at the step's end, but not at once
+    auto ahead = [&](int u, int s, uint8_t* buf) {
+        if (u < 4) {
+            copy(2 * u, s, buf);
+            copy(2 * u + 1, s, buf);
+        }
+        fence();
     };
     float4v acc[8][4] = {};
     lds_barrier();   // the tile before is done with LDS
@@ -339,7 +348,7 @@ template <Elem EL, Mode MODE> __device__ __forceinline__ void group_tile(const A
                     w = lds_frag(buf, 128 * wn + 16 * (u + 1) + r, q);
                     ws = reinterpret_cast<const float*>(buf + S::WS)[8 * wn + u + 1];
                 }
-                copy(u, s + 1, to);
+                ahead(u, s + 1, to);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) acc[u][j] = scaled_add(d[j], xs[j] * sc, acc[u][j]);
             }
@@ -360,8 +369,8 @@ template <Elem EL, Mode MODE> __device__ __forceinline__ void group_tile(const A
                     const float ws = reinterpret_cast<const float*>(buf + S::WS)[8 * wn + u];
 #pragma unroll
                     for (int j = 0; j < 2; ++j) acc[u][2 * h + j] = step_mma<EL>(w, x[j], acc[u][2 * h + j], xs[j] * ws);
-                    if (u % 2 == 0) copy(4 * h + u / 2, s + 1, to);
-                    else asm volatile("" ::: "memory");
+                    if (h == 0) copy(u, s + 1, to);
+                    fence();
                 }
             }
         } else {
@@ -371,7 +380,7 @@ template <Elem EL, Mode MODE> __device__ __forceinline__ void group_tile(const A
 #pragma unroll
             for (int u = 0; u < 8; ++u) {
                 const Frag w = lds_frag(buf, 128 * wn + 16 * u + r, q);
-                copy(u, s + 1, to);
+                ahead(u, s + 1, to);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) acc[u][j] = step_mma<EL>(w, x[j], acc[u][j], 1.f);
             }

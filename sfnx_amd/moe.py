@@ -19,8 +19,16 @@ def _p(t):
     return None if t is None else t.data_ptr()
 
 
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+_device = getattr(torch._C, "_cuda_getDevice", None)
+
+
 def _st():
-    return torch.cuda.current_stream().cuda_stream
+    """torch's current stream on the current GPU; its number without a Stream object around it, 0.2 us for 2.8 (a small
+    call's launch is 4)"""
+    if _raw_stream is None or _device is None:
+        return torch.cuda.current_stream().cuda_stream
+    return _raw_stream(_device())
 
 
 def row_bytes(wtype: int, cols: int) -> int:
@@ -212,20 +220,45 @@ def _need(t, name: str, dtypes, shape=None, rows_strided: bool = False) -> None:
         raise ValueError(f"{name}: not on the current GPU")
 
 
+def _fine(t, dtypes, shape, dev) -> bool:
+    """_need's usual case at a third of its time (a shape without None); where it is false, _need says why or allows it"""
+    return t.dtype in dtypes and t.shape == shape and t.get_device() == dev and t.is_contiguous()
+
+
 _F8_BYTES = (torch.uint8, torch.float8_e4m3fn)
+_F32, _I32 = (torch.float32,), (torch.int32,)
 
 
-def _need_rows(q, s, qn: str, sn: str, cols: int) -> None:
+def _need_rows(q, s, qn: str, sn: str, cols: int, dev) -> None:
     """8-bit rows and their scales"""
-    _need(q, qn, _F8_BYTES, (None, cols))
-    _need(s, sn, (torch.float32,), (q.shape[0], (cols + 127) // 128))
+    n = q.shape[0] if q.dim() else 0
+    if not (_fine(q, _F8_BYTES, (n, cols), dev) and _fine(s, _F32, (n, (cols + 127) // 128), dev)):
+        _need(q, qn, _F8_BYTES, (None, cols))
+        _need(s, sn, _F32, (n, (cols + 127) // 128))
 
 
-def _need_jobs(jobs, njobs, n: int, ints: int) -> None:
-    _need(jobs, "jobs", (torch.int32,))
-    _need(njobs, "njobs", (torch.int32,))
+def _need_out(t, name: str, dtypes, cols: int, dev) -> None:
+    """rows of cols values"""
+    if not _fine(t, dtypes, (t.shape[0] if t.dim() else 0, cols), dev):
+        _need(t, name, dtypes, (None, cols))
+
+
+def _need_jobs(A, jobs, njobs, n: int, ints: int, dev) -> None:
+    if not A.is_contiguous() or A.get_device() != dev:
+        _need(A, "A", (A.dtype,))
+    if not (_fine(jobs, _I32, jobs.shape, dev) and _fine(njobs, _I32, njobs.shape, dev)):
+        _need(jobs, "jobs", _I32)
+        _need(njobs, "njobs", _I32)
     if n < 0 or jobs.numel() < n * ints or njobs.numel() < 1:
         raise ValueError("jobs: smaller than the jobs announced, or njobs empty")
+
+
+def _current() -> int:
+    """the current GPU; without one no tensor is on it"""
+    try:
+        return _device() if _device is not None else torch.cuda.current_device()
+    except RuntimeError:
+        return -2
 
 
 def f8_matrix_bytes(rows: int, cols: int) -> int:
@@ -235,65 +268,81 @@ def f8_matrix_bytes(rows: int, cols: int) -> int:
 
 def quantize_f8(x, q, s) -> None:
     """rows of x (f32, f16 or bf16; rows may be strided) as e4m3 rows q with a scale s for each 128 values"""
-    _need(x, "x", tuple(_TYPE_ID), (None, None), rows_strided=True)
+    dev = _current()
+    if x.dim() != 2 or not _fine(x, _TYPE_ID, x.shape, dev):
+        _need(x, "x", tuple(_TYPE_ID), (None, None), rows_strided=True)
     rows, cols = x.shape
-    _need(q, "q", _F8_BYTES, (rows, cols))
-    _need(s, "s", (torch.float32,), (rows, (cols + 127) // 128))
-    check(lib().sfnx_quantize_f8(_TYPE_ID[x.dtype], _p(x), x.stride(0) if rows > 1 else cols, rows, cols, _p(q), _p(s), _st()))
+    if not _fine(q, _F8_BYTES, (rows, cols), dev) or not _fine(s, _F32, (rows, (cols + 127) // 128), dev):
+        _need(q, "q", _F8_BYTES, (rows, cols))
+        _need(s, "s", _F32, (rows, (cols + 127) // 128))
+    check(lib().sfnx_quantize_f8(_TYPE_ID[x.dtype], x.data_ptr(), x.stride(0) if rows > 1 else cols, rows, cols, q.data_ptr(),
+                                 s.data_ptr(), _st()))
 
 
 def f8_gemm(W, rows: int, cols: int, xq, xs, out) -> None:
     """out [C][rows] (f32, f16 or bf16; rows may be strided) = the 8-bit rows xq, xs [C][cols] times the 8-bit matrix W"""
-    _need(W, "W", (torch.uint8,))
+    dev = _current()
+    if W.dtype is not torch.uint8 or W.get_device() != dev or not W.is_contiguous():
+        _need(W, "W", (torch.uint8,))
     if W.numel() < rows * cols + 4 * ((rows + 127) // 128) * ((cols + 127) // 128):
         raise ValueError("W: smaller than the matrix")
-    _need_rows(xq, xs, "xq", "xs", cols)
-    _need(out, "out", tuple(_TYPE_ID), (xq.shape[0], rows), rows_strided=True)
-    check(lib().sfnx_f8_gemm(_p(W), rows, cols, _p(xq), _p(xs), xq.shape[0], _TYPE_ID[out.dtype], _p(out),
-                             out.stride(0) if out.shape[0] > 1 else rows, _st()))
+    _need_rows(xq, xs, "xq", "xs", cols, dev)
+    C = xq.shape[0]
+    if not _fine(out, _TYPE_ID, (C, rows), dev):
+        _need(out, "out", tuple(_TYPE_ID), (C, rows), rows_strided=True)
+    check(lib().sfnx_f8_gemm(W.data_ptr(), rows, cols, xq.data_ptr(), xs.data_ptr(), C, _TYPE_ID[out.dtype], out.data_ptr(),
+                             out.stride(0) if C > 1 else rows, _st()))
 
 
 def moe_gate_up_swiglu_f8(A, sa, n_in, ff, jobs, njobs, njobs_max, xq, xs, h) -> None:
     """a window's h rows (f32) = silu(gate) * up of the 8-bit rows xq, xs, over jobs"""
-    _need_jobs(jobs, njobs, njobs_max, JOB_INTS)
-    _need_rows(xq, xs, "xq", "xs", n_in)
-    _need(h, "h", (torch.float32,), (None, ff))
-    check(lib().sfnx_moe_gate_up_swiglu_f8(_p(A), sa, n_in, ff, _p(jobs), _p(njobs), njobs_max, _p(xq), _p(xs), _p(h), _st()))
+    dev = _current()
+    _need_jobs(A, jobs, njobs, njobs_max, JOB_INTS, dev)
+    _need_rows(xq, xs, "xq", "xs", n_in, dev)
+    _need_out(h, "h", _F32, ff, dev)
+    check(lib().sfnx_moe_gate_up_swiglu_f8(A.data_ptr(), sa, n_in, ff, jobs.data_ptr(), njobs.data_ptr(), njobs_max, xq.data_ptr(),
+                                           xs.data_ptr(), h.data_ptr(), _st()))
 
 
 def moe_down_f8(A, sa, n_in, n_out, jobs, njobs, njobs_max, h, out) -> None:
     """a window's out rows = the experts' rows times h's (f32, quantized in the call), over jobs"""
-    _need_jobs(jobs, njobs, njobs_max, JOB_INTS)
-    _need(h, "h", (torch.float32,), (None, n_in))
-    _need(out, "out", tuple(_TYPE_ID), (None, n_out))
-    check(lib().sfnx_moe_down_f8(_p(A), sa, n_in, n_out, _p(jobs), _p(njobs), njobs_max, _p(h), _TYPE_ID[out.dtype], _p(out), _st()))
+    dev = _current()
+    _need_jobs(A, jobs, njobs, njobs_max, JOB_INTS, dev)
+    _need_out(h, "h", _F32, n_in, dev)
+    _need_out(out, "out", _TYPE_ID, n_out, dev)
+    check(lib().sfnx_moe_down_f8(A.data_ptr(), sa, n_in, n_out, jobs.data_ptr(), njobs.data_ptr(), njobs_max, h.data_ptr(),
+                                 _TYPE_ID[out.dtype], out.data_ptr(), _st()))
 
 
 def moe_gate_up_swiglu_f8_big(A, sa, n_in, ff, jobs, njobs, njobs_cap, xq, xs, hq, hs) -> None:
     """a chunk's 8-bit h rows hq, hs = silu(gate) * up of the 8-bit rows xq, xs, over BigJobs"""
-    _need_jobs(jobs, njobs, njobs_cap, BIGJOB_INTS)
-    _need_rows(xq, xs, "xq", "xs", n_in)
-    _need_rows(hq, hs, "hq", "hs", ff)
-    check(lib().sfnx_moe_gate_up_swiglu_f8_big(_p(A), sa, n_in, ff, _p(jobs), _p(njobs), njobs_cap, _p(xq), _p(xs), _p(hq),
-                                               _p(hs), _st()))
+    dev = _current()
+    _need_jobs(A, jobs, njobs, njobs_cap, BIGJOB_INTS, dev)
+    _need_rows(xq, xs, "xq", "xs", n_in, dev)
+    _need_rows(hq, hs, "hq", "hs", ff, dev)
+    check(lib().sfnx_moe_gate_up_swiglu_f8_big(A.data_ptr(), sa, n_in, ff, jobs.data_ptr(), njobs.data_ptr(), njobs_cap,
+                                               xq.data_ptr(), xs.data_ptr(), hq.data_ptr(), hs.data_ptr(), _st()))
 
 
 def moe_down_f8_big(A, sa, n_in, n_out, jobs, njobs, njobs_cap, hq, hs, out) -> None:
     """a chunk's out rows = the experts' rows times the 8-bit rows hq, hs, over BigJobs"""
-    _need_jobs(jobs, njobs, njobs_cap, BIGJOB_INTS)
-    _need_rows(hq, hs, "hq", "hs", n_in)
-    _need(out, "out", tuple(_TYPE_ID), (None, n_out))
-    check(lib().sfnx_moe_down_f8_big(_p(A), sa, n_in, n_out, _p(jobs), _p(njobs), njobs_cap, _p(hq), _p(hs),
-                                     _TYPE_ID[out.dtype], _p(out), _st()))
+    dev = _current()
+    _need_jobs(A, jobs, njobs, njobs_cap, BIGJOB_INTS, dev)
+    _need_rows(hq, hs, "hq", "hs", n_in, dev)
+    _need_out(out, "out", _TYPE_ID, n_out, dev)
+    check(lib().sfnx_moe_down_f8_big(A.data_ptr(), sa, n_in, n_out, jobs.data_ptr(), njobs.data_ptr(), njobs_cap, hq.data_ptr(),
+                                     hs.data_ptr(), _TYPE_ID[out.dtype], out.data_ptr(), _st()))
 
 
 def _mm_16(fn, ints, A, sa, n_in, n_out, jobs, njobs, n, x, out) -> None:
-    _need_jobs(jobs, njobs, n, ints)
-    _need(x, "x", (torch.float16, torch.bfloat16), (None, n_in))
-    _need(out, "out", tuple(_TYPE_ID), (None, n_out))
-    if sa != 0 and A.dtype != x.dtype:
+    dev = _current()
+    _need_jobs(A, jobs, njobs, n, ints, dev)
+    _need_out(x, "x", (torch.float16, torch.bfloat16), n_in, dev)
+    _need_out(out, "out", _TYPE_ID, n_out, dev)
+    if sa != 0 and A.dtype is not x.dtype:
         raise ValueError("A: another type than x")
-    check(fn(_p(A), sa, _TYPE_ID[x.dtype], n_in, n_out, _p(jobs), _p(njobs), n, _p(x), _TYPE_ID[out.dtype], _p(out), _st()))
+    check(fn(A.data_ptr(), sa, _TYPE_ID[x.dtype], n_in, n_out, jobs.data_ptr(), njobs.data_ptr(), n, x.data_ptr(),
+             _TYPE_ID[out.dtype], out.data_ptr(), _st()))
 
 
 def moe_mm_16(A, sa, n_in, n_out, jobs, njobs, njobs_max, x, out) -> None:
