@@ -1,7 +1,7 @@
 // Experts and dense matrices in block-scaled 8-bit floating point (e4m3 values, an f32 scale for each 128 x 128 block of a
 // matrix and for each 128 values of an activation row): the activation quantizer, the dense product, and the products
 // grouped by expert over the routers' jobs.
-#include "mm_few.hpp"
+#include "mm_mid.hpp"
 #include "mm_tiles.hpp"
 
 namespace sfnx {
@@ -109,6 +109,14 @@ extern "C" int sfnx_f8_gemm(const void* W, int rows, int cols, const uint8_t* xq
         check_out(out, out_type);
         Args a{(const uint8_t*) W, sfnx_f8_matrix_bytes(rows, cols), cols, rows, nullptr, nullptr, C, xq, xs, out, nullptr, out_type, ldo,
                vec_ok(out, out_type, ldo)};
+        if (getenv("SFNX_MID")) {
+            int v = atoi(getenv("SFNX_MID"));
+            hipStream_t h = stream_of(st);
+            if (out_type == SFNX_F32) { if (v == 42) launch_mid_as<F8X, 4, 2>(a, h); if (v == 41) launch_mid_as<F8X, 4, 1>(a, h); if (v == 22) launch_mid_as<F8X, 2, 2>(a, h); if (v == 21) launch_mid_as<F8X, 2, 1>(a, h); if (v==44) launch_mid_as<F8X,4,4>(a,h); }
+            else { if (v == 44) launch_mid_as<F8, 4, 4>(a, h); if (v == 42) launch_mid_as<F8, 4, 2>(a, h); if (v == 41) launch_mid_as<F8, 4, 1>(a, h); if (v == 22) launch_mid_as<F8, 2, 2>(a, h); if (v == 24) launch_mid_as<F8, 2, 4>(a, h); if (v==21) launch_mid_as<F8,2,1>(a,h); }
+            if (v == 3) { if (out_type == SFNX_F32) launch_narrow<F8X>(a, (C + 63) / 64, h); else launch_narrow<F8>(a, (C + 63) / 64, h); }
+            if (v > 2) return;
+        }
         if (C <= FEW_M) launch_few<F8X, STORE, false>(a, 1, stream_of(st));
         else if (out_type == SFNX_F32) launch_tiles<F8X, STORE>(a, (C + BM1 - 1) / BM1, stream_of(st));
         else launch_tiles<F8, STORE>(a, (C + BM1 - 1) / BM1, stream_of(st));

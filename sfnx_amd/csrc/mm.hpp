@@ -15,6 +15,7 @@
 #pragma once
 
 #include <algorithm>
+#include <cstdlib>
 #include <type_traits>
 
 #include "common.hpp"

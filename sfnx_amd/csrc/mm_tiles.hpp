@@ -17,13 +17,19 @@ constexpr int BM1 = SFNX_PF_JOB, BN = 256;   // rows of a job and of a slice
 constexpr int GJ = 4, BMG = GJ * BM1;        // jobs and rows of a group
 constexpr int HP = BLK + 16;                 // row pitch of the quantized h on its way out
 
-// a stage in LDS: BN weight rows, M activation rows, their scales, a scale for each 16 weight rows (padded to a request)
-template <int M> struct Stage {
-    static constexpr int X = BN * STEP, XS = X + M * STEP, WS = XS + M * 4, SIZE = WS + 256;
+// a stage in LDS: N weight rows, M activation rows, their scales, a scale for each 16 weight rows (padded to a request)
+template <int M, int N = BN> struct Stage {
+    static constexpr int X = N * STEP, XS = X + M * STEP, WS = XS + M * 4, SIZE = WS + 256;
 };
-constexpr int S1_STAGES = 3, S1_SLOT = 768, S1_SLOTS = 4;   // S1_SLOT: a job's description
-constexpr int S1_JOBS = S1_STAGES * Stage<BM1>::SIZE, S1_EPI = S1_JOBS + S1_SLOTS * S1_SLOT;
-constexpr int S1_LDS = S1_EPI + TW * BM1 * 4 + BM1 * HP;
+// streamed tiles: NT row tiles a wavefront, so slices of 128 NT rows; KS K steps a stage, so that a wavefront has as many matrix
+// instructions between barriers with one tile as with two
+constexpr int S1_SLOT = 768, S1_SLOTS = 4;   // a job's description
+template <int NT> struct Stream {
+    typedef Stage<BM1, 128 * NT> S;
+    static constexpr int STAGES = 3, KS = NT == 2 ? 1 : 2, JOBS = STAGES * KS * S::SIZE, EPI = JOBS + (NT == 2 ? S1_SLOTS * S1_SLOT : 0);
+    static constexpr int LDS = EPI + (NT == 2 ? TW * BM1 * 4 + BM1 * HP : 0);   // NT = 1: dense products, stored as they are
+};
+constexpr int S1_LDS = Stream<2>::LDS;
 constexpr int SG_LIST = 2 * Stage<BMG>::SIZE, WINDOW = 8192;   // the groups of WINDOW jobs, as 16-bit job numbers
 constexpr int T_LDS = SG_LIST + 2 * WINDOW > S1_LDS ? SG_LIST + 2 * WINDOW : S1_LDS;
 static_assert(T_LDS + 64 <= 160 * 1024 && 4 * WINDOW <= SG_LIST && 2 * BMG * 4 + BMG * HP <= SG_LIST, "LDS");
@@ -42,9 +48,9 @@ __host__ __device__ __forceinline__ int64_t tiles_of(int nsl, int n) { return (i
 
 // The place of a slice's weight row in LDS.  STORE: wavefronts' rows in order.  SWIGLU: of each W = 2 NT tiles of 16 that a
 // wavefront owns, the first NT are gate tiles and the others their up tiles.
-template <Mode MODE, int NT2> __device__ __forceinline__ int weight_row(const Args& a, int sl, int i) {
+template <Mode MODE, int NT2, int N = BN> __device__ __forceinline__ int weight_row(const Args& a, int sl, int i) {
     const int n_eff = MODE == SWIGLU ? a.n_out / 2 : a.n_out;
-    if (MODE == STORE) return min(sl * BN + i, a.n_out - 1);
+    if (MODE == STORE) return min(sl * N + i, a.n_out - 1);
     const int w = i / (16 * NT2), u = i / 16 % NT2, nt = NT2 / 2;
     return min(sl * (BN / 2) + 16 * (nt * w + u % nt) + i % 16, n_eff - 1) + (u >= nt ? n_eff : 0);
 }
@@ -103,17 +109,18 @@ __device__ __forceinline__ void swiglu_out(const Args& a, float4v (&acc)[2 * NT]
 }
 
 // ------------------------------------------------------------------------------------------------ one job a tile
-// The tiles are one unbroken stream of K steps: while a step is multiplied the next two are on their way into LDS, across
+// The tiles are one unbroken stream of stages: while one is multiplied the next two are on their way into LDS, across
 // the ends of tiles too, so no tile waits for its first weights.  The descriptions of later jobs come by asynchronous copies
 // as well: a load the compiler waits for would drain the stream.  A wavefront owns 32 of the tile's weight rows for all of
 // the job's rows.
-template <Elem EL, Mode MODE> __device__ __forceinline__ void stream_tiles(const Args& a, int nj, uint8_t* lds) {
-    constexpr int REQ = 5 + (IS8<EL> ? 2 : 0);   // copies a wavefront issues for a step
-    typedef Stage<BM1> S;
+template <Elem EL, Mode MODE, int NT> __device__ __forceinline__ void stream_tiles(const Args& a, int nj, uint8_t* lds) {
+    constexpr int KS = Stream<NT>::KS, D = Stream<NT>::STAGES, N = 128 * NT;
+    constexpr int REQ = KS * (2 * NT + 1 + (IS8<EL> ? 2 : 0));   // copies a wavefront issues for a stage
+    typedef typename Stream<NT>::S S;
     const int lane = threadIdx.x % WAVE, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
     const int r = lane % 16, q = lane / 16, r8 = lane / 8, p8 = (lane % 8) ^ r8;
     const int rb = a.n_in * ESZ<EL>, steps = (rb + STEP - 1) / STEP, nb = blocks_of(a.n_in);
-    const int nsl = a.slices, grid = (int) gridDim.x, tiles = (int) tiles_of(nsl, nj);
+    const int nsl = (a.n_out + N - 1) / N, grid = (int) gridDim.x, tiles = (int) tiles_of(nsl, nj);
     const bool dense = a.dense_c > 0;
     const sfnx_bigjob* jobs = (const sfnx_bigjob*) a.jobs;
 
@@ -122,7 +129,7 @@ template <Elem EL, Mode MODE> __device__ __forceinline__ void stream_tiles(const
             if (tile_at(b, nsl, nj, sl, ji)) return b;
         return -1;
     };
-    auto slot_of = [&](int c) { return reinterpret_cast<const int*>(lds + S1_JOBS + (c % S1_SLOTS) * S1_SLOT); };
+    auto slot_of = [&](int c) { return reinterpret_cast<const int*>(lds + Stream<NT>::JOBS + (c % S1_SLOTS) * S1_SLOT); };
     auto request_job = [&](int c, int ji) {   // the job's 130 words
         if (dense) return;
         const int* src = reinterpret_cast<const int*>(jobs + (nj - 1 - ji));   // the last job first: the shared expert's are the longest
@@ -141,45 +148,50 @@ template <Elem EL, Mode MODE> __device__ __forceinline__ void stream_tiles(const
     // the producer: tile pt (its pc-th), whose step ps is requested next; nt, the tile after it, whose job is under way
     int pt, psl, pji, pc = 0, ps = 0, nt, nsl_ = 0, nji = 0;
     const uint8_t *wbase, *xsrc;
-    uint32_t woff[4];
+    uint32_t woff[2 * NT];
     const float *xs_src, *ws_src;
     auto enter = [&]() {   // the pc-th tile's addresses; its job is in its slot
         const int n = job_rows(pc, pji), e = dense ? 0 : __builtin_amdgcn_readfirstlane(slot_of(pc)[0]);
         wbase = uniform_ptr(expert_at(a.A, a.sa, e));
 #pragma unroll
-        for (int i = 0; i < 4; ++i) woff[i] = (uint32_t) weight_row<MODE, 2>(a, psl, 32 * wave + 8 * i + r8) * (uint32_t) rb + 16 * p8;
+        for (int i = 0; i < 2 * NT; ++i) woff[i] = (uint32_t) weight_row<MODE, NT, N>(a, psl, 16 * NT * wave + 8 * i + r8) * (uint32_t) rb + 16 * p8;
         xsrc = a.x + (size_t) act_row(pc, pji, n, 8 * wave + r8) * rb + 16 * p8;
         if constexpr (IS8<EL>) {
             xs_src = a.xs + (size_t) act_row(pc, pji, n, lane) * nb;
-            ws_src = scales_of(wbase, a.n_out, a.n_in) + (size_t) (weight_row<MODE, 2>(a, psl, 16 * r) / BLK) * nb;
+            ws_src = scales_of(wbase, a.n_out, a.n_in) + (size_t) (weight_row<MODE, NT, N>(a, psl, 16 * (r % (8 * NT))) / BLK) * nb;
         }
         nt = next_tile(pt + grid, nsl_, nji);
         if (nt >= 0) request_job(pc + 1, nji);
     };
-    auto produce = [&](uint8_t* buf) {   // the next step of the stream into a stage; false: there is none
-        if (ps == steps) {
+    auto produce = [&](uint8_t* stage) {   // the next KS steps of the stream into a stage; false: there are none
+        if (ps >= steps) {
             if (nt < 0) return false;
-            if (steps < 2) vm_wait<0>();   // the job was requested in the step before this one; else an older wait covers it
+            if (steps <= KS) vm_wait<0>();   // the job was requested in the stage before this one; else an older wait covers it
             pt = nt, psl = nsl_, pji = nji, ps = 0, ++pc;
             enter();
         }
-        const int k = ps * STEP;
-        const uint8_t* x = xsrc + k;
-        if (k + STEP <= rb) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) copy16(uniform_ptr(wbase + k), woff[i], buf + (32 * wave + 8 * i) * STEP);
-        } else {   // zero past the rows' end
-            const bool in = k + 16 * p8 < rb;
+        for (int h = 0; h < KS; ++h) {
+            const int s = min(ps + h, steps - 1), k = s * STEP;   // past the last step that again
+            uint8_t* buf = stage + h * S::SIZE;
+            const uint8_t* x = xsrc + k;
+            if (k + STEP <= rb) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) copy16(in ? wbase + k + woff[i] : (const uint8_t*) &ZERO16, buf + (32 * wave + 8 * i) * STEP);
-            if (!in) x = (const uint8_t*) &ZERO16;
+                for (int i = 0; i < 2 * NT; ++i) copy16(uniform_ptr(wbase + k), woff[i], buf + (16 * NT * wave + 8 * i) * STEP);
+            } else {   // zero past the rows' end
+                const bool in = k + 16 * p8 < rb;
+#pragma unroll
+                for (int i = 0; i < 2 * NT; ++i)
+                    copy16(in ? wbase + k + woff[i] : (const uint8_t*) &ZERO16, buf + (16 * NT * wave + 8 * i) * STEP);
+                if (!in) x = (const uint8_t*) &ZERO16;
+            }
+            copy16(x, buf + S::X + 8 * wave * STEP);
+            if constexpr (IS8<EL>) {   // every wavefront copies them all: the same values, and each counts the same requests
+                copy4(xs_src + s, buf + S::XS);
+                copy4(ws_src + s, buf + S::WS);
+            }
         }
-        copy16(x, buf + S::X + 8 * wave * STEP);
-        if constexpr (IS8<EL>) {   // every wavefront copies them all: the same values, and each counts the same requests
-            copy4(xs_src + ps, buf + S::XS);
-            copy4(ws_src + ps, buf + S::WS);
-        }
-        ++ps;
+        ps += KS;
         return true;
     };
 
@@ -189,35 +201,41 @@ template <Elem EL, Mode MODE> __device__ __forceinline__ void stream_tiles(const
     vm_wait<0>();
     int ct = pt, csl = psl, cji = pji;   // the tile that is multiplied
     enter();
-    produce(lds);
-    bool ahead = produce(lds + S::SIZE);   // whether a stage after the one to be multiplied has been requested
-    int at = 0;                            // the stage to be multiplied
+    int ahead = -1;   // how many stages after the one to be multiplied have been requested
+#pragma unroll
+    for (int i = 0; i < D - 1; ++i) ahead += produce(lds + i * KS * S::SIZE);
+    int at = 0;       // the stage to be multiplied
     for (int c = 0; ct >= 0; ++c) {
         const int n = job_rows(c, cji);
-        float4v acc[2][4] = {};
+        float4v acc[NT][4] = {};
         auto walk = [&](auto mt) {
             constexpr int MT = decltype(mt)::value;
-            for (int s = 0; s < steps; ++s) {
-                if (ahead) vm_wait<REQ>();
+            for (int s = 0; s < steps; s += KS) {
+                if (ahead == D - 2) vm_wait<REQ * (D - 2)>();
                 else vm_wait<0>();
                 lds_barrier();   // every wavefront's copies of this stage landed, and every wavefront is past the one before
-                const uint8_t* buf = lds + at * S::SIZE;
-                ahead = produce(lds + (at == 0 ? 2 : at - 1) * S::SIZE);
-                at = at == 2 ? 0 : at + 1;
-                Operand<EL> w[2];
-                float ws[2];
+                const uint8_t* stage = lds + at * KS * S::SIZE;
+                ahead += (int) produce(lds + (at == 0 ? D - 1 : at - 1) * KS * S::SIZE) - 1;
+                at = at == D - 1 ? 0 : at + 1;
 #pragma unroll
-                for (int t = 0; t < 2; ++t) {
-                    w[t] = operand<EL>(lds_frag(buf, 32 * wave + 16 * t + r, q));
-                    if constexpr (IS8<EL>) ws[t] = reinterpret_cast<const float*>(buf + S::WS)[2 * wave + t];
-                }
+                for (int h = 0; h < KS; ++h) {
+                    if (h > 0 && s + h >= steps) break;
+                    const uint8_t* buf = stage + h * S::SIZE;
+                    Operand<EL> w[NT];
+                    float ws[NT];
 #pragma unroll
-                for (int j = 0; j < MT; ++j) {
-                    const Operand<EL> x = operand<EL>(lds_frag(buf + S::X, 16 * j + r, q));
-                    float xs = 1.f;
-                    if constexpr (IS8<EL>) xs = reinterpret_cast<const float*>(buf + S::XS)[16 * j + r];
+                    for (int t = 0; t < NT; ++t) {
+                        w[t] = operand<EL>(lds_frag(buf, 16 * NT * wave + 16 * t + r, q));
+                        if constexpr (IS8<EL>) ws[t] = reinterpret_cast<const float*>(buf + S::WS)[NT * wave + t];
+                    }
 #pragma unroll
-                    for (int t = 0; t < 2; ++t) acc[t][j] = step_mma<EL>(w[t], x, acc[t][j], IS8<EL> ? xs * ws[t] : 1.f);
+                    for (int j = 0; j < MT; ++j) {
+                        const Operand<EL> x = operand<EL>(lds_frag(buf + S::X, 16 * j + r, q));
+                        float xs = 1.f;
+                        if constexpr (IS8<EL>) xs = reinterpret_cast<const float*>(buf + S::XS)[16 * j + r];
+#pragma unroll
+                        for (int t = 0; t < NT; ++t) acc[t][j] = step_mma<EL>(w[t], x, acc[t][j], IS8<EL> ? xs * ws[t] : 1.f);
+                    }
                 }
             }
         };
@@ -236,24 +254,26 @@ template <Elem EL, Mode MODE> __device__ __forceinline__ void stream_tiles(const
                 if (m >= n) continue;
                 const size_t o = (size_t) out_row(m) * a.ldo;
 #pragma unroll
-                for (int t = 0; t < 2; ++t) {
-                    const int col = csl * BN + 32 * wave + 16 * t + 4 * q;
+                for (int t = 0; t < NT; ++t) {
+                    const int col = csl * N + 16 * NT * wave + 16 * t + 4 * q;
                     store4(a.out, a.out_type, o + col, acc[t][j], a.n_out - col, a.vec);
                 }
             }
         } else {
-            swiglu_out<TW, 1, 4, BM1>(a, acc, csl, wave, 0, n, n, lds + S1_EPI, out_row);
+            swiglu_out<TW, 1, 4, BM1>(a, acc, csl, wave, 0, n, n, lds + Stream<NT>::EPI, out_row);
         }
         ct = next_tile(ct + grid, csl, cji);
     }
 }
 
 // ------------------------------------------------------------------------------------------------ a group of jobs a tile
-// A wavefront owns a job's 64 rows (wavefronts 2 w and 2 w + 1 the w-th of the group) and 128 of the tile's weight rows.
-template <Elem EL, Mode MODE> __device__ __forceinline__ void group_tile(const Args& a, int sl, int j0, int count, uint8_t* lds) {
-    typedef Stage<BMG> S;
+// A wavefront owns a job's 64 rows and NT of the tile's 16 weight tiles: of a group of C jobs (3 are taken as 4), 8 / C wavefronts
+// share a job.
+template <Elem EL, Mode MODE, int C> __device__ __forceinline__ void group_tile(const Args& a, int sl, int j0, int count, uint8_t* lds) {
+    constexpr int WN = TW / C, NT = 16 / WN;
+    typedef Stage<BM1 * C> S;
     const int lane = threadIdx.x % WAVE, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
-    const int r = lane % 16, q = lane / 16, r8 = lane / 8, p8 = (lane % 8) ^ r8, wm = wave / 2, wn = wave % 2;
+    const int r = lane % 16, q = lane / 16, r8 = lane / 8, p8 = (lane % 8) ^ r8, wm = wave / WN, wn = wave % WN;
     const int rb = a.n_in * ESZ<EL>, steps = (rb + STEP - 1) / STEP, nb = blocks_of(a.n_in);
     const bool dense = a.dense_c > 0;
     const sfnx_bigjob* jobs = (const sfnx_bigjob*) a.jobs + j0;
@@ -275,58 +295,78 @@ template <Elem EL, Mode MODE> __device__ __forceinline__ void group_tile(const A
     const uint8_t* mat = uniform_ptr(expert_at(a.A, a.sa, dense ? 0 : jobs[0].w));
     const int n = __builtin_amdgcn_readfirstlane(rows_of(wm));
 
+    // Of a stage, the rows of the activations and of each wavefront's first half of the weight tiles are read in the first half of a
+    // step, and copied over from the middle of it on, two steps ahead (EARLY); the other weight tiles' rows, one step ahead from
+    // its start on.  F8X reads everything until the end: one step ahead, spread over the step's first half.
+    constexpr bool EARLY = EL != F8X;
     uint32_t woff[4];
-    const uint8_t* xsrc[4];
+    const uint8_t* xsrc[C];
     const float *xs_src = nullptr, *ws_src = nullptr;
+    int wto[4];   // this wavefront's 8-row pieces of the weights: two of first, two of other tiles
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        woff[i] = (uint32_t) weight_row<MODE, 8>(a, sl, 32 * wave + 8 * i + r8) * (uint32_t) rb;
-        xsrc[i] = a.x + (size_t) act_row(32 * wave + 8 * i + r8) * rb;
+        const int h = 2 * wave + i % 2;
+        wto[i] = 16 * NT * (h / NT) + 8 * NT * (i / 2) + 8 * (h % NT);
+        woff[i] = (uint32_t) weight_row<MODE, NT>(a, sl, wto[i] + r8) * (uint32_t) rb;
     }
+#pragma unroll
+    for (int i = 0; i < C; ++i) xsrc[i] = a.x + (size_t) act_row(8 * (C * wave + i) + r8) * rb;
     if constexpr (IS8<EL>) {
         xs_src = a.xs + (size_t) act_row(64 * wm + lane) * nb;
-        ws_src = scales_of(mat, a.n_out, a.n_in) + (size_t) (weight_row<MODE, 8>(a, sl, 16 * r) / BLK) * nb;
+        ws_src = scales_of(mat, a.n_out, a.n_in) + (size_t) (weight_row<MODE, NT>(a, sl, 16 * r) / BLK) * nb;
     }
-    // the u-th eighth of step s into a stage; past the rows' end their last piece (see below), past the last step that again
+    // copy u (0 .. 3 weights, 4 .. 3 + C activations) of step s into a stage; past the rows' end their last piece (see below), past
+    // the last step that again
     auto copy = [&](int u, int s, uint8_t* buf) {
-        s = min(s, steps - 1);
-        const uint32_t k = (uint32_t) min(s * STEP + 16 * p8, rb - 16);
-        const int i = u % 4;
-        if (u < 4) copy16(mat, woff[i] + k, buf + (32 * wave + 8 * i) * STEP);
-        else copy16(xsrc[i] + k, buf + S::X + (32 * wave + 8 * i) * STEP);
+        const uint32_t k = (uint32_t) min(min(s, steps - 1) * STEP + 16 * p8, rb - 16);
+        if (u < 4) copy16(mat, woff[u] + k, buf + wto[u] * STEP);
+        else copy16(xsrc[u - 4] + k, buf + S::X + 8 * (C * wave + u - 4) * STEP);
+    };
+    auto copy_scales = [&](int s, uint8_t* buf) {
         if constexpr (IS8<EL>) {
-            if (u == 2) copy4(xs_src + s, buf + S::XS + 256 * wm);
-            if (u == 3) copy4(ws_src + s, buf + S::WS);
+            copy4(xs_src + min(s, steps - 1), buf + S::XS + 256 * wm);
+            copy4(ws_src + min(s, steps - 1), buf + S::WS);
         }
+    };
+    auto copy_early = [&](int s, uint8_t* buf) {
+#pragma unroll
+        for (int u = 0; u < 4 + C; ++u)
+            if (u < 2 || u >= 4) copy(u, s, buf);
+    };
+    auto copy_late = [&](int s, uint8_t* buf) {
+        copy(2, s, buf);
+        copy(3, s, buf);
+        copy_scales(s, buf);
     };
     auto fence = [] { asm volatile("" ::: "memory"); };   // LDS reads stay where they are: all at once they would not fit the registers
-    // what a wavefront copies of the next step beside its u-th weight tile (of 8): all of it in the first half of the step, so
-    // that it is there at the step's end, but not at once
-    auto ahead = [&](int u, int s, uint8_t* buf) {
-        if (u < 4) {
-            copy(2 * u, s, buf);
-            copy(2 * u + 1, s, buf);
-        }
-        fence();
-    };
-    float4v acc[8][4] = {};
+    float4v acc[NT][4] = {};
     lds_barrier();   // the tile before is done with LDS
-#pragma unroll
-    for (int u = 0; u < 8; ++u) copy(u, 0, lds);
+    copy_early(0, lds);
+    copy_late(0, lds);
+    if (EARLY) copy_early(1, lds + S::SIZE);
     for (int s = 0; s < steps; ++s) {
         uint8_t* buf = lds + (s & 1) * S::SIZE;
         uint8_t* to = lds + ((s + 1) & 1) * S::SIZE;
-        vm_wait<0>();
+        if (EARLY) vm_wait<2 + C>();   // all but the early copies of the step after this one
+        else vm_wait<0>();
         if (s == steps - 1 && rb % STEP) {   // zero past the rows' end, whatever lies there: each wavefront in what it copied
             const int k = s * STEP + 16 * p8;
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-                if (k >= rb) {
-                    *reinterpret_cast<uint4*>(buf + (32 * wave + 8 * i) * STEP + 16 * lane) = uint4{};
-                    *reinterpret_cast<uint4*>(buf + S::X + (32 * wave + 8 * i) * STEP + 16 * lane) = uint4{};
-                }
+                if (k >= rb) *reinterpret_cast<uint4*>(buf + wto[i] * STEP + 16 * lane) = uint4{};
+#pragma unroll
+            for (int i = 0; i < C; ++i)
+                if (k >= rb) *reinterpret_cast<uint4*>(buf + S::X + 8 * (C * wave + i) * STEP + 16 * lane) = uint4{};
         }
         lds_barrier();   // every wavefront's copies of this stage landed, and every wavefront is past the one before
+        auto middle = [&](int u) {   // after a wavefront's u-th weight tile
+            if (u == 0) copy_late(s + 1, to);
+            if (u == NT / 2 - 1) {
+                lds_barrier();   // every wavefront has read the activations and the first tiles
+                copy_early(s + 2, buf);
+            }
+            fence();
+        };
         if constexpr (EL == F8) {
             // the products of a weight tile are added while the next tile's are made
             Frag x[4];
@@ -336,19 +376,19 @@ template <Elem EL, Mode MODE> __device__ __forceinline__ void group_tile(const A
                 x[j] = lds_frag(buf + S::X, 64 * wm + 16 * j + r, q);
                 xs[j] = reinterpret_cast<const float*>(buf + S::XS)[64 * wm + 16 * j + r];
             }
-            Frag w = lds_frag(buf, 128 * wn + r, q);
-            float ws = reinterpret_cast<const float*>(buf + S::WS)[8 * wn];
+            Frag w = lds_frag(buf, 16 * NT * wn + r, q);
+            float ws = reinterpret_cast<const float*>(buf + S::WS)[NT * wn];
 #pragma unroll
-            for (int u = 0; u < 8; ++u) {
+            for (int u = 0; u < NT; ++u) {
                 float4v d[4];
 #pragma unroll
                 for (int j = 0; j < 4; ++j) d[j] = step_dot<EL>(w, x[j]);
                 const float sc = ws;
-                if (u < 7) {
-                    w = lds_frag(buf, 128 * wn + 16 * (u + 1) + r, q);
-                    ws = reinterpret_cast<const float*>(buf + S::WS)[8 * wn + u + 1];
+                if (u < NT - 1) {
+                    w = lds_frag(buf, 16 * NT * wn + 16 * (u + 1) + r, q);
+                    ws = reinterpret_cast<const float*>(buf + S::WS)[NT * wn + u + 1];
                 }
-                ahead(u, s + 1, to);
+                middle(u);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) acc[u][j] = scaled_add(d[j], xs[j] * sc, acc[u][j]);
             }
@@ -364,12 +404,15 @@ template <Elem EL, Mode MODE> __device__ __forceinline__ void group_tile(const A
                     xs[j] = reinterpret_cast<const float*>(buf + S::XS)[64 * wm + 32 * h + 16 * j + r];
                 }
 #pragma unroll
-                for (int u = 0; u < 8; ++u) {
-                    const FragX w = operand<EL>(lds_frag(buf, 128 * wn + 16 * u + r, q));
-                    const float ws = reinterpret_cast<const float*>(buf + S::WS)[8 * wn + u];
+                for (int u = 0; u < NT; ++u) {
+                    const FragX w = operand<EL>(lds_frag(buf, 16 * NT * wn + 16 * u + r, q));
+                    const float ws = reinterpret_cast<const float*>(buf + S::WS)[NT * wn + u];
 #pragma unroll
                     for (int j = 0; j < 2; ++j) acc[u][2 * h + j] = step_mma<EL>(w, x[j], acc[u][2 * h + j], xs[j] * ws);
-                    if (h == 0) copy(u, s + 1, to);
+                    if (h == 0)
+#pragma unroll
+                        for (int i = u * (4 + C) / NT; i < (u + 1) * (4 + C) / NT; ++i) copy(i, s + 1, to);
+                    if (h == 0 && u == NT - 1) copy_scales(s + 1, to);
                     fence();
                 }
             }
@@ -377,12 +420,14 @@ template <Elem EL, Mode MODE> __device__ __forceinline__ void group_tile(const A
             Frag x[4];
 #pragma unroll
             for (int j = 0; j < 4; ++j) x[j] = lds_frag(buf + S::X, 64 * wm + 16 * j + r, q);
+            Frag w = lds_frag(buf, 16 * NT * wn + r, q);
 #pragma unroll
-            for (int u = 0; u < 8; ++u) {
-                const Frag w = lds_frag(buf, 128 * wn + 16 * u + r, q);
-                ahead(u, s + 1, to);
+            for (int u = 0; u < NT; ++u) {
+                const Frag v = w;
+                if (u < NT - 1) w = lds_frag(buf, 16 * NT * wn + 16 * (u + 1) + r, q);
+                middle(u);
 #pragma unroll
-                for (int j = 0; j < 4; ++j) acc[u][j] = step_mma<EL>(w, x[j], acc[u][j], 1.f);
+                for (int j = 0; j < 4; ++j) acc[u][j] = step_mma<EL>(v, x[j], acc[u][j], 1.f);
             }
         }
     }
@@ -394,14 +439,14 @@ template <Elem EL, Mode MODE> __device__ __forceinline__ void group_tile(const A
             if (m >= n) continue;
             const size_t o = (size_t) out_row(64 * wm + m) * a.ldo;
 #pragma unroll
-            for (int u = 0; u < 8; ++u) {
-                const int col = sl * BN + 128 * wn + 16 * u + 4 * q;
+            for (int u = 0; u < NT; ++u) {
+                const int col = sl * BN + 16 * NT * wn + 16 * u + 4 * q;
                 store4(a.out, a.out_type, o + col, acc[u][j], a.n_out - col, a.vec);
             }
         }
     } else {
         lds_barrier();   // the stages are free
-        swiglu_out<2, 4, 4, BMG>(a, acc, sl, wn, 64 * wm, n, BMG, lds, out_row);
+        swiglu_out<WN, NT / 2, 4, BM1 * C>(a, acc, sl, wn, 64 * wm, n, BM1 * C, lds, out_row);
     }
 }
 
@@ -453,10 +498,24 @@ template <Elem EL, Mode MODE> __global__ void __launch_bounds__(TT, 2) k_mm_tile
             if (!tile_at(b, a.slices, n, sl, i)) continue;
             i = n - 1 - i;   // the last group first: the shared expert's
             const int j0 = dense ? GJ * i : list[i], j1 = dense ? min(j0 + GJ, count) : i + 1 < n ? list[i + 1] : count;
-            group_tile<EL, MODE>(a, sl, w0 + j0, j1 - j0, lds);
+            if (j1 - j0 > 2) group_tile<EL, MODE, 4>(a, sl, w0 + j0, j1 - j0, lds);
+            else if (j1 - j0 == 2) group_tile<EL, MODE, 2>(a, sl, w0 + j0, 2, lds);
+            else group_tile<EL, MODE, 1>(a, sl, w0 + j0, 1, lds);
         }
     }
-    if (!group) stream_tiles<EL, MODE>(a, nj, lds);
+    if (!group) stream_tiles<EL, MODE, 2>(a, nj, lds);
+}
+
+// a dense product in streamed tiles of 64 x 128
+template <Elem EL> __global__ void __launch_bounds__(TT, 2) k_mm_narrow(Args a, int jobs) {
+    extern __shared__ __align__(16) uint8_t lds[];
+    stream_tiles<EL, STORE, 1>(a, jobs, lds);
+}
+template <Elem EL> void launch_narrow(const Args& a, int jobs, hipStream_t s) {
+    const int64_t tiles = tiles_of((a.n_out + 127) / 128, jobs);
+    require(tiles < (1 << 30), "too many jobs for one launch");
+    require((uint64_t) a.n_out * a.n_in * ESZ<EL> < ((uint64_t) 1 << 32), "a matrix must be smaller than 4 GiB");
+    k_mm_narrow<EL><<<(unsigned) std::min<int64_t>(tiles, CUS), TT, Stream<1>::LDS, s>>>(a, jobs);
 }
 
 template <Elem EL, Mode MODE> void launch_tiles(Args a, int njobs_cap, hipStream_t s) {
@@ -464,7 +523,7 @@ template <Elem EL, Mode MODE> void launch_tiles(Args a, int njobs_cap, hipStream
     a.slices = (a.n_out + BN - 1) / BN;
     const int64_t tiles = tiles_of(a.slices, njobs_cap);
     require(tiles < (1 << 30), "too many jobs for one launch");
-    const int group = a.dense_c > 0 && (int64_t) a.slices * ((njobs_cap + GJ - 1) / GJ) >= CUS / 2;
+    const int group = getenv("SFNX_MID") && atoi(getenv("SFNX_MID")) > 0 ? atoi(getenv("SFNX_MID")) - 1 : a.dense_c > 0 && (int64_t) a.slices * ((njobs_cap + GJ - 1) / GJ) >= CUS / 2;
     k_mm_tiles<EL, MODE><<<(unsigned) std::min<int64_t>(tiles, CUS), TT, T_LDS + 64, s>>>(a, njobs_cap, group);
 }
 
