@@ -9,35 +9,70 @@ namespace {
 using namespace mm;
 
 // ------------------------------------------------------------------------------------------------ the quantizer
-// four values of a row from column k on, as fp32
-template <int TYPE> __device__ __forceinline__ float4 load4(const void* x, size_t i) {
+// eight values of a row, as fp32
+template <int TYPE> __device__ __forceinline__ void load8(const void* x, size_t i, float (&v)[8]) {
     if constexpr (TYPE == SFNX_F32) {
-        return *reinterpret_cast<const float4*>((const float*) x + i);
+        const float4 a = reinterpret_cast<const float4*>((const float*) x + i)[0], b = reinterpret_cast<const float4*>((const float*) x + i)[1];
+        v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
     } else {
-        const uint2 u = *reinterpret_cast<const uint2*>((const uint16_t*) x + i);
-        if constexpr (TYPE == SFNX_F16)
-            return float4{h2f(u.x & 0xffff), h2f(u.x >> 16), h2f(u.y & 0xffff), h2f(u.y >> 16)};
-        else
-            return float4{__uint_as_float(u.x << 16), __uint_as_float(u.x & 0xffff0000u), __uint_as_float(u.y << 16),
-                          __uint_as_float(u.y & 0xffff0000u)};
+        const uint4 u = *reinterpret_cast<const uint4*>((const uint16_t*) x + i);
+        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            v[2 * k] = TYPE == SFNX_F16 ? h2f(w[k] & 0xffff) : __uint_as_float(w[k] << 16);
+            v[2 * k + 1] = TYPE == SFNX_F16 ? h2f(w[k] >> 16) : __uint_as_float(w[k] & 0xffff0000u);
+        }
     }
 }
 
-// half a wavefront a block of 128 values
-template <int TYPE>
-__global__ void __launch_bounds__(256) k_quantize_f8(const void* __restrict__ x, int64_t ldx, int rows, int cols,
+// 16 lanes a block of 128 values.  A workgroup's 16 groups of lanes are GX along a row (as many as it has blocks, at most 16)
+// by 16 / GX rows, U times; all U rows are requested before the first is used.
+template <int TYPE, int U>
+__global__ void __launch_bounds__(256) k_quantize_f8(const void* __restrict__ x, int64_t ldx, int rows, int cols, int gx_log,
                                                      uint8_t* __restrict__ q, float* __restrict__ s) {
-    const int nb = blocks_of(cols), c = 4 * (threadIdx.x % 32);
-    for (int64_t i = (int64_t) blockIdx.x * 8 + threadIdx.x / 32; i < (int64_t) rows * nb; i += (int64_t) gridDim.x * 8) {
-        const int64_t r = i / nb;
-        const int k = (int) (i % nb) * BLK + c;
-        float4 v = {0, 0, 0, 0};
-        if (k < cols) v = load4<TYPE>(x, (size_t) (r * ldx + k));
-        const float am = group_max<32>(fmaxf(fmaxf(finite_abs(v.x), finite_abs(v.y)), fmaxf(finite_abs(v.z), finite_abs(v.w))));
-        const float sc = f8_scale(am);
-        if (k < cols) *reinterpret_cast<uint32_t*>(q + r * cols + k) = f8_pack4(v.x, v.y, v.z, v.w, sc);
-        if (c == 0) s[i] = sc;
+    const int g = threadIdx.x / 16, nb = blocks_of(cols), b = (blockIdx.y << gx_log) + (g & ((1 << gx_log) - 1)), k = b * BLK + 8 * (threadIdx.x % 16);
+    const int gy = 16 >> gx_log, r0 = blockIdx.x * (U * gy) + (g >> gx_log);
+    float v[U][8];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const int r = r0 + u * gy;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[u][i] = 0.f;
+        if (r < rows && k < cols) load8<TYPE>(x, (size_t) (r * ldx + k), v[u]);
     }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const int r = r0 + u * gy;
+        uint32_t top = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) top = max(top, abs_bits(v[u][i]));
+        top = (uint32_t) group_reduce<16>((int) top, [](int a, int c) { return max(a, c); });
+        float am = __uint_as_float(top);
+        const bool fin = top < 0x7f800000u;
+        if (__any(!fin)) {
+            am = 0.f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) am = fmaxf(am, finite_abs(v[u][i]));
+            am = group_max<16>(am);
+        }
+        const F8Scale sc = f8_scale(am, fin);
+        const uint2 o = {f8_pack4(v[u][0], v[u][1], v[u][2], v[u][3], sc), f8_pack4(v[u][4], v[u][5], v[u][6], v[u][7], sc)};
+        if (r < rows && k < cols) *reinterpret_cast<uint2*>(q + (size_t) r * cols + k) = o;
+        if (r < rows && b < nb && threadIdx.x % 16 == 0) s[(size_t) r * nb + b] = sc.s;
+    }
+}
+
+template <int TYPE> void quantize(const void* x, int64_t ldx, int rows, int cols, uint8_t* q, float* s, hipStream_t st) {
+    const int nb = blocks_of(cols);
+    int gx_log = 0;
+    while (gx_log < 4 && (1 << gx_log) < nb) ++gx_log;
+    const int gx = 1 << gx_log, gy = 16 / gx;
+    // four rows a lane where that still makes four workgroups a compute unit: 4096 x 4096 bf16 one at a time 14.2 us, four 12.4
+    const int64_t per = (int64_t) ((nb + gx - 1) / gx) * ((rows + gy - 1) / gy);
+    if (per >= 16 * CUS)
+        k_quantize_f8<TYPE, 4><<<dim3((rows + 4 * gy - 1) / (4 * gy), (nb + gx - 1) / gx), 256, 0, st>>>(x, ldx, rows, cols, gx_log, q, s);
+    else
+        k_quantize_f8<TYPE, 1><<<dim3((rows + gy - 1) / gy, (nb + gx - 1) / gx), 256, 0, st>>>(x, ldx, rows, cols, gx_log, q, s);
 }
 
 // ------------------------------------------------------------------------------------------------ checks
@@ -61,12 +96,48 @@ void check_f8_matrix(const void* A, size_t sa, int n_in, int n_out) {
     require(al16(A), ALIGN_MSG);
     require(n_in > 0 && n_in % 16 == 0 && n_in <= (1 << 20), "input width must be a multiple of 16, at most 2^20");
     require(n_out > 0 && n_out <= (1 << 20), "n_out out of range");
+    require((uint64_t) n_out * n_in < ((uint64_t) 1 << 32), "a matrix must be smaller than 4 GiB");
     require(stride_ok(sa, sfnx_f8_matrix_bytes(n_out, n_in)), "expert stride smaller than a matrix");
     require(sa % 16 == 0, "expert stride must be a multiple of 16");
 }
 void check_f8_rows(const uint8_t* xq, const float* xs) {
     require(xq != nullptr && xs != nullptr, "null pointer");
     require(al16(xq), ALIGN_MSG);
+}
+
+// A dense product of more than 16 rows: the form of the least estimated time.  A form's tile takes `one` us for 4096 columns
+// when all tiles run at once, `more` in further rounds of 256 workgroups, and `fixed` us whatever the columns; measured with
+// matrices of 256 to 4096 rows, 512 to 4096 columns and 17 to 4096 rows of activations (us, into bf16; 4096 columns):
+//   rows x rows      32x16 mid  32x32 mid  32x64 mid  64x128 streamed  64x256 streamed  256x256 grouped
+//   128 x 256           9.4        11.3       15.5          27               31               52
+//   256 x 1024         16.8        11.8       15.6          27               33               64
+//   512 x 2048         58          37         30            28               33               65
+//   1024 x 4096       224         141        114            69               36               66
+//   4096 x 4096                                                             127               72
+struct DenseForm {
+    int rows, cols;
+    float one, more, fixed;
+};
+template <Elem EL> void dense_many(const Args& a, hipStream_t st) {
+    constexpr DenseForm forms[2][6] = {
+        {{32, 16, 4.4f, 6.6f, 0.5f}, {32, 32, 6.3f, 8.1f, 0.5f}, {32, 64, 10.5f, 12.5f, 0.5f}, {64, 128, 21.f, 21.f, 1.5f}, {64, 256, 28.f, 29.f, 1.7f}, {256, 256, 47.f, 51.f, 9.f}},
+        {{32, 16, 4.5f, 6.6f, 0.5f}, {32, 32, 6.5f, 9.1f, 0.5f}, {64, 32, 13.f, 15.5f, 0.5f}, {64, 128, 32.f, 31.f, 1.5f}, {64, 256, 38.f, 39.f, 1.7f}, {256, 256, 110.f, 112.f, 9.f}}};
+    int best = 0;
+    float least = 0.f;
+    for (int i = 0; i < 6; ++i) {
+        const DenseForm& f = forms[EL == F8X][i];
+        const int64_t tiles = (int64_t) ((a.dense_c + f.rows - 1) / f.rows) * ((a.n_out + f.cols - 1) / f.cols), rounds = (tiles + CUS - 1) / CUS;
+        const float t = rounds * ((rounds == 1 ? f.one : f.more) * a.n_in / 4096.f + f.fixed);
+        if (i == 0 || t < least) best = i, least = t;
+    }
+    const int jobs = (a.dense_c + BM1 - 1) / BM1;
+    switch (best) {
+        case 0: return launch_mid<EL, 2, 1>(a, st);
+        case 1: return launch_mid<EL, 2, 2>(a, st);
+        case 2: return launch_mid<EL, EL == F8X ? 4 : 2, EL == F8X ? 2 : 4>(a, st);
+        case 3: return launch_narrow<EL>(a, jobs, st);
+        default: return launch_tiles<EL, STORE>(a, jobs, best == 5, st);
+    }
 }
 
 }  // namespace
@@ -83,18 +154,16 @@ extern "C" size_t sfnx_f8_matrix_bytes(int rows, int cols) {
 extern "C" int sfnx_quantize_f8(uint32_t type, const void* x, int64_t ldx, int rows, int cols, uint8_t* q, float* s, void* st) {
     return guarded("sfnx_quantize_f8", [&] {
         require(out_type_ok(type), "x type must be F32 (0), F16 (1) or BF16 (30)");
-        require(cols > 0 && cols % 16 == 0, "cols must be a multiple of 16");
-        require(rows >= 0, "rows out of range");
+        require(cols > 0 && cols % 16 == 0 && cols <= (1 << 20), "cols must be a multiple of 16, at most 2^20");
+        require(rows >= 0 && rows <= (1 << 24), "rows out of range");
         require(ldx >= cols && ldx % 16 == 0, "ldx must be a multiple of 16, at least cols");
         if (rows == 0) return;
         require(x != nullptr && q != nullptr && s != nullptr, "null pointer");
         require(al16(x) && al16(q), ALIGN_MSG);
-        const int64_t items = (int64_t) rows * blocks_of(cols);
-        const unsigned grid = (unsigned) std::min<int64_t>((items + 7) / 8, 1 << 16);
         hipStream_t h = stream_of(st);
-        if (type == SFNX_F32) k_quantize_f8<SFNX_F32><<<grid, 256, 0, h>>>(x, ldx, rows, cols, q, s);
-        else if (type == SFNX_F16) k_quantize_f8<SFNX_F16><<<grid, 256, 0, h>>>(x, ldx, rows, cols, q, s);
-        else k_quantize_f8<SFNX_BF16><<<grid, 256, 0, h>>>(x, ldx, rows, cols, q, s);
+        if (type == SFNX_F32) quantize<SFNX_F32>(x, ldx, rows, cols, q, s, h);
+        else if (type == SFNX_F16) quantize<SFNX_F16>(x, ldx, rows, cols, q, s, h);
+        else quantize<SFNX_BF16>(x, ldx, rows, cols, q, s, h);
     });
 }
 
@@ -109,17 +178,9 @@ extern "C" int sfnx_f8_gemm(const void* W, int rows, int cols, const uint8_t* xq
         check_out(out, out_type);
         Args a{(const uint8_t*) W, sfnx_f8_matrix_bytes(rows, cols), cols, rows, nullptr, nullptr, C, xq, xs, out, nullptr, out_type, ldo,
                vec_ok(out, out_type, ldo)};
-        if (getenv("SFNX_MID")) {
-            int v = atoi(getenv("SFNX_MID"));
-            hipStream_t h = stream_of(st);
-            if (out_type == SFNX_F32) { if (v == 42) launch_mid_as<F8X, 4, 2>(a, h); if (v == 41) launch_mid_as<F8X, 4, 1>(a, h); if (v == 22) launch_mid_as<F8X, 2, 2>(a, h); if (v == 21) launch_mid_as<F8X, 2, 1>(a, h); if (v==44) launch_mid_as<F8X,4,4>(a,h); }
-            else { if (v == 44) launch_mid_as<F8, 4, 4>(a, h); if (v == 42) launch_mid_as<F8, 4, 2>(a, h); if (v == 41) launch_mid_as<F8, 4, 1>(a, h); if (v == 22) launch_mid_as<F8, 2, 2>(a, h); if (v == 24) launch_mid_as<F8, 2, 4>(a, h); if (v==21) launch_mid_as<F8,2,1>(a,h); }
-            if (v == 3) { if (out_type == SFNX_F32) launch_narrow<F8X>(a, (C + 63) / 64, h); else launch_narrow<F8>(a, (C + 63) / 64, h); }
-            if (v > 2) return;
-        }
         if (C <= FEW_M) launch_few<F8X, STORE, false>(a, 1, stream_of(st));
-        else if (out_type == SFNX_F32) launch_tiles<F8X, STORE>(a, (C + BM1 - 1) / BM1, stream_of(st));
-        else launch_tiles<F8, STORE>(a, (C + BM1 - 1) / BM1, stream_of(st));
+        else if (out_type == SFNX_F32) dense_many<F8X>(a, stream_of(st));
+        else dense_many<F8>(a, stream_of(st));
     });
 }
 
@@ -164,7 +225,7 @@ extern "C" int sfnx_moe_gate_up_swiglu_f8_big(const void* A, size_t sa, int n_in
         check_f8_rows(xq, xs);
         check_f8_rows(hq, hs);
         Args a{(const uint8_t*) A, sa, n_in, 2 * ff, jobs, njobs, 0, xq, xs, hq, hs, SFNX_F32, ff, 1};
-        launch_tiles<F8X, SWIGLU>(a, njobs_cap, stream_of(st));
+        launch_tiles<F8X, SWIGLU>(a, njobs_cap, false, stream_of(st));
     });
 }
 
@@ -177,7 +238,7 @@ extern "C" int sfnx_moe_down_f8_big(const void* A, size_t sa, int n_in, int n_ou
         check_f8_rows(hq, hs);
         check_out(out, out_type);
         Args a{(const uint8_t*) A, sa, n_in, n_out, jobs, njobs, 0, hq, hs, out, nullptr, out_type, n_out, vec_ok(out, out_type, n_out)};
-        if (out_type == SFNX_F32) launch_tiles<F8X, STORE>(a, njobs_cap, stream_of(st));
-        else launch_tiles<F8, STORE>(a, njobs_cap, stream_of(st));
+        if (out_type == SFNX_F32) launch_tiles<F8X, STORE>(a, njobs_cap, false, stream_of(st));
+        else launch_tiles<F8, STORE>(a, njobs_cap, false, stream_of(st));
     });
 }

@@ -15,7 +15,6 @@
 #pragma once
 
 #include <algorithm>
-#include <cstdlib>
 #include <type_traits>
 
 #include "common.hpp"
@@ -102,28 +101,41 @@ __device__ __forceinline__ const float* scales_of(const uint8_t* mat, int rows, 
 // s = max(max |x| c, 2^-126) over a block's finite values, c = 1 / 448 rounded to fp32; q = e4m3(x / s), one rounding of the
 // fp32 quotient, at most 448 in size.  The floor of s keeps the quotient of a block of zeros (or of values below 448 2^-126) defined.  What is not
 // finite becomes the type's NaN.
-__device__ __forceinline__ float finite_abs(float v) {
-    const float a = fabsf(v);
-    return a < __builtin_inff() ? a : 0.f;   // NaN compares false
+//
+// The quotient: with r = 1 / s rounded, x r is within a unit of x / s, and adding (x - (x r) s) r, both products fused, rounds
+// it correctly (Markstein): three instructions for a division's ten.  The remainder has to stay above the smallest numbers,
+// so scales below 2^-90 divide; so do blocks with values that are not finite.
+__device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }   // not finite: 0x7f800000 on
+struct F8Scale {
+    float s, r;
+    bool plain;   // by division, value by value
+};
+__device__ __forceinline__ float finite_abs(float v) { return abs_bits(v) < 0x7f800000u ? fabsf(v) : 0.f; }
+// amax: over the block's finite values; all_finite: whether there are others
+__device__ __forceinline__ F8Scale f8_scale(float amax, bool all_finite) {
+    const float s = fmaxf(amax * F8_INV, S_MIN);
+    return F8Scale{s, 1.f / s, !all_finite || s < 0x1p-90f};
 }
-__device__ __forceinline__ float f8_scale(float amax) { return fmaxf(amax * F8_INV, S_MIN); }
-__device__ __forceinline__ uint32_t f8_pack4(float a, float b, float c, float d, float s) {
+__device__ __forceinline__ uint32_t f8_pack4(float a, float b, float c, float d, const F8Scale& k) {
     const float v[4] = {a, b, c, d};
     float t[4];
-    uint32_t nan = 0;
+    if (!k.plain) {   // at most 448 (1 + 2^-22), which rounds to 448
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        t[i] = fminf(fmaxf(v[i] / s, -F8_MAX), F8_MAX);
-        if (!(fabsf(v[i]) < __builtin_inff())) nan |= 0x7fu << (8 * i);
+        for (int i = 0; i < 4; ++i) {
+            const float q = v[i] * k.r;
+            t[i] = fmaf(fmaf(-q, k.s, v[i]), k.r, q);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) t[i] = fminf(fmaxf(v[i] / k.s, -F8_MAX), F8_MAX);
     }
     int r = __builtin_amdgcn_cvt_pk_fp8_f32(t[0], t[1], 0, false);
     r = __builtin_amdgcn_cvt_pk_fp8_f32(t[2], t[3], r, true);
     uint32_t u = (uint32_t) r;
-    if (nan) {
+    if (k.plain)
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-            if ((nan >> (8 * i)) & 0xff) u = (u & ~(0xffu << (8 * i))) | (0x7fu << (8 * i));
-    }
+            if (abs_bits(v[i]) >= 0x7f800000u) u = (u & ~(0xffu << (8 * i))) | (0x7fu << (8 * i));
     return u;
 }
 

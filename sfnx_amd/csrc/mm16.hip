@@ -12,6 +12,7 @@ Args mm16_args(const void* A, size_t sa, uint32_t type, int n_in, int n_out, con
     require(out_type_ok(out_type), "out type must be F32 (0), F16 (1) or BF16 (30)");
     require(n_in > 0 && n_in % 8 == 0 && n_in <= (1 << 20), "input width must be a multiple of 8, at most 2^20");
     require(n_out > 0 && n_out <= (1 << 20), "n_out out of range");
+    require(2 * (uint64_t) n_out * n_in < ((uint64_t) 1 << 32), "a matrix must be smaller than 4 GiB");
     require(stride_ok(sa, 2 * (size_t) n_out * n_in), "expert stride smaller than a matrix");
     require(sa % 16 == 0, "expert stride must be a multiple of 16");
     require(cap >= 0 && cap <= (1 << 20), "njobs out of range");
@@ -42,7 +43,7 @@ extern "C" int sfnx_moe_mm_16_big(const void* A, size_t sa, uint32_t type, int n
     return guarded("sfnx_moe_mm_16_big", [&] {
         const Args a = mm16_args(A, sa, type, n_in, n_out, jobs, njobs, njobs_cap, x, out_type, out);
         if (njobs_cap == 0) return;
-        if (type == SFNX_F16) launch_tiles<F16, STORE>(a, njobs_cap, stream_of(st));
-        else launch_tiles<BF16, STORE>(a, njobs_cap, stream_of(st));
+        if (type == SFNX_F16) launch_tiles<F16, STORE>(a, njobs_cap, false, stream_of(st));
+        else launch_tiles<BF16, STORE>(a, njobs_cap, false, stream_of(st));
     });
 }

@@ -64,10 +64,12 @@ __global__ void __launch_bounds__(FEW_THREADS) k_mm_few(Args a) {
             const int yy = a.dense_c > 0 ? m : jb->y[m];
             float4 v = {0, 0, 0, 0};
             if (k < a.n_in) v = *reinterpret_cast<const float4*>(h + (size_t) yy * a.n_in + k);
+            const uint32_t top = max(max(abs_bits(v.x), abs_bits(v.y)), max(abs_bits(v.z), abs_bits(v.w)));
+            const bool fin = (uint32_t) group_reduce<32>((int) top, [](int a, int b) { return max(a, b); }) < 0x7f800000u;
             const float am = group_max<32>(fmaxf(fmaxf(finite_abs(v.x), finite_abs(v.y)), fmaxf(finite_abs(v.z), finite_abs(v.w))));
-            const float s = f8_scale(am);
+            const F8Scale s = f8_scale(am, fin);
             *reinterpret_cast<uint32_t*>(hq + m * pitch + k) = f8_pack4(v.x, v.y, v.z, v.w, s);
-            if (c == 0) hs[m * nb + b] = s;
+            if (c == 0) hs[m * nb + b] = s.s;
         }
         lds_barrier();
     }

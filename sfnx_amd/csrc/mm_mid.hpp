@@ -83,7 +83,7 @@ template <Elem EL, int MT, int NT> __global__ void __launch_bounds__(MID_THREADS
     }
 }
 
-template <Elem EL, int MT, int NT> void launch_mid_as(const Args& a, hipStream_t s) {
+template <Elem EL, int MT, int NT> void launch_mid(const Args& a, hipStream_t s) {
     const int nsl = (a.n_out + 16 * NT - 1) / (16 * NT), rows = (a.dense_c + 16 * MT - 1) / (16 * MT);
     k_mm_mid<EL, MT, NT><<<grid_of(nsl, rows, MID_THREADS), MID_THREADS, MID_LDS<MT, NT>, s>>>(a);
 }

@@ -71,6 +71,7 @@ __device__ __forceinline__ void swiglu_out(const Args& a, float4v (&acc)[2 * NT]
     for (int j = 0; j < MT; ++j) {
         if (16 * j >= n) continue;
         float am = 0.f;
+        int odd = 0;   // a value that is not finite
 #pragma unroll
         for (int u = 0; u < NT; ++u)
 #pragma unroll
@@ -78,10 +79,13 @@ __device__ __forceinline__ void swiglu_out(const Args& a, float4v (&acc)[2 * NT]
                 const bool in = sl * BLK + 16 * (NT * wn + u) < n_eff;   // FF is a multiple of 16
                 acc[u][j][i] = in ? silu_f(acc[u][j][i]) * acc[NT + u][j][i] : 0.f;
                 am = fmaxf(am, finite_abs(acc[u][j][i]));
+                odd |= abs_bits(acc[u][j][i]) >= 0x7f800000u;
             }
         am = fmaxf(am, lane_xor<16>(am));
         am = fmaxf(am, lane_xor<32>(am));
-        if (q == 0) mx[wn * M + m0 + 16 * j + r] = am;
+        odd |= lane_xor<16>(odd);
+        odd |= lane_xor<32>(odd);
+        if (q == 0) mx[wn * M + m0 + 16 * j + r] = odd ? -1.f - am : am;   // below zero: not all finite
     }
     lds_barrier();
 #pragma unroll
@@ -89,14 +93,19 @@ __device__ __forceinline__ void swiglu_out(const Args& a, float4v (&acc)[2 * NT]
         if (16 * j >= n) continue;
         const int m = 16 * j + r;
         float am = 0.f;
+        bool fin = true;
 #pragma unroll
-        for (int w = 0; w < WN; ++w) am = fmaxf(am, mx[w * M + m0 + m]);
-        const float s = f8_scale(am);
+        for (int w = 0; w < WN; ++w) {
+            const float v = mx[w * M + m0 + m];
+            am = fmaxf(am, v < 0.f ? -1.f - v : v);
+            fin = fin && v >= 0.f;
+        }
+        const F8Scale s = f8_scale(am, fin);
 #pragma unroll
         for (int u = 0; u < NT; ++u)
             *reinterpret_cast<uint32_t*>(hb + (m0 + m) * HP + 16 * (NT * wn + u) + 4 * q) =
                 f8_pack4(acc[u][j][0], acc[u][j][1], acc[u][j][2], acc[u][j][3], s);
-        if (wn == 0 && q == 0 && m < n) a.out_s[out_row(m0 + m) * blocks_of(n_eff) + sl] = s;
+        if (wn == 0 && q == 0 && m < n) a.out_s[out_row(m0 + m) * blocks_of(n_eff) + sl] = s.s;
     }
     lds_barrier();
     for (int i = threadIdx.x; i < M * 8; i += TT) {
@@ -514,17 +523,15 @@ template <Elem EL> __global__ void __launch_bounds__(TT, 2) k_mm_narrow(Args a, 
 template <Elem EL> void launch_narrow(const Args& a, int jobs, hipStream_t s) {
     const int64_t tiles = tiles_of((a.n_out + 127) / 128, jobs);
     require(tiles < (1 << 30), "too many jobs for one launch");
-    require((uint64_t) a.n_out * a.n_in * ESZ<EL> < ((uint64_t) 1 << 32), "a matrix must be smaller than 4 GiB");
     k_mm_narrow<EL><<<(unsigned) std::min<int64_t>(tiles, CUS), TT, Stream<1>::LDS, s>>>(a, jobs);
 }
 
-template <Elem EL, Mode MODE> void launch_tiles(Args a, int njobs_cap, hipStream_t s) {
-    require((uint64_t) a.n_out * a.n_in * ESZ<EL> < ((uint64_t) 1 << 32), "a matrix must be smaller than 4 GiB");
+// group: of a dense product, whether its tiles are groups; a grouped product's jobs say so themselves
+template <Elem EL, Mode MODE> void launch_tiles(Args a, int njobs_cap, bool group, hipStream_t s) {
     a.slices = (a.n_out + BN - 1) / BN;
     const int64_t tiles = tiles_of(a.slices, njobs_cap);
     require(tiles < (1 << 30), "too many jobs for one launch");
-    const int group = getenv("SFNX_MID") && atoi(getenv("SFNX_MID")) > 0 ? atoi(getenv("SFNX_MID")) - 1 : a.dense_c > 0 && (int64_t) a.slices * ((njobs_cap + GJ - 1) / GJ) >= CUS / 2;
-    k_mm_tiles<EL, MODE><<<(unsigned) std::min<int64_t>(tiles, CUS), TT, T_LDS + 64, s>>>(a, njobs_cap, group);
+    k_mm_tiles<EL, MODE><<<(unsigned) std::min<int64_t>(tiles, CUS), TT, T_LDS + 64, s>>>(a, njobs_cap, (int) group);
 }
 
 }  // namespace mm
