@@ -21,7 +21,7 @@ __device__ __forceinline__ Frag load_frag(const uint8_t* row, int k0, int q, int
 // tile and its up tile) and the steps wk, wk + WK, ... of K.  The partial sums meet in LDS and are added in wavefront order.
 // QH: x holds fp32 rows, quantized here into LDS (each block quantizes the job's rows: a few thousand values).
 template <Elem EL, Mode MODE, int WK, bool QH>
-__global__ void __launch_bounds__(FEW_THREADS) k_mm_few(Args a) {
+__global__ void __launch_bounds__(FEW_THREADS, EL == F8X && !QH ? 6 : 8) k_mm_few(Args a) {
     constexpr int WR = FEW_WAVES / WK, ROWS = MODE == SWIGLU ? 16 * WR : 32 * WR;   // output values of a block
     __shared__ float red[WK][WR][2][FEW_M][16];
     extern __shared__ __align__(16) uint8_t hq[];   // QH: [16][pitch] e4m3, then [16][blocks] scales
@@ -34,12 +34,12 @@ __global__ void __launch_bounds__(FEW_THREADS) k_mm_few(Args a) {
     if (a.dense_c > 0) {
         n = a.dense_c;
         y = min(r, n - 1);
-    } else {
-        if (ji >= *a.njobs) return;
-        n = min(jb->n, FEW_M);
-        if (n <= 0) return;
-        e = jb->w;
-        y = jb->y[min(r, n - 1)];
+    } else {   // the job's fields at once with the count that says whether it is one; a lane without a row takes the first
+        const int nj = *a.njobs, yr = jb->y[r], y0 = jb->y[0];
+        n = __builtin_amdgcn_readfirstlane(min(jb->n, FEW_M));
+        e = __builtin_amdgcn_readfirstlane(jb->w);
+        if (ji >= nj || n <= 0) return;
+        y = r < n ? yr : y0;
     }
     const uint8_t* mat = expert_at(a.A, a.sa, e);
     const int rb = a.n_in * ESZ<EL>, steps = (rb + STEP - 1) / STEP, nb = blocks_of(a.n_in);
@@ -55,6 +55,11 @@ __global__ void __launch_bounds__(FEW_THREADS) k_mm_few(Args a) {
         wrow[t] = mat + (size_t) min(row0[t] + r, a.n_out - 1) * rb;
         if (IS8<EL>) ws[t] = scales_of(mat, a.n_out, a.n_in) + (size_t) (row0[t] / BLK) * nb;
     }
+    // QH: the first step's weights are on their way while the job's rows are quantized
+    Frag w0[2];
+    if (QH && wk < steps)
+#pragma unroll
+        for (int t = 0; t < 2; ++t) w0[t] = load_frag(wrow[t], wk * STEP, q, rb);
     const int pitch = steps * STEP + 16;
     float* hs = reinterpret_cast<float*>(hq + 16 * pitch);
     if constexpr (QH) {   // half a wavefront a block of 128 values
@@ -73,7 +78,7 @@ __global__ void __launch_bounds__(FEW_THREADS) k_mm_few(Args a) {
         }
         lds_barrier();
     }
-    const int m = min(r, n - 1);
+    const int m = r < n ? r : 0;
     const uint8_t* xrow = QH ? hq + m * pitch : a.x + (size_t) y * rb;
     const float* xs = QH ? hs + m * nb : a.xs + (size_t) y * nb;
     float4v acc[2] = {};
@@ -86,8 +91,10 @@ __global__ void __launch_bounds__(FEW_THREADS) k_mm_few(Args a) {
             x = load_frag(xrow, s * STEP, q, rb);
         }
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
-            acc[t] = step_mma<EL>(operand<EL>(load_frag(wrow[t], s * STEP, q, rb)), operand<EL>(x), acc[t], IS8<EL> ? xs[s] * ws[t][s] : 1.f);
+        for (int t = 0; t < 2; ++t) {
+            const Frag w = QH && s == wk ? w0[t] : load_frag(wrow[t], s * STEP, q, rb);
+            acc[t] = step_mma<EL>(operand<EL>(w), operand<EL>(x), acc[t], IS8<EL> ? xs[s] * ws[t][s] : 1.f);
+        }
     }
 #pragma unroll
     for (int t = 0; t < 2; ++t) *reinterpret_cast<float4v*>(&red[wk][wr][t][r][4 * q]) = acc[t];
