@@ -35,10 +35,11 @@ constexpr int T_LDS = SG_LIST + 2 * WINDOW > S1_LDS ? SG_LIST + 2 * WINDOW : S1_
 static_assert(T_LDS + 64 <= 160 * 1024 && 4 * WINDOW <= SG_LIST && 2 * BMG * 4 + BMG * HP <= SG_LIST, "LDS");
 
 // Workgroup b runs on XCD b % 8: the slices of xg consecutive groups (an expert's jobs are consecutive) go to one XCD, so
-// an expert's weights come from HBM once for them; xg = 4, or 1 where there are too few to use all XCDs evenly.  false: no
+// an expert's weights come from HBM once for them; xg = XG, or 1 where there are too few to use all XCDs evenly (single jobs, few
+// of one expert, 2 for 4: down of 777 tokens 129 -> 124 us; groups 4 for 1: bf16 experts of 4096 tokens 307 -> 297).  false: no
 // such group
-__device__ __forceinline__ bool tile_at(int b, int nsl, int n, int& sl, int& i) {
-    const int xg = n >= 64 ? 4 : 1;
+template <int XG> __device__ __forceinline__ bool tile_at(int b, int nsl, int n, int& sl, int& i) {
+    const int xg = n >= 64 ? XG : 1;
     const int x = b % XCDS, k = b / XCDS, m = k / nsl;
     sl = k % nsl;
     i = xg * (XCDS * (m / xg) + x) + m % xg;
@@ -135,7 +136,7 @@ template <Elem EL, Mode MODE, int NT> __device__ __forceinline__ void stream_til
 
     auto next_tile = [&](int b, int& sl, int& ji) {   // the first tile of this workgroup from b on; its number, or -1
         for (; b < tiles; b += grid)
-            if (tile_at(b, nsl, nj, sl, ji)) return b;
+            if (tile_at<2>(b, nsl, nj, sl, ji)) return b;
         return -1;
     };
     auto slot_of = [&](int c) { return reinterpret_cast<const int*>(lds + Stream<NT>::JOBS + (c % S1_SLOTS) * S1_SLOT); };
@@ -504,7 +505,7 @@ template <Elem EL, Mode MODE> __global__ void __launch_bounds__(TT, 2) k_mm_tile
         const int tiles = (int) tiles_of(a.slices, n);
         for (int b = blockIdx.x; b < tiles; b += gridDim.x) {
             int sl, i;
-            if (!tile_at(b, a.slices, n, sl, i)) continue;
+            if (!tile_at<4>(b, a.slices, n, sl, i)) continue;
             i = n - 1 - i;   // the last group first: the shared expert's
             const int j0 = dense ? GJ * i : list[i], j1 = dense ? min(j0 + GJ, count) : i + 1 < n ? list[i + 1] : count;
             if (j1 - j0 > 2) group_tile<EL, MODE, 4>(a, sl, w0 + j0, j1 - j0, lds);
