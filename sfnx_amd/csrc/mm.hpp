@@ -197,21 +197,27 @@ __device__ __forceinline__ const uint8_t* uniform_ptr(const uint8_t* p) {
     return (const uint8_t*) ((uint64_t) hi << 32 | lo);
 }
 
-// Copies to LDS that a caller spreads among its matrix instructions: issued all at once they hold up the wavefront until the
-// address unit has taken them (about 35 cycles each).  As lds_copy_async, but no compiler barrier, so LDS reads of other
-// places move across them; the order against vm_wait and lds_barrier stays.  lds: wave-uniform; lane l's bytes land at lds + 16 l
-// (copy4: 4 l).  copy16's address is a uniform base and a lane's 32-bit offset, or a lane's pointer.
-__device__ __forceinline__ uint32_t lds_address(const void* lds) {
-    return __builtin_amdgcn_readfirstlane((uint32_t) reinterpret_cast<uintptr_t>((const __attribute__((address_space(3))) void*) lds));
+// Copies to LDS as lds_copy_async, but no compiler barrier, so LDS reads of other places move across them; the order against
+// vm_wait and lds_barrier stays.  to: a wave-uniform LDS address (Lds::at); lane l's bytes land at to + 16 l (copy4: 4 l).
+// copy16's source is a uniform base and a lane's 32-bit offset, or a lane's pointer.
+__device__ __forceinline__ void copy16(const uint8_t* base, uint32_t off, uint32_t to) {
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(to) : "m0");
 }
-__device__ __forceinline__ void copy16(const uint8_t* base, uint32_t off, const void* lds) {
-    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(lds_address(lds)) : "m0");
+__device__ __forceinline__ void copy16(const uint8_t* p, uint32_t to) {
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(p), "s"(to) : "m0");
 }
-__device__ __forceinline__ void copy16(const uint8_t* p, const void* lds) {
-    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(p), "s"(lds_address(lds)) : "m0");
+__device__ __forceinline__ void copy4(const void* p, uint32_t to) {
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(p), "s"(to) : "m0");
 }
-__device__ __forceinline__ void copy4(const void* p, const void* lds) {
-    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(p), "s"(lds_address(lds)) : "m0");
+// a workgroup's LDS, as a pointer to read through and as the address copies take: cast once, where the compiler sees the array
+// itself (a generic pointer's cast tests it for null each time)
+struct Lds {
+    uint8_t* p;
+    uint32_t base;
+    __device__ __forceinline__ uint32_t at(const void* q) const { return base + (uint32_t) ((const uint8_t*) q - p); }
+};
+__device__ __forceinline__ Lds lds_of(uint8_t* p) {
+    return Lds{p, (uint32_t) reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) uint8_t*) p)};
 }
 
 enum Mode { STORE, SWIGLU };

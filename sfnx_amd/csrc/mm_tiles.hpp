@@ -123,7 +123,8 @@ __device__ __forceinline__ void swiglu_out(const Args& a, float4v (&acc)[2 * NT]
 // the ends of tiles too, so no tile waits for its first weights.  The descriptions of later jobs come by asynchronous copies
 // as well: a load the compiler waits for would drain the stream.  A wavefront owns 32 of the tile's weight rows for all of
 // the job's rows.
-template <Elem EL, Mode MODE, int NT> __device__ __forceinline__ void stream_tiles(const Args& a, int nj, uint8_t* lds) {
+template <Elem EL, Mode MODE, int NT> __device__ __forceinline__ void stream_tiles(const Args& a, int nj, const Lds& L) {
+    uint8_t* const lds = L.p;
     constexpr int KS = Stream<NT>::KS, D = Stream<NT>::STAGES, N = 128 * NT;
     constexpr int REQ = KS * (2 * NT + 1 + (IS8<EL> ? 2 : 0));   // copies a wavefront issues for a stage
     typedef typename Stream<NT>::S S;
@@ -144,7 +145,7 @@ template <Elem EL, Mode MODE, int NT> __device__ __forceinline__ void stream_til
         if (dense) return;
         const int* src = reinterpret_cast<const int*>(jobs + (nj - 1 - ji));   // the last job first: the shared expert's are the longest
 #pragma unroll
-        for (int i = 0; i < 3; ++i) lds_copy_async<4>(src + min(64 * i + lane, 129), slot_of(c) + 64 * i);
+        for (int i = 0; i < 3; ++i) copy4(src + min(64 * i + lane, 129), L.at(slot_of(c) + 64 * i));
     };
     auto job_rows = [&](int c, int ji) {
         return __builtin_amdgcn_readfirstlane(dense ? min(BM1, a.dense_c - BM1 * ji) : min(slot_of(c)[1], BM1));
@@ -187,18 +188,18 @@ template <Elem EL, Mode MODE, int NT> __device__ __forceinline__ void stream_til
             const uint8_t* x = xsrc + k;
             if (k + STEP <= rb) {
 #pragma unroll
-                for (int i = 0; i < 2 * NT; ++i) copy16(uniform_ptr(wbase + k), woff[i], buf + (16 * NT * wave + 8 * i) * STEP);
+                for (int i = 0; i < 2 * NT; ++i) copy16(uniform_ptr(wbase + k), woff[i], L.at(buf + (16 * NT * wave + 8 * i) * STEP));
             } else {   // zero past the rows' end
                 const bool in = k + 16 * p8 < rb;
 #pragma unroll
                 for (int i = 0; i < 2 * NT; ++i)
-                    copy16(in ? wbase + k + woff[i] : (const uint8_t*) &ZERO16, buf + (16 * NT * wave + 8 * i) * STEP);
+                    copy16(in ? wbase + k + woff[i] : (const uint8_t*) &ZERO16, L.at(buf + (16 * NT * wave + 8 * i) * STEP));
                 if (!in) x = (const uint8_t*) &ZERO16;
             }
-            copy16(x, buf + S::X + 8 * wave * STEP);
+            copy16(x, L.at(buf + S::X + 8 * wave * STEP));
             if constexpr (IS8<EL>) {   // every wavefront copies them all: the same values, and each counts the same requests
-                copy4(xs_src + s, buf + S::XS);
-                copy4(ws_src + s, buf + S::WS);
+                copy4(xs_src + s, L.at(buf + S::XS));
+                copy4(ws_src + s, L.at(buf + S::WS));
             }
         }
         ps += KS;
@@ -225,26 +226,34 @@ template <Elem EL, Mode MODE, int NT> __device__ __forceinline__ void stream_til
                 else vm_wait<0>();
                 lds_barrier();   // every wavefront's copies of this stage landed, and every wavefront is past the one before
                 const uint8_t* stage = lds + at * KS * S::SIZE;
-                ahead += (int) produce(lds + (at == 0 ? D - 1 : at - 1) * KS * S::SIZE) - 1;
+                uint8_t* to = lds + (at == 0 ? D - 1 : at - 1) * KS * S::SIZE;
                 at = at == D - 1 ? 0 : at + 1;
 #pragma unroll
                 for (int h = 0; h < KS; ++h) {
                     if (h > 0 && s + h >= steps) break;
                     const uint8_t* buf = stage + h * S::SIZE;
-                    Operand<EL> w[NT];
-                    float ws[NT];
+                    // the next stage's copies go out while the first reads come in
+                    Frag w[NT], x[MT];
+                    float ws[NT], xs[MT];
 #pragma unroll
                     for (int t = 0; t < NT; ++t) {
-                        w[t] = operand<EL>(lds_frag(buf, 16 * NT * wave + 16 * t + r, q));
-                        if constexpr (IS8<EL>) ws[t] = reinterpret_cast<const float*>(buf + S::WS)[NT * wave + t];
+                        w[t] = lds_frag(buf, 16 * NT * wave + 16 * t + r, q);
+                        ws[t] = IS8<EL> ? reinterpret_cast<const float*>(buf + S::WS)[NT * wave + t] : 1.f;
                     }
 #pragma unroll
                     for (int j = 0; j < MT; ++j) {
-                        const Operand<EL> x = operand<EL>(lds_frag(buf + S::X, 16 * j + r, q));
-                        float xs = 1.f;
-                        if constexpr (IS8<EL>) xs = reinterpret_cast<const float*>(buf + S::XS)[16 * j + r];
+                        x[j] = lds_frag(buf + S::X, 16 * j + r, q);
+                        xs[j] = IS8<EL> ? reinterpret_cast<const float*>(buf + S::XS)[16 * j + r] : 1.f;
+                    }
+                    if (h == 0) ahead += (int) produce(to) - 1;
+                    Operand<EL> wo[NT];
 #pragma unroll
-                        for (int t = 0; t < NT; ++t) acc[t][j] = step_mma<EL>(w[t], x, acc[t][j], IS8<EL> ? xs * ws[t] : 1.f);
+                    for (int t = 0; t < NT; ++t) wo[t] = operand<EL>(w[t]);
+#pragma unroll
+                    for (int j = 0; j < MT; ++j) {
+                        const Operand<EL> xo = operand<EL>(x[j]);
+#pragma unroll
+                        for (int t = 0; t < NT; ++t) acc[t][j] = step_mma<EL>(wo[t], xo, acc[t][j], xs[j] * ws[t]);
                     }
                 }
             }
@@ -279,7 +288,8 @@ template <Elem EL, Mode MODE, int NT> __device__ __forceinline__ void stream_til
 // ------------------------------------------------------------------------------------------------ a group of jobs a tile
 // A wavefront owns a job's 64 rows and NT of the tile's 16 weight tiles: of a group of C jobs (3 are taken as 4), 8 / C wavefronts
 // share a job.
-template <Elem EL, Mode MODE, int C> __device__ __forceinline__ void group_tile(const Args& a, int sl, int j0, int count, uint8_t* lds) {
+template <Elem EL, Mode MODE, int C> __device__ __forceinline__ void group_tile(const Args& a, int sl, int j0, int count, const Lds& L) {
+    uint8_t* const lds = L.p;
     constexpr int WN = TW / C, NT = 16 / WN;
     typedef Stage<BM1 * C> S;
     const int lane = threadIdx.x % WAVE, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
@@ -329,13 +339,13 @@ template <Elem EL, Mode MODE, int C> __device__ __forceinline__ void group_tile(
     // the last step that again
     auto copy = [&](int u, int s, uint8_t* buf) {
         const uint32_t k = (uint32_t) min(min(s, steps - 1) * STEP + 16 * p8, rb - 16);
-        if (u < 4) copy16(mat, woff[u] + k, buf + wto[u] * STEP);
-        else copy16(xsrc[u - 4] + k, buf + S::X + 8 * (C * wave + u - 4) * STEP);
+        if (u < 4) copy16(mat, woff[u] + k, L.at(buf + wto[u] * STEP));
+        else copy16(xsrc[u - 4] + k, L.at(buf + S::X + 8 * (C * wave + u - 4) * STEP));
     };
     auto copy_scales = [&](int s, uint8_t* buf) {
         if constexpr (IS8<EL>) {
-            copy4(xs_src + min(s, steps - 1), buf + S::XS + 256 * wm);
-            copy4(ws_src + min(s, steps - 1), buf + S::WS);
+            copy4(xs_src + min(s, steps - 1), L.at(buf + S::XS + 256 * wm));
+            copy4(ws_src + min(s, steps - 1), L.at(buf + S::WS));
         }
     };
     auto copy_early = [&](int s, uint8_t* buf) {
@@ -493,6 +503,7 @@ __device__ __forceinline__ int list_groups(const sfnx_bigjob* jobs, int w0, int 
 // which the jobs themselves say
 template <Elem EL, Mode MODE> __global__ void __launch_bounds__(TT, 2) k_mm_tiles(Args a, int cap, int group) {
     extern __shared__ __align__(16) uint8_t lds[];
+    const Lds L = lds_of(lds);
     const bool dense = a.dense_c > 0;
     const int nj = dense ? cap : min(*a.njobs, cap);
     const sfnx_bigjob* jobs = (const sfnx_bigjob*) a.jobs;
@@ -508,18 +519,18 @@ template <Elem EL, Mode MODE> __global__ void __launch_bounds__(TT, 2) k_mm_tile
             if (!tile_at<4>(b, a.slices, n, sl, i)) continue;
             i = n - 1 - i;   // the last group first: the shared expert's
             const int j0 = dense ? GJ * i : list[i], j1 = dense ? min(j0 + GJ, count) : i + 1 < n ? list[i + 1] : count;
-            if (j1 - j0 > 2) group_tile<EL, MODE, 4>(a, sl, w0 + j0, j1 - j0, lds);
-            else if (j1 - j0 == 2) group_tile<EL, MODE, 2>(a, sl, w0 + j0, 2, lds);
-            else group_tile<EL, MODE, 1>(a, sl, w0 + j0, 1, lds);
+            if (j1 - j0 > 2) group_tile<EL, MODE, 4>(a, sl, w0 + j0, j1 - j0, L);
+            else if (j1 - j0 == 2) group_tile<EL, MODE, 2>(a, sl, w0 + j0, 2, L);
+            else group_tile<EL, MODE, 1>(a, sl, w0 + j0, 1, L);
         }
     }
-    if (!group) stream_tiles<EL, MODE, 2>(a, nj, lds);
+    if (!group) stream_tiles<EL, MODE, 2>(a, nj, L);
 }
 
 // a dense product in streamed tiles of 64 x 128
 template <Elem EL> __global__ void __launch_bounds__(TT, 2) k_mm_narrow(Args a, int jobs) {
     extern __shared__ __align__(16) uint8_t lds[];
-    stream_tiles<EL, STORE, 1>(a, jobs, lds);
+    stream_tiles<EL, STORE, 1>(a, jobs, lds_of(lds));
 }
 template <Elem EL> void launch_narrow(const Args& a, int jobs, hipStream_t s) {
     const int64_t tiles = tiles_of((a.n_out + 127) / 128, jobs);
