@@ -1,4 +1,6 @@
-// Products of few rows (jobs of up to 16): the weight stream alone counts, each weight byte is used once.
+// Products of few rows (jobs of up to 16): the weight stream alone counts, each weight byte is used once.  Bound by HBM where
+// there are many jobs (16 tokens: 5.2 TB/s of gate|up weights, 4.5 of down's), by the chain of dependent loads (job, its
+// weights) and the launch where there are few (one token: 8 us, of which the host's call takes 6).
 #pragma once
 
 #include "mm.hpp"
@@ -119,7 +121,10 @@ __global__ void __launch_bounds__(FEW_THREADS, EL == F8X && !QH ? 6 : 8) k_mm_fe
     }
 }
 
-// WK: as many wavefronts along K as there are steps, for the shortest chain and the most blocks
+// WK: as many wavefronts along K as there are steps, for the shortest chain and the most blocks; where each block quantizes the
+// job's rows, half as many, for blocks of twice the rows.  gate|up (2048 columns, 16 steps) with 8, 4, 2 along K: one token 9.2,
+// 9.5, 12.3 us, 16 tokens (133 jobs) 53, 55, 58; down (512 columns, 4 steps) with 4, 2, 1: one token 8.0, 7.7, 8.2, 16 tokens 35,
+// 32, 32; f16 experts of 2048 columns as gate|up (101, 109, 112 us at 16 tokens, 5.4 TB/s of weights).
 template <Elem EL, Mode MODE, bool QH> void launch_few(const Args& a, int njobs_cap, hipStream_t s) {
     const int steps = (a.n_in * ESZ<EL> + STEP - 1) / STEP, n_eff = MODE == SWIGLU ? a.n_out / 2 : a.n_out;
     const int per = MODE == SWIGLU ? 16 : 32;
@@ -129,9 +134,10 @@ template <Elem EL, Mode MODE, bool QH> void launch_few(const Args& a, int njobs_
         const int rows = per * (FEW_WAVES / WK);
         k_mm_few<EL, MODE, WK, QH><<<grid_of((n_eff + rows - 1) / rows, njobs_cap, FEW_THREADS), FEW_THREADS, lds, s>>>(a);
     };
-    if (steps >= 8) go(std::integral_constant<int, 8>{});
-    else if (steps >= 4) go(std::integral_constant<int, 4>{});
-    else if (steps >= 2) go(std::integral_constant<int, 2>{});
+    const int along = QH ? steps / 2 : steps;
+    if (along >= 8) go(std::integral_constant<int, 8>{});
+    else if (along >= 4) go(std::integral_constant<int, 4>{});
+    else if (along >= 2) go(std::integral_constant<int, 2>{});
     else go(std::integral_constant<int, 1>{});
 }
 
