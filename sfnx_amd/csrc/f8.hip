@@ -122,8 +122,9 @@ template <Elem EL> void dense_many(const Args& a, hipStream_t st) {
         case 0: return launch_mid<EL, 2, 1>(a, st);
         case 1: return launch_mid<EL, 2, 2>(a, st);
         case 2: return launch_mid<EL, EL == F8X ? 4 : 2, EL == F8X ? 2 : 4>(a, st);
-        case 3: return launch_narrow<EL>(a, jobs, st);
-        default: return launch_tiles<EL, STORE>(a, jobs, best == 5, st);
+        case 3: return launch_stream<EL, STORE, 1>(a, jobs, st);
+        case 4: return launch_stream<EL, STORE>(a, jobs, st);
+        default: return launch_group<EL>(a, jobs, st);
     }
 }
 
@@ -212,7 +213,7 @@ extern "C" int sfnx_moe_gate_up_swiglu_f8_big(const void* A, size_t sa, int n_in
         check_f8_rows(xq, xs);
         check_f8_rows(hq, hs);
         Args a{(const uint8_t*) A, sa, n_in, 2 * ff, jobs, njobs, 0, xq, xs, hq, hs, SFNX_F32, ff, 1};
-        launch_tiles<F8X, SWIGLU>(a, njobs_cap, false, stream_of(st));
+        launch_stream<F8X, SWIGLU>(a, njobs_cap, stream_of(st));
     });
 }
 
@@ -225,7 +226,7 @@ extern "C" int sfnx_moe_down_f8_big(const void* A, size_t sa, int n_in, int n_ou
         check_f8_rows(hq, hs);
         check_out(out, out_type);
         Args a{(const uint8_t*) A, sa, n_in, n_out, jobs, njobs, 0, hq, hs, out, nullptr, out_type, n_out, vec_ok(out, out_type, n_out)};
-        if (out_type == SFNX_F32) launch_tiles<F8X, STORE>(a, njobs_cap, false, stream_of(st));
-        else launch_tiles<F8, STORE>(a, njobs_cap, false, stream_of(st));
+        if (out_type == SFNX_F32) launch_stream<F8X, STORE>(a, njobs_cap, stream_of(st));
+        else launch_stream<F8, STORE>(a, njobs_cap, stream_of(st));
     });
 }

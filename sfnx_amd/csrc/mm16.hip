@@ -43,7 +43,7 @@ extern "C" int sfnx_moe_mm_16_big(const void* A, size_t sa, uint32_t type, int n
     return guarded("sfnx_moe_mm_16_big", [&] {
         const Args a = mm16_args(A, sa, type, n_in, n_out, jobs, njobs, njobs_cap, x, out_type, out);
         if (njobs_cap == 0) return;
-        if (type == SFNX_F16) launch_tiles<F16, STORE>(a, njobs_cap, false, stream_of(st));
-        else launch_tiles<BF16, STORE>(a, njobs_cap, false, stream_of(st));
+        if (type == SFNX_F16) launch_experts<F16>(a, njobs_cap, stream_of(st));
+        else launch_experts<BF16>(a, njobs_cap, stream_of(st));
     });
 }

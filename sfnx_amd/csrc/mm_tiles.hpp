@@ -31,8 +31,8 @@ template <int NT> struct Stream {
 };
 constexpr int S1_LDS = Stream<2>::LDS;
 constexpr int SG_LIST = 2 * Stage<BMG>::SIZE, WINDOW = 8192;   // the groups of WINDOW jobs, as 16-bit job numbers
-constexpr int T_LDS = SG_LIST + 2 * WINDOW > S1_LDS ? SG_LIST + 2 * WINDOW : S1_LDS;
-static_assert(T_LDS + 64 <= 160 * 1024 && 4 * WINDOW <= SG_LIST && 2 * BMG * 4 + BMG * HP <= SG_LIST, "LDS");
+constexpr int T_LDS = SG_LIST + 2 * WINDOW + 64;   // and their number
+static_assert(T_LDS <= 160 * 1024 && T_LDS >= S1_LDS && 4 * WINDOW <= SG_LIST, "LDS");
 
 // Workgroup b runs on XCD b % 8: the slices of xg consecutive groups (an expert's jobs are consecutive) go to one XCD, so
 // an expert's weights come from HBM once for them; xg = XG, or 1 where there are too few to use all XCDs evenly (single jobs, few
@@ -289,7 +289,7 @@ template <Elem EL, Mode MODE, int NT> __device__ __forceinline__ void stream_til
 // ------------------------------------------------------------------------------------------------ a group of jobs a tile
 // A wavefront owns a job's 64 rows and NT of the tile's 16 weight tiles: of a group of C jobs (3 are taken as 4), 8 / C wavefronts
 // share a job.
-template <Elem EL, Mode MODE, int C> __device__ __forceinline__ void group_tile(const Args& a, int sl, int j0, int count, const Lds& L) {
+template <Elem EL, int C> __device__ __forceinline__ void group_tile(const Args& a, int sl, int j0, int count, const Lds& L) {
     uint8_t* const lds = L.p;
     constexpr int WN = TW / C, NT = 16 / WN;
     typedef Stage<BM1 * C> S;
@@ -328,13 +328,13 @@ template <Elem EL, Mode MODE, int C> __device__ __forceinline__ void group_tile(
     for (int i = 0; i < 4; ++i) {
         const int h = 2 * wave + i % 2;
         wto[i] = 16 * NT * (h / NT) + 8 * NT * (i / 2) + 8 * (h % NT);
-        woff[i] = (uint32_t) weight_row<MODE, NT>(a, sl, wto[i] + r8) * (uint32_t) rb;
+        woff[i] = (uint32_t) weight_row<STORE, NT>(a, sl, wto[i] + r8) * (uint32_t) rb;
     }
 #pragma unroll
     for (int i = 0; i < C; ++i) xsrc[i] = a.x + (size_t) act_row(8 * (C * wave + i) + r8) * rb;
     if constexpr (IS8<EL>) {
         xs_src = a.xs + (size_t) act_row(64 * wm + lane) * nb;
-        ws_src = scales_of(mat, a.n_out, a.n_in) + (size_t) (weight_row<MODE, NT>(a, sl, 16 * r) / BLK) * nb;
+        ws_src = scales_of(mat, a.n_out, a.n_in) + (size_t) (weight_row<STORE, NT>(a, sl, 16 * r) / BLK) * nb;
     }
     // copy u (0 .. 3 weights, 4 .. 3 + C activations) of step s into a stage; past the rows' end their last piece (see below), past
     // the last step that again
@@ -345,8 +345,8 @@ template <Elem EL, Mode MODE, int C> __device__ __forceinline__ void group_tile(
     };
     auto copy_scales = [&](int s, uint8_t* buf) {
         if constexpr (IS8<EL>) {
-            if (wn == 0) copy4(xs_src + min(s, steps - 1), L.at(buf + S::XS + 256 * wm));
-            if (wave == 1) copy4(ws_src + min(s, steps - 1), L.at(buf + S::WS));
+            if (EL == F8X || wn == 0) copy4(xs_src + min(s, steps - 1), L.at(buf + S::XS + 256 * wm));
+            if (EL == F8X || wave == 1) copy4(ws_src + min(s, steps - 1), L.at(buf + S::WS));
         }
     };
     auto copy_early = [&](int s, uint8_t* buf) {
@@ -453,21 +453,16 @@ template <Elem EL, Mode MODE, int C> __device__ __forceinline__ void group_tile(
         }
     }
     vm_wait<0>();   // the copies past the end
-    if constexpr (MODE == STORE) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int m = 16 * j + r;
-            if (m >= n) continue;
-            const size_t o = (size_t) out_row(64 * wm + m) * a.ldo;
+    for (int j = 0; j < 4; ++j) {
+        const int m = 16 * j + r;
+        if (m >= n) continue;
+        const size_t o = (size_t) out_row(64 * wm + m) * a.ldo;
 #pragma unroll
-            for (int u = 0; u < NT; ++u) {
-                const int col = sl * BN + 16 * NT * wn + 16 * u + 4 * q;
-                store4(a.out, a.out_type, o + col, acc[u][j], a.n_out - col, a.vec);
-            }
+        for (int u = 0; u < NT; ++u) {
+            const int col = sl * BN + 16 * NT * wn + 16 * u + 4 * q;
+            store4(a.out, a.out_type, o + col, acc[u][j], a.n_out - col, a.vec);
         }
-    } else {
-        lds_barrier();   // the stages are free
-        swiglu_out<WN, NT / 2, 4, BM1 * C>(a, acc, sl, wn, 64 * wm, n, BM1 * C, lds, out_row);
     }
 }
 
@@ -476,7 +471,7 @@ template <Elem EL, Mode MODE, int C> __device__ __forceinline__ void group_tile(
 __device__ __forceinline__ int list_groups(const sfnx_bigjob* jobs, int w0, int count, uint8_t* lds) {
     int* w = reinterpret_cast<int*>(lds);                                   // the jobs' experts, where the stages come later
     uint16_t* list = reinterpret_cast<uint16_t*>(lds + SG_LIST);
-    int* total = reinterpret_cast<int*>(lds + T_LDS);
+    int* total = reinterpret_cast<int*>(lds + SG_LIST + 2 * WINDOW);
     lds_barrier();
     for (int i = threadIdx.x; i < count; i += TT) w[i] = jobs[w0 + i].w;
     __syncthreads();
@@ -500,51 +495,68 @@ __device__ __forceinline__ int list_groups(const sfnx_bigjob* jobs, int w0, int 
     return __builtin_amdgcn_readfirstlane(*total);
 }
 
-// group: whether tiles are groups of jobs; 0 in a grouped product: they are where the jobs make less than half as many groups,
-// which the jobs themselves say
-template <Elem EL, Mode MODE> __global__ void __launch_bounds__(TT, 2) k_mm_tiles(Args a, int cap, int group) {
+// the tiles of the groups in list (or of a dense product's jobs [0, count), every GJ)
+template <Elem EL> __device__ __forceinline__ void group_tiles(const Args& a, int w0, int count, int n, const uint16_t* list, const Lds& L) {
+    const int tiles = (int) tiles_of(a.slices, n);
+    for (int b = blockIdx.x; b < tiles; b += gridDim.x) {
+        int sl, i;
+        if (!tile_at<4>(b, a.slices, n, sl, i)) continue;
+        i = n - 1 - i;   // the last group first: the shared expert's
+        const int j0 = list ? list[i] : GJ * i, j1 = list ? (i + 1 < n ? list[i + 1] : count) : min(j0 + GJ, count);
+        if (j1 - j0 > 2) group_tile<EL, 4>(a, sl, w0 + j0, j1 - j0, L);
+        else if (j1 - j0 == 2) group_tile<EL, 2>(a, sl, w0 + j0, 2, L);
+        else group_tile<EL, 1>(a, sl, w0 + j0, 1, L);
+    }
+}
+
+// ------------------------------------------------------------------------------------------------ kernels
+template <Elem EL, Mode MODE, int NT> __global__ void __launch_bounds__(TT, 2) k_mm_stream(Args a, int cap) {
+    extern __shared__ __align__(16) uint8_t lds[];
+    stream_tiles<EL, MODE, NT>(a, a.dense_c > 0 ? cap : min(*a.njobs, cap), lds_of(lds));
+}
+
+template <Elem EL> __global__ void __launch_bounds__(TT, 2) k_mm_group(Args a, int jobs) {
+    extern __shared__ __align__(16) uint8_t lds[];
+    group_tiles<EL>(a, 0, jobs, (jobs + GJ - 1) / GJ, nullptr, lds_of(lds));
+}
+
+// 16-bit experts: groups where their rounds of workgroups, each of which takes twice a round of single jobs, are fewer than half
+// of those; which the jobs themselves say.  Streamed and grouped (us; 2048 columns, 1024 rows, bf16, tokens / experts / top k):
+// 600 / 8 / 2 25 and 54; 1024 / 64 / 6 95 and 127; 2048 / 64 / 6 126 and 129; 4096 / 64 / 6 212 and 177; 4096 / 128 / 8 282 and 206.
+// The 8-bit products of experts are streamed: grouped, their steps' scales and conversions keep the matrix cores waiting, and
+// only experts of a thousand rows gain (gate|up of 4096 / 64 / 6 201 and 230, 1024 / 64 / 6 79 and 150).
+template <Elem EL> __global__ void __launch_bounds__(TT, 2) k_mm_experts(Args a, int cap) {
     extern __shared__ __align__(16) uint8_t lds[];
     const Lds L = lds_of(lds);
-    const bool dense = a.dense_c > 0;
-    const int nj = dense ? cap : min(*a.njobs, cap);
+    const int nj = min(*a.njobs, cap);
     const sfnx_bigjob* jobs = (const sfnx_bigjob*) a.jobs;
+    auto rounds = [&](int n) { return ((int64_t) n * a.slices + CUS - 1) / CUS; };
+    bool group = false;
     for (int w0 = 0; w0 < nj; w0 += WINDOW) {
         const int count = min(WINDOW, nj - w0);
-        const int n = dense ? (count + GJ - 1) / GJ : list_groups(jobs, w0, count, lds);
-        if (!group && (dense || count < 2 * n)) break;
-        group = 1;
-        const uint16_t* list = reinterpret_cast<const uint16_t*>(lds + SG_LIST);
-        const int tiles = (int) tiles_of(a.slices, n);
-        for (int b = blockIdx.x; b < tiles; b += gridDim.x) {
-            int sl, i;
-            if (!tile_at<4>(b, a.slices, n, sl, i)) continue;
-            i = n - 1 - i;   // the last group first: the shared expert's
-            const int j0 = dense ? GJ * i : list[i], j1 = dense ? min(j0 + GJ, count) : i + 1 < n ? list[i + 1] : count;
-            if (j1 - j0 > 2) group_tile<EL, MODE, 4>(a, sl, w0 + j0, j1 - j0, L);
-            else if (j1 - j0 == 2) group_tile<EL, MODE, 2>(a, sl, w0 + j0, 2, L);
-            else group_tile<EL, MODE, 1>(a, sl, w0 + j0, 1, L);
-        }
+        const int n = list_groups(jobs, w0, count, lds);
+        if (!group && 2 * rounds(n) >= rounds(count)) break;
+        group = true;
+        group_tiles<EL>(a, w0, count, n, reinterpret_cast<const uint16_t*>(lds + SG_LIST), L);
     }
-    if (!group) stream_tiles<EL, MODE, 2>(a, nj, L);
+    if (!group) stream_tiles<EL, STORE, 2>(a, nj, L);
 }
 
-// a dense product in streamed tiles of 64 x 128
-template <Elem EL> __global__ void __launch_bounds__(TT, 2) k_mm_narrow(Args a, int jobs) {
-    extern __shared__ __align__(16) uint8_t lds[];
-    stream_tiles<EL, STORE, 1>(a, jobs, lds_of(lds));
-}
-template <Elem EL> void launch_narrow(const Args& a, int jobs, hipStream_t s) {
-    const int64_t tiles = tiles_of((a.n_out + 127) / 128, jobs);
+inline unsigned tile_grid(int slices, int jobs) {
+    const int64_t tiles = tiles_of(slices, jobs);
     require(tiles < (1 << 30), "too many jobs for one launch");
-    k_mm_narrow<EL><<<(unsigned) std::min<int64_t>(tiles, CUS), TT, Stream<1>::LDS, s>>>(a, jobs);
+    return (unsigned) std::min<int64_t>(tiles, CUS);
 }
-
-// group: of a dense product, whether its tiles are groups; a grouped product's jobs say so themselves
-template <Elem EL, Mode MODE> void launch_tiles(Args a, int njobs_cap, bool group, hipStream_t s) {
+template <Elem EL, Mode MODE, int NT = 2> void launch_stream(const Args& a, int jobs, hipStream_t s) {
+    k_mm_stream<EL, MODE, NT><<<tile_grid((a.n_out + 128 * NT - 1) / (128 * NT), jobs), TT, Stream<NT>::LDS, s>>>(a, jobs);
+}
+template <Elem EL> void launch_group(Args a, int jobs, hipStream_t s) {
     a.slices = (a.n_out + BN - 1) / BN;
-    const int64_t tiles = tiles_of(a.slices, njobs_cap);
-    require(tiles < (1 << 30), "too many jobs for one launch");
-    k_mm_tiles<EL, MODE><<<(unsigned) std::min<int64_t>(tiles, CUS), TT, T_LDS + 64, s>>>(a, njobs_cap, (int) group);
+    k_mm_group<EL><<<tile_grid(a.slices, (jobs + GJ - 1) / GJ), TT, T_LDS, s>>>(a, jobs);
+}
+template <Elem EL> void launch_experts(Args a, int njobs_cap, hipStream_t s) {
+    a.slices = (a.n_out + BN - 1) / BN;
+    k_mm_experts<EL><<<tile_grid(a.slices, njobs_cap), TT, T_LDS, s>>>(a, njobs_cap);
 }
 
 }  // namespace mm

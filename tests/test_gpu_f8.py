@@ -104,6 +104,20 @@ def test_gemm(C, n_in, n_out, t):
     assert (out[C] == 77).all()
 
 
+@pytest.mark.parametrize("t", sorted(OUT))
+@pytest.mark.parametrize("C, n_in, n_out", [(700, 2064, 2050), (1290, 2064, 4101), (3001, 2064, 4101)])
+def test_gemm_large(C, n_in, n_out, t):
+    """sizes that take each of the forms for many rows, short last blocks in every direction (the 64-bit products on the GPU)"""
+    g = gen(C)
+    blob, W = matrices(g, 1, n_out, n_in)
+    q, s = quantize(torch.randn((C, n_in), generator=g))
+    out = torch.full((C, n_out + 3), 77.0, dtype=OUT[t], device="cuda")
+    moe.f8_gemm(dev(blob), n_out, n_in, dev(q), dev(s), out[:, :n_out])
+    want, bound = product(dev(dequantize(q, s)), dev(W[0]), True)
+    close(out[:, :n_out], want.cpu(), bound.cpu(), OUT[t], True)
+    assert (out[:, n_out:] == 77).all()
+
+
 @pytest.mark.parametrize("C", [3, 100])
 @pytest.mark.parametrize("pad", [4, 5])
 def test_gemm_strided_output(C, pad):

@@ -44,6 +44,7 @@ def test_window(T, E, K, n_in, n_out, t, out_t):
 
 
 @pytest.mark.parametrize("t, out_t", [("f16", "f32"), ("f16", "f16"), ("bf16", "f32"), ("bf16", "bf16")])
-@pytest.mark.parametrize("T, E, K, n_in, n_out", [(1, 8, 3, 256, 128), (17, 5, 2, 8, 1), (65, 16, 4, 200, 145), (200, 12, 6, 1024, 512), (300, 4, 3, 584, 272)])
+@pytest.mark.parametrize("T, E, K, n_in, n_out", [(1, 8, 3, 256, 128), (17, 5, 2, 8, 1), (65, 16, 4, 200, 145), (200, 12, 6, 1024, 512), (300, 4, 3, 584, 272),
+                                               (300, 4, 3, 72, 8190), (380, 4, 3, 200, 8190)])   # the last two: groups of 1, 2 and 4 jobs
 def test_prompt(T, E, K, n_in, n_out, t, out_t):
     run(moe.moe_mm_16_big, 64, T, E, K, n_in, n_out, t, out_t, table=T == 65, shuffle=random.Random(4) if T == 200 else None)
