@@ -61,61 +61,50 @@ __device__ __forceinline__ Frag lds_frag(const uint8_t* rows, int row, int q) {
     return Frag{*reinterpret_cast<const uint4*>(p + 16 * (q ^ (row & 7))), *reinterpret_cast<const uint4*>(p + 16 * ((q + 4) ^ (row & 7)))};
 }
 
-// h = silu(gate) up on the accumulators acc[u][j] (gate) and acc[NT + u][j] (up), quantized: the tile's 128 columns are a
-// scale block of h.  WN wavefronts share a token's columns; lds: scratch of all wavefronts.
-template <int WN, int NT, int MT, int M, typename Out>
-__device__ __forceinline__ void swiglu_out(const Args& a, float4v (&acc)[2 * NT][MT], int sl, int wn, int m0, int n, int rows, uint8_t* lds, Out out_row) {
-    const int lane = threadIdx.x % WAVE, r = lane % 16, q = lane / 16, n_eff = a.n_out / 2;
-    float* mx = reinterpret_cast<float*>(lds);     // [WN][M]
-    uint8_t* hb = lds + WN * M * 4;                // [M][HP]
+// h = silu(gate) up on the accumulators (gate tile, up tile) of a tile's n <= 64 rows, quantized: the tile's 128 columns, 16 a
+// wavefront, are a scale block of h.  lds: scratch of all wavefronts.
+template <typename Out> __device__ __forceinline__ void swiglu_out(const Args& a, float4v (&acc)[2][4], int sl, int wave, int n, uint8_t* lds, Out out_row) {
+    const int lane = threadIdx.x % WAVE, r = lane % 16, q = lane / 16, ff = a.n_out / 2;
+    const bool in = sl * BLK + 16 * wave < ff;     // FF is a multiple of 16
+    uint32_t* mx = reinterpret_cast<uint32_t*>(lds);   // [TW][BM1]: the largest finite |h|, the top bit set where there are others
+    uint8_t* hb = lds + TW * BM1 * 4;                  // [BM1][HP]
 #pragma unroll
-    for (int j = 0; j < MT; ++j) {
+    for (int j = 0; j < 4; ++j) {
         if (16 * j >= n) continue;
         float am = 0.f;
-        int odd = 0;   // a value that is not finite
+        int odd = 0;
 #pragma unroll
-        for (int u = 0; u < NT; ++u)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const bool in = sl * BLK + 16 * (NT * wn + u) < n_eff;   // FF is a multiple of 16
-                acc[u][j][i] = in ? silu_f(acc[u][j][i]) * acc[NT + u][j][i] : 0.f;
-                am = fmaxf(am, finite_abs(acc[u][j][i]));
-                odd |= abs_bits(acc[u][j][i]) >= 0x7f800000u;
-            }
+        for (int i = 0; i < 4; ++i) {
+            acc[0][j][i] = in ? silu_f(acc[0][j][i]) * acc[1][j][i] : 0.f;
+            am = fmaxf(am, finite_abs(acc[0][j][i]));
+            odd |= abs_bits(acc[0][j][i]) >= 0x7f800000u;
+        }
         am = fmaxf(am, lane_xor<16>(am));
         am = fmaxf(am, lane_xor<32>(am));
         odd |= lane_xor<16>(odd);
         odd |= lane_xor<32>(odd);
-        if (q == 0) mx[wn * M + m0 + 16 * j + r] = odd ? -1.f - am : am;   // below zero: not all finite
+        if (q == 0) mx[wave * BM1 + 16 * j + r] = __float_as_uint(am) | (uint32_t) odd << 31;
     }
     lds_barrier();
 #pragma unroll
-    for (int j = 0; j < MT; ++j) {
+    for (int j = 0; j < 4; ++j) {
         if (16 * j >= n) continue;
         const int m = 16 * j + r;
-        float am = 0.f;
-        bool fin = true;
+        uint32_t top = 0, any = 0;   // of values that are not negative, the largest has the largest bits
 #pragma unroll
-        for (int w = 0; w < WN; ++w) {
-            const float v = mx[w * M + m0 + m];
-            am = fmaxf(am, v < 0.f ? -1.f - v : v);
-            fin = fin && v >= 0.f;
+        for (int w = 0; w < TW; ++w) {
+            const uint32_t v = mx[w * BM1 + m];
+            top = max(top, v & 0x7fffffffu);
+            any |= v;
         }
-        const F8Scale s = f8_scale(am, fin);
-#pragma unroll
-        for (int u = 0; u < NT; ++u)
-            *reinterpret_cast<uint32_t*>(hb + (m0 + m) * HP + 16 * (NT * wn + u) + 4 * q) =
-                f8_pack4(acc[u][j][0], acc[u][j][1], acc[u][j][2], acc[u][j][3], s);
-        if (wn == 0 && q == 0 && m < n) a.out_s[out_row(m0 + m) * blocks_of(n_eff) + sl] = s.s;
+        const F8Scale s = f8_scale(__uint_as_float(top), any < 0x80000000u);
+        *reinterpret_cast<uint32_t*>(hb + m * HP + 16 * wave + 4 * q) = f8_pack4(acc[0][j][0], acc[0][j][1], acc[0][j][2], acc[0][j][3], s);
+        if (wave == 0 && q == 0 && m < n) a.out_s[out_row(m) * blocks_of(ff) + sl] = s.s;
     }
     lds_barrier();
-    for (int i = threadIdx.x; i < M * 8; i += TT) {
-        const int m = i / 8, c = 16 * (i % 8);
-        if (m < rows && sl * BLK + c < n_eff) {
-            const int64_t o = out_row(m);
-            if (o >= 0) *reinterpret_cast<uint4*>((uint8_t*) a.out + (size_t) o * n_eff + sl * BLK + c) = *reinterpret_cast<const uint4*>(hb + m * HP + c);
-        }
-    }
+    const int m = threadIdx.x / 8, c = 16 * (threadIdx.x % 8);
+    if (m < n && sl * BLK + c < ff)
+        *reinterpret_cast<uint4*>((uint8_t*) a.out + out_row(m) * ff + sl * BLK + c) = *reinterpret_cast<const uint4*>(hb + m * HP + c);
 }
 
 // ------------------------------------------------------------------------------------------------ one job a tile
@@ -266,7 +255,7 @@ template <Elem EL, Mode MODE, int NT> __device__ __forceinline__ void stream_til
         else walk(std::integral_constant<int, 1>{});
 
         const int* outs = slot_of(c) + 2 + SFNX_PF_JOB;
-        auto out_row = [&](int m) { return (int64_t) (dense ? BM1 * cji + m : outs[m]); };
+        auto out_row = [&](int m) { return (size_t) (dense ? BM1 * cji + m : outs[m]); };
         if constexpr (MODE == STORE) {
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
@@ -280,7 +269,7 @@ template <Elem EL, Mode MODE, int NT> __device__ __forceinline__ void stream_til
                 }
             }
         } else {
-            swiglu_out<TW, 1, 4, BM1>(a, acc, csl, wave, 0, n, n, lds + Stream<NT>::EPI, out_row);
+            swiglu_out(a, acc, csl, wave, n, lds + Stream<NT>::EPI, out_row);
         }
         ct = next_tile(ct + grid, csl, cji);
     }

@@ -235,6 +235,40 @@ def test_gate_up_prompt(T, E, K, H, ff, table):
     assert (hq.cpu()[rest] == 0x55).all() and (hs.cpu()[rest] == 77).all()
 
 
+def test_gate_up_prompt_with_values_that_are_not_finite():
+    """a NaN weight row and an overflowing activation row: NaN where they reach, the block's scale from its finite values"""
+    T, E, K, H, ff = 70, 4, 2, 256, 192
+    blob, W, q, s, topi, P = gate_up_case(T, E, K, H, ff, True, 0.0, 8)
+    blob[2, 5 * H] = 0x7F            # expert 2's gate row 5
+    s[9] = 3e38                      # token 9's products overflow, all of them or their products
+    a, n, flat = jobs(topi, E, True, 64, True)
+    jt, nt, cap = job_tensors(a, n)
+    d = dev(blob)
+    hq, hs = torch.zeros((P, ff), dtype=torch.uint8, device="cuda"), torch.zeros((P, 2), device="cuda")
+    moe.moe_gate_up_swiglu_f8_big(d, d.stride(0), H, ff, jt, nt, cap, dev(q), dev(s), hq, hs)
+    r, b, where = grouped(dequantize(q, s), W, flat, True)
+    want, bound = swiglu(r, b, ff)
+    token = {o: y for _, y, o in flat}
+    sick = torch.tensor([token[int(o)] == 9 for o in where])
+    expert = {o: e for e, _, o in flat}
+    nan = torch.zeros((len(where), ff), dtype=torch.bool)
+    nan[torch.tensor([expert[int(o)] == 2 for o in where]), 5] = True
+    got, sc = hq.cpu()[where], hs.cpu()[where].double()
+    fine = ~sick
+    assert ((got[nan] & 0x7F) == 0x7F).all()
+    assert torch.isfinite(sc).all()
+    want = torch.where(nan, torch.zeros((), dtype=torch.float64), want)
+    bound = torch.where(nan, torch.zeros((), dtype=torch.float64), bound)
+    amax = torch.stack([v.amax(1) for v in want.abs().split(BLK, 1)], 1)
+    off = torch.stack([v.amax(1) for v in bound.split(BLK, 1)], 1)
+    assert ((sc - amax / F8_MAX).abs() <= off / F8_MAX + ULP * sc)[fine].all()
+    v = got.view(F8).double()
+    ok = (v * spread(sc, ff) - want).abs() <= bound + (E4M3_HALF + 2 * ULP) * (want.abs() + bound) + E4M3_SUB * spread(sc, ff)
+    assert (ok | nan)[fine].all()
+    # the overflowing row: what is finite in it is at most 448 of its scale, the rest NaN
+    assert (torch.isnan(v[sick]) | (v[sick].abs() <= F8_MAX)).all()
+
+
 @pytest.mark.parametrize("t", sorted(OUT))
 @pytest.mark.parametrize("T, E, K, H, ff", BIG)
 def test_down_prompt(T, E, K, H, ff, t):
