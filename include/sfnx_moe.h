@@ -190,16 +190,17 @@ int sfnx_pf_dense(const sfnx_q8s* W, int rows, int cols, const uint16_t* xh, int
  * [ceil(rows / 128)][ceil(cols / 128)] (the last blocks of a row or column may be shorter); an activation row has a scale for
  * each 128 values, [rows][ceil(cols / 128)].  A product is the
  * sum over b of (xs_b ws_b) (sum over the block's k of xq[k] wq[k]), on the matrix cores: in fp32 where the result is kept
- * in 32 bits or quantized again, and for jobs of up to 16 rows; where it is rounded to 16 bits (more than 16 rows), sums of
- * 8 consecutive products keep 13 bits of the largest, 1.5e-5 of the result's norm, and the rest is fp32.
- * cols % 16 == 0; pointers 16-byte aligned (outputs and scales to their type); expert strides a multiple of 16, or 0 for a
- * table of expert pointers; out_type SFNX_F32, SFNX_F16 or SFNX_BF16.  Rows that no job names are left as they were.
+ * in 32 bits or quantized again, in a window's calls and in dense ones of up to 16 rows; where a larger call rounds it to 16
+ * bits, sums of 8 consecutive products keep 13 bits of the largest, 1.5e-5 of the result's norm, and the rest is fp32.
+ * cols % 16 == 0, rows and cols at most 2^20, a matrix smaller than 4 GiB; pointers 16-byte aligned (outputs and scales to
+ * their type); expert strides a multiple of 16, or 0 for a table of expert pointers; out_type SFNX_F32, SFNX_F16 or SFNX_BF16.
+ * jobs holds njobs_max (njobs_cap) entries, of which the first *njobs are jobs.  Rows that no job names are left as they were.
  * A matrix's values and the activation rows are read as they are: a NaN reaches every output it belongs to. */
 /* bytes of a matrix of the 8-bit store, rounded up to 16 */
 size_t sfnx_f8_matrix_bytes(int rows, int cols);
 /* rows of x (type SFNX_F32, SFNX_F16 or SFNX_BF16, ldx values apart) as 8-bit rows: per 128 values
  * s = max(max |x| c, 2^-126) over the finite ones with c = 1 / 448 in fp32, q = e4m3(x / s); values that are not finite
- * become NaN */
+ * become NaN.  ldx % 16 == 0, fewer than 2^24 rows */
 int sfnx_quantize_f8(uint32_t type, const void* x, int64_t ldx, int rows, int cols, uint8_t* q, float* s, void* st);
 /* out[c][n] (rows ldo values apart) = row n of the matrix W times 8-bit row c, c < C */
 int sfnx_f8_gemm(const void* W, int rows, int cols, const uint8_t* xq, const float* xs, int C, uint32_t out_type, void* out,
@@ -221,7 +222,8 @@ int sfnx_moe_down_f8_big(const void* A, size_t sa, int n_in, int n_out, const sf
 /* ---------------------------------------------------------------------------------------------- 16-bit experts
  * No counterpart in the reference: experts that are not quantized, matrices [n_out][n_in] of f16 or bf16 (type SFNX_F16 or
  * SFNX_BF16) sa bytes apart (a multiple of 16, or 0 for a table of pointers), over a window's jobs or a chunk's BigJobs:
- * out[out[j]] = the expert's rows times row y[j] of x (the same type), summed in fp32.  n_in % 8 == 0. */
+ * out[out[j]] = the expert's rows times row y[j] of x (the same type), summed in fp32.  n_in % 8 == 0; n_in,
+ * n_out and the size of a matrix limited as above. */
 int sfnx_moe_mm_16(const void* A, size_t sa, uint32_t type, int n_in, int n_out, const sfnx_job* jobs, const int* njobs,
                    int njobs_max, const uint16_t* x, uint32_t out_type, void* out, void* st);
 int sfnx_moe_mm_16_big(const void* A, size_t sa, uint32_t type, int n_in, int n_out, const sfnx_bigjob* jobs,

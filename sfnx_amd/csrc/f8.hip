@@ -64,6 +64,7 @@ template <int TYPE> void quantize(const void* x, int64_t ldx, int rows, int cols
 
 // ------------------------------------------------------------------------------------------------ checks
 constexpr const char* ALIGN_MSG = "pointers must be 16-byte aligned";
+constexpr const char* SCALES_MSG = "scales must be 4-byte aligned";
 bool al16(const void* p) { return ((uintptr_t) p & 15) == 0; }
 void check_out(const void* out, uint32_t out_type) {
     require(out_type_ok(out_type), "out type must be F32 (0), F16 (1) or BF16 (30)");
@@ -90,6 +91,7 @@ void check_f8_matrix(const void* A, size_t sa, int n_in, int n_out) {
 void check_f8_rows(const uint8_t* xq, const float* xs) {
     require(xq != nullptr && xs != nullptr, "null pointer");
     require(al16(xq), ALIGN_MSG);
+    require(((uintptr_t) xs & 3) == 0, SCALES_MSG);
 }
 
 // A dense product of more than 16 rows: the form of the least estimated time.  A form's tile takes `one` us for 4096 columns
@@ -143,11 +145,12 @@ extern "C" int sfnx_quantize_f8(uint32_t type, const void* x, int64_t ldx, int r
     return guarded("sfnx_quantize_f8", [&] {
         require(out_type_ok(type), "x type must be F32 (0), F16 (1) or BF16 (30)");
         require(cols > 0 && cols % 16 == 0 && cols <= (1 << 20), "cols must be a multiple of 16, at most 2^20");
-        require(rows >= 0 && rows <= (1 << 24), "rows out of range");
+        require(rows >= 0 && rows < (1 << 24), "rows out of range");   // with a workgroup a row, fewer than 2^32 threads
         require(ldx >= cols && ldx % 16 == 0, "ldx must be a multiple of 16, at least cols");
         if (rows == 0) return;
         require(x != nullptr && q != nullptr && s != nullptr, "null pointer");
         require(al16(x) && al16(q), ALIGN_MSG);
+        require(((uintptr_t) s & 3) == 0, SCALES_MSG);
         hipStream_t h = stream_of(st);
         if (type == SFNX_F32) quantize<SFNX_F32>(x, ldx, rows, cols, q, s, h);
         else if (type == SFNX_F16) quantize<SFNX_F16>(x, ldx, rows, cols, q, s, h);

@@ -48,6 +48,26 @@ def test_library_refuses(call, msg):
     assert msg in L.sfnx_last_error().decode()
 
 
+@pytest.mark.parametrize("call, msg", [
+    (lambda L: L.sfnx_quantize_f8(0, P, 128, 1 << 24, 128, P, P, None), "rows out of range"),
+    (lambda L: L.sfnx_quantize_f8(0, P, 128, 1, 128, P, P + 2, None), "scales must be"),
+    (lambda L: L.sfnx_f8_gemm(P, 128, 128, P, P + 2, 1, 0, P, 128, None), "scales must be"),
+    (lambda L: L.sfnx_moe_gate_up_swiglu_f8(P, BIG, 128, 128, P, P, 1, P, P + 1, P, None), "scales must be"),
+    (lambda L: L.sfnx_moe_gate_up_swiglu_f8_big(P, BIG, 128, 128, P, P, 1, P, P, P, P + 2, None), "scales must be"),
+    (lambda L: L.sfnx_moe_down_f8_big(P, BIG, 128, 128, P, P, 1, P, P + 2, 0, P, None), "scales must be"),
+    (lambda L: L.sfnx_f8_gemm(P, 1 << 16, 1 << 16, P, P, 1, 0, P, 1 << 16, None), "smaller than 4 GiB"),
+    (lambda L: L.sfnx_f8_gemm(P, 128, (1 << 20) + 16, P, P, 1, 0, P, 128, None), "at most 2^20"),
+    (lambda L: L.sfnx_moe_down_f8_big(P, BIG, 1 << 16, 1 << 16, P, P, 1, P, P, 0, P, None), "smaller than 4 GiB"),
+    (lambda L: L.sfnx_moe_mm_16(P, BIG, 1, 1 << 16, 1 << 15, P, P, 1, P, 0, P, None), "smaller than 4 GiB"),
+    (lambda L: L.sfnx_moe_mm_16_big(P, BIG, 30, (1 << 20) + 8, 8, P, P, 1, P, 0, P, None), "at most 2^20"),
+])
+def test_library_refuses_sizes(call, msg):
+    """sizes past what the kernels' 32-bit offsets and launches hold, and scales off their type's alignment"""
+    L = _abi.lib()
+    assert call(L) == -1
+    assert msg in L.sfnx_last_error().decode()
+
+
 def test_matrix_bytes():
     L = _abi.lib()
     assert L.sfnx_f8_matrix_bytes(1024, 2048) == 1024 * 2048 + 4 * 8 * 16
