@@ -102,7 +102,7 @@ void check_f8_rows(const uint8_t* xq, const float* xs) {
 //   256 x 1024         16.8        11.8       15.6          27               33               64
 //   512 x 2048         58          37         30            28               33               65
 //   1024 x 4096       224         141        114            69               36               66
-//   4096 x 4096                                                             127               72
+//   4096 x 4096                                                             127               69
 struct DenseForm {
     int rows, cols;
     float one, more, fixed;

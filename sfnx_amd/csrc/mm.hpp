@@ -209,6 +209,9 @@ __device__ __forceinline__ void copy16(const uint8_t* p, uint32_t to) {
 __device__ __forceinline__ void copy4(const void* p, uint32_t to) {
     asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(p), "s"(to) : "m0");
 }
+__device__ __forceinline__ void copy4(const uint8_t* base, uint32_t off, uint32_t to) {
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %0, %1" ::"v"(off), "s"(base), "s"(to) : "m0");
+}
 // a workgroup's LDS, as a pointer to read through and as the address copies take: cast once, where the compiler sees the array
 // itself (a generic pointer's cast tests it for null each time)
 struct Lds {

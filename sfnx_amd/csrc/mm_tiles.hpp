@@ -2,9 +2,9 @@
 //
 // One workgroup a compute unit walks tiles of 256 weight rows (SWIGLU: 128 gate rows and their up rows) times either one job
 // (stream_tiles: where the weights' way from HBM is the time) or up to four consecutive jobs of one expert, 256 rows
-// (group_tiles: where experts have many rows and the matrix cores are).  Both bring a K step of both operands and its scales
-// into LDS by asynchronous copies: whole 128-byte lines, 8 rows a request; 16-byte piece p of row r at place p ^ (r % 8), so
-// that the 16 lanes of a fragment's rows read different banks.
+// (group_tiles: large dense products, and 16-bit experts of many rows, where the matrix cores are).  Both bring a K step of both
+// operands and its scales into LDS by asynchronous copies: whole 128-byte lines, 8 rows a request; 16-byte piece p of row r at
+// place p ^ (r % 8), so that the 16 lanes of a fragment's rows read different banks (no conflicts counted).
 #pragma once
 
 #include "mm.hpp"
@@ -111,7 +111,8 @@ template <typename Out> __device__ __forceinline__ void swiglu_out(const Args& a
 // The tiles are one unbroken stream of stages: while one is multiplied the next two are on their way into LDS, across
 // the ends of tiles too, so no tile waits for its first weights.  The descriptions of later jobs come by asynchronous copies
 // as well: a load the compiler waits for would drain the stream.  A wavefront owns 32 of the tile's weight rows for all of
-// the job's rows.
+// the job's rows.  Bound by memory: gate|up of 2048 tokens over 513 experts of 2048 x 1024, 1.07 GB of weights, 247 us, 4.4 TB/s
+// (a copy of that size 4.9, reads into LDS alone 6.0); the matrix cores are 21% busy.
 template <Elem EL, Mode MODE, int NT> __device__ __forceinline__ void stream_tiles(const Args& a, int nj, const Lds& L) {
     uint8_t* const lds = L.p;
     constexpr int KS = Stream<NT>::KS, D = Stream<NT>::STAGES, N = 128 * NT;
@@ -277,7 +278,9 @@ template <Elem EL, Mode MODE, int NT> __device__ __forceinline__ void stream_til
 
 // ------------------------------------------------------------------------------------------------ a group of jobs a tile
 // A wavefront owns a job's 64 rows and NT of the tile's 16 weight tiles: of a group of C jobs (3 are taken as 4), 8 / C wavefronts
-// share a job.
+// share a job.  4096 x 4096 x 4096 e4m3 into bf16 69 us, 2.0 PFLOP/s (72.5 with all wavefronts reading and multiplying at once);
+// 4096 tokens over 65 bf16 experts of 2048 x 2048 282 us, 0.85 PFLOP/s (295), of which tiles that experts' last jobs leave part
+// empty cost a quarter.  Timed apart, a step's copies hide but for 10 us of the 69, its fragments' reads but for 20.
 template <Elem EL, int C> __device__ __forceinline__ void group_tile(const Args& a, int sl, int j0, int count, const Lds& L) {
     uint8_t* const lds = L.p;
     constexpr int WN = TW / C, NT = 16 / WN;
@@ -285,7 +288,7 @@ template <Elem EL, int C> __device__ __forceinline__ void group_tile(const Args&
     const int lane = threadIdx.x % WAVE, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
     const int r = lane % 16, q = lane / 16, r8 = lane / 8, p8 = (lane % 8) ^ r8, wm = wave / WN, wn = wave % WN;
     const int rb = a.n_in * ESZ<EL>, steps = (rb + STEP - 1) / STEP, nb = blocks_of(a.n_in);
-    const bool dense = a.dense_c > 0;
+    constexpr bool dense = IS8<EL>;   // grouped are dense products in 8 bits and jobs in 16
     const sfnx_bigjob* jobs = (const sfnx_bigjob*) a.jobs + j0;
     // rows of the group's job i, its activation rows and output rows
     auto rows_of = [&](int i) {
@@ -294,7 +297,7 @@ template <Elem EL, int C> __device__ __forceinline__ void group_tile(const Args&
     };
     auto act_row = [&](int m) {
         const int n = rows_of(m / BM1);
-        if (n == 0) return 0;   // some row: a job that the group does not have
+        if (n == 0) return dense ? BM1 * j0 : 0;   // some row: a job that the group does not have
         const int mm = min(m % BM1, n - 1);
         return dense ? BM1 * (j0 + m / BM1) + mm : jobs[m / BM1].y[mm];
     };
@@ -305,105 +308,161 @@ template <Elem EL, int C> __device__ __forceinline__ void group_tile(const Args&
     const uint8_t* mat = uniform_ptr(expert_at(a.A, a.sa, dense ? 0 : jobs[0].w));
     const int n = __builtin_amdgcn_readfirstlane(rows_of(wm));
 
-    // Of a stage, the rows of the activations and of each wavefront's first half of the weight tiles are read in the first half of a
-    // step, and copied over from the middle of it on, two steps ahead (EARLY); the other weight tiles' rows, one step ahead from
-    // its start on.  F8X reads everything until the end: one step ahead, spread over the step's first half.
-    constexpr bool EARLY = EL != F8X;
     uint32_t woff[4];
     const uint8_t* xsrc[C];
-    const float *xs_src = nullptr, *ws_src = nullptr;
+    uint32_t xs_off = 0, ws_off = 0;
     int wto[4];   // this wavefront's 8-row pieces of the weights: two of first, two of other tiles
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const int h = 2 * wave + i % 2;
         wto[i] = 16 * NT * (h / NT) + 8 * NT * (i / 2) + 8 * (h % NT);
-        woff[i] = (uint32_t) weight_row<STORE, NT>(a, sl, wto[i] + r8) * (uint32_t) rb;
+        if constexpr (!dense) woff[i] = (uint32_t) weight_row<STORE, NT>(a, sl, wto[i] + r8) * (uint32_t) rb;
     }
+    if constexpr (!dense)
 #pragma unroll
-    for (int i = 0; i < C; ++i) xsrc[i] = a.x + (size_t) act_row(8 * (C * wave + i) + r8) * rb;
+        for (int i = 0; i < C; ++i) xsrc[i] = a.x + (size_t) act_row(8 * (C * wave + i) + r8) * rb;
+    const uint8_t *xs_base = nullptr, *ws_base = nullptr;
     if constexpr (IS8<EL>) {
-        xs_src = a.xs + (size_t) act_row(64 * wm + lane) * nb;
-        ws_src = scales_of(mat, a.n_out, a.n_in) + (size_t) (weight_row<STORE, NT>(a, sl, 16 * r) / BLK) * nb;
+        xs_base = uniform_ptr((const uint8_t*) (a.xs + (size_t) BM1 * j0 * nb));
+        ws_base = uniform_ptr((const uint8_t*) scales_of(mat, a.n_out, a.n_in));
+        xs_off = 4 * (uint32_t) (act_row(64 * wm + lane) - BM1 * j0) * (uint32_t) nb;
+        ws_off = 4 * (uint32_t) (weight_row<STORE, NT>(a, sl, 16 * r) / BLK) * (uint32_t) nb;
     }
     // copy u (0 .. 3 weights, 4 .. 3 + C activations) of step s into a stage; past the rows' end their last piece (see below), past
     // the last step that again
     auto copy = [&](int u, int s, uint8_t* buf) {
         const uint32_t k = (uint32_t) min(min(s, steps - 1) * STEP + 16 * p8, rb - 16);
-        if (u < 4) copy16(mat, woff[u] + k, L.at(buf + wto[u] * STEP));
-        else copy16(xsrc[u - 4] + k, L.at(buf + S::X + 8 * (C * wave + u - 4) * STEP));
-    };
-    auto copy_scales = [&](int s, uint8_t* buf) {
-        if constexpr (IS8<EL>) {
-            if (EL == F8X || wn == 0) copy4(xs_src + min(s, steps - 1), L.at(buf + S::XS + 256 * wm));
-            if (EL == F8X || wave == 1) copy4(ws_src + min(s, steps - 1), L.at(buf + S::WS));
+        const uint32_t to = L.at(buf + (u < 4 ? wto[u] * STEP : S::X + 8 * (C * wave + u - 4) * STEP));
+        if constexpr (dense) {   // 8 consecutive rows (past the last that again): their addresses are cheaper made than kept
+            const int end = u < 4 ? a.n_out : a.dense_c, first = min(u < 4 ? sl * BN + wto[u] : BM1 * j0 + 8 * (C * wave + u - 4), end - 1);
+            copy16(uniform_ptr((u < 4 ? mat : a.x) + (size_t) first * rb), (uint32_t) __umul24(min(r8, end - 1 - first), rb) + k, to);
+        } else if (u < 4) {
+            copy16(mat, woff[u] + k, to);
+        } else {
+            copy16(xsrc[u - 4] + k, to);
         }
     };
-    auto copy_early = [&](int s, uint8_t* buf) {
-#pragma unroll
-        for (int u = 0; u < 4 + C; ++u)
-            if (u < 2 || u >= 4) copy(u, s, buf);
+    auto copy_scales = [&](int s, uint8_t* xs_to, uint8_t* ws_to) {
+        const int k = 4 * min(s, steps - 1);
+        if (EL == F8X || wn == 0) copy4(xs_base + k, xs_off, L.at(xs_to + 256 * wm));   // F8X: without branches, which would spill
+        if (EL == F8X || wave == 1) copy4(ws_base + k, ws_off, L.at(ws_to));
     };
-    auto copy_late = [&](int s, uint8_t* buf) {
-        copy(2, s, buf);
-        copy(3, s, buf);
-        copy_scales(s, buf);
+    auto clear = [&](int u, uint8_t* buf) {   // zero past the rows' end, whatever lies there: each wavefront in what it copied
+        if ((steps - 1) * STEP + 16 * p8 >= rb)
+            *reinterpret_cast<uint4*>(buf + (u < 4 ? wto[u] * STEP : S::X + 8 * (C * wave + u - 4) * STEP) + 16 * lane) = uint4{};
     };
-    auto fence = [] { asm volatile("" ::: "memory"); };   // LDS reads stay where they are: all at once they would not fit the registers
+    const bool tail = rb % STEP != 0;
     float4v acc[NT][4] = {};
-    lds_barrier();   // the tile before is done with LDS
-    copy_early(0, lds);
-    copy_late(0, lds);
-    if (EARLY) copy_early(1, lds + S::SIZE);
-    for (int s = 0; s < steps; ++s) {
-        uint8_t* buf = lds + (s & 1) * S::SIZE;
-        uint8_t* to = lds + ((s + 1) & 1) * S::SIZE;
-        if (EARLY) vm_wait<2 + C>();   // all but the early copies of the step after this one
-        else vm_wait<0>();
-        if (s == steps - 1 && rb % STEP) {   // zero past the rows' end, whatever lies there: each wavefront in what it copied
-            const int k = s * STEP + 16 * p8;
+    if constexpr (EL != F8X) {
+        // The wavefronts of one half read fragments while those of the other, the second ones of their SIMDs, multiply, and the
+        // other way about: a step is four turns (read x and the first weight tiles, multiply, read the others, multiply), and the
+        // second half is a turn behind.  Copies into a place go out when both halves have read it, to be waited for four
+        // turns later, before the first half reads them: those of x and the first tiles two steps ahead, the others one.
+        // (Raised priority for the multiplying half: 72.5 us for 69.)
+        constexpr int H = NT / 2, SLOT = BMG * 4 + 256;
+        static_assert(!IS8<EL> || 4 * SLOT <= 2 * WINDOW, "the scales' places, where a list of groups would be");
+        const bool behind = wave >= TW / 2;
+        auto slot_of = [&](int s) { return lds + SG_LIST + (s & 3) * SLOT; };
+        auto copy_first = [&](int s, uint8_t* buf) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (k >= rb) *reinterpret_cast<uint4*>(buf + wto[i] * STEP + 16 * lane) = uint4{};
-#pragma unroll
-            for (int i = 0; i < C; ++i)
-                if (k >= rb) *reinterpret_cast<uint4*>(buf + S::X + 8 * (C * wave + i) * STEP + 16 * lane) = uint4{};
-        }
-        lds_barrier();   // every wavefront's copies of this stage landed, and every wavefront is past the one before
-        auto middle = [&](int u) {   // after a wavefront's u-th weight tile
-            if (u == 0) copy_late(s + 1, to);
-            if (u == NT / 2 - 1) {
-                lds_barrier();   // every wavefront has read the activations and the first tiles
-                copy_early(s + 2, buf);
-            }
-            fence();
+            for (int u = 0; u < 4 + C; ++u)
+                if (u < 2 || u >= 4) copy(u, s, buf);
+            if constexpr (IS8<EL>) copy_scales(s, slot_of(s), slot_of(s) + BMG * 4);
         };
-        if constexpr (EL == F8) {
-            // the products of a weight tile are added while the next tile's are made
-            Frag x[4];
-            float xs[4];
+        auto landed = [] { vm_wait<2 + C + 2>(); };   // all but this turn's copies and those of the reading turn before it
+        auto clear_first = [&](uint8_t* buf) {
+#pragma unroll
+            for (int u = 0; u < 4 + C; ++u)
+                if (u < 2 || u >= 4) clear(u, buf);
+        };
+        auto turn = [] {
+            __builtin_amdgcn_sched_barrier(0);
+            lds_barrier();
+            __builtin_amdgcn_sched_barrier(0);
+        };
+        Frag x[4], w[H];
+        float xs[4], ws[H];
+        auto read = [&](int s, const uint8_t* buf, int u0) {
+#pragma unroll
+            for (int u = 0; u < H; ++u) {
+                w[u] = lds_frag(buf, 16 * NT * wn + 16 * (u0 + u) + r, q);
+                if constexpr (IS8<EL>) ws[u] = reinterpret_cast<const float*>(slot_of(s) + BMG * 4)[NT * wn + u0 + u];
+            }
+        };
+        auto multiply = [&](int u0) {
+            if constexpr (IS8<EL>) {   // a product is scaled and added while the three after it are made
+                float4v d[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) d[j] = step_dot<EL>(w[0], x[j]);
+#pragma unroll
+                for (int u = 0; u < H; ++u)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        __builtin_amdgcn_sched_barrier(0);
+                        acc[u0 + u][j] = scaled_add(d[j], xs[j] * ws[u], acc[u0 + u][j]);
+                        if (u < H - 1) d[j] = step_dot<EL>(w[u + 1], x[j]);
+                    }
+            } else {
+#pragma unroll
+                for (int u = 0; u < H; ++u)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) acc[u0 + u][j] = step_mma<EL>(w[u], x[j], acc[u0 + u][j], 1.f);
+            }
+            if constexpr (IS8<EL>)
+#pragma unroll
+                for (int u = 0; u < H; ++u)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) asm volatile("" : "+v"(acc[u0 + u][j]));   // here, not sunk past the turn's end
+        };
+        lds_barrier();   // the tile before is done with LDS
+        copy_first(0, lds);
+        copy(2, 0, lds);
+        copy(3, 0, lds);
+        copy_first(1, lds + S::SIZE);
+        landed();
+        if (steps == 1 && tail) clear_first(lds);
+        lds_barrier();
+        if (behind) lds_barrier();
+        for (int s = 0; s < steps; ++s) {
+            uint8_t* buf = lds + (s & 1) * S::SIZE;
+            uint8_t* to = lds + ((s + 1) & 1) * S::SIZE;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 x[j] = lds_frag(buf + S::X, 64 * wm + 16 * j + r, q);
-                xs[j] = reinterpret_cast<const float*>(buf + S::XS)[64 * wm + 16 * j + r];
+                if constexpr (IS8<EL>) xs[j] = reinterpret_cast<const float*>(slot_of(s))[64 * wm + 16 * j + r];
             }
-            Frag w = lds_frag(buf, 16 * NT * wn + r, q);
-            float ws = reinterpret_cast<const float*>(buf + S::WS)[NT * wn];
+            read(s, buf, 0);
+            copy(2, s + 1, to);
+            copy(3, s + 1, to);
+            landed();
+            if (s == steps - 1 && tail) clear(2, buf), clear(3, buf);
+            turn();
+            multiply(0);
+            turn();
+            read(s, buf, H);
+            copy_first(s + 2, buf);
+            landed();
+            if (s == steps - 2 && tail) clear_first(to);
+            turn();
+            multiply(H);
+            turn();
+        }
+    } else {
+        // one step ahead, spread over the step's first half; converted, 64 activation rows are too many registers beside the sums:
+        // half of them at a time
+        auto fence = [] { asm volatile("" ::: "memory"); };   // LDS reads stay where they are: all at once they would not fit the registers
+        lds_barrier();   // the tile before is done with LDS
 #pragma unroll
-            for (int u = 0; u < NT; ++u) {
-                float4v d[4];
+        for (int u = 0; u < 4 + C; ++u) copy(u, 0, lds);
+        copy_scales(0, lds + S::XS, lds + S::WS);
+        for (int s = 0; s < steps; ++s) {
+            uint8_t* buf = lds + (s & 1) * S::SIZE;
+            uint8_t* to = lds + ((s + 1) & 1) * S::SIZE;
+            vm_wait<0>();
+            if (s == steps - 1 && tail)
 #pragma unroll
-                for (int j = 0; j < 4; ++j) d[j] = step_dot<EL>(w, x[j]);
-                const float sc = ws;
-                if (u < NT - 1) {
-                    w = lds_frag(buf, 16 * NT * wn + 16 * (u + 1) + r, q);
-                    ws = reinterpret_cast<const float*>(buf + S::WS)[NT * wn + u + 1];
-                }
-                middle(u);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) acc[u][j] = scaled_add(d[j], xs[j] * sc, acc[u][j]);
-            }
-        } else if constexpr (EL == F8X) {
-            // converted, 64 activation rows are too many registers beside the sums: half of them at a time
+                for (int u = 0; u < 4 + C; ++u) clear(u, buf);
+            lds_barrier();   // every wavefront's copies of this stage landed, and every wavefront is past the one before
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 FragX x[2];
@@ -422,22 +481,9 @@ template <Elem EL, int C> __device__ __forceinline__ void group_tile(const Args&
                     if (h == 0)
 #pragma unroll
                         for (int i = u * (4 + C) / NT; i < (u + 1) * (4 + C) / NT; ++i) copy(i, s + 1, to);
-                    if (h == 0 && u == NT - 1) copy_scales(s + 1, to);
+                    if (h == 0 && u == NT - 1) copy_scales(s + 1, to + S::XS, to + S::WS);
                     fence();
                 }
-            }
-        } else {
-            Frag x[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) x[j] = lds_frag(buf + S::X, 64 * wm + 16 * j + r, q);
-            Frag w = lds_frag(buf, 16 * NT * wn + r, q);
-#pragma unroll
-            for (int u = 0; u < NT; ++u) {
-                const Frag v = w;
-                if (u < NT - 1) w = lds_frag(buf, 16 * NT * wn + 16 * (u + 1) + r, q);
-                middle(u);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) acc[u][j] = step_mma<EL>(v, x[j], acc[u][j], 1.f);
             }
         }
     }
@@ -453,6 +499,7 @@ template <Elem EL, int C> __device__ __forceinline__ void group_tile(const Args&
             store4(a.out, a.out_type, o + col, acc[u][j], a.n_out - col, a.vec);
         }
     }
+    if (EL != F8X && wave < TW / 2) lds_barrier();   // the turn the second half was behind
 }
 
 // The groups of the jobs [w0, w0 + count): the numbers (from w0) of the jobs that start one, in LDS; returns how many.
