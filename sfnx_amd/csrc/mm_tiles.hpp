@@ -279,8 +279,9 @@ template <Elem EL, Mode MODE, int NT> __device__ __forceinline__ void stream_til
 // ------------------------------------------------------------------------------------------------ a group of jobs a tile
 // A wavefront owns a job's 64 rows and NT of the tile's 16 weight tiles: of a group of C jobs (3 are taken as 4), 8 / C wavefronts
 // share a job.  4096 x 4096 x 4096 e4m3 into bf16 69 us, 2.0 PFLOP/s (72.5 with all wavefronts reading and multiplying at once);
-// 4096 tokens over 65 bf16 experts of 2048 x 2048 282 us, 0.85 PFLOP/s (295), of which tiles that experts' last jobs leave part
-// empty cost a quarter.  Timed apart, a step's copies hide but for 10 us of the 69, its fragments' reads but for 20.
+// 4096 tokens over 65 bf16 experts of 2048 x 2048 282 us, 0.85 PFLOP/s (295); its 154 groups, 58 of them of one to three jobs, are
+// 4.8 rounds of workgroups where full ones would be 3.5.  Of the 69 us, all of a step's copies but 10 us hide behind its
+// products, and all of its fragments' reads but 20.
 template <Elem EL, int C> __device__ __forceinline__ void group_tile(const Args& a, int sl, int j0, int count, const Lds& L) {
     uint8_t* const lds = L.p;
     constexpr int WN = TW / C, NT = 16 / WN;
@@ -558,7 +559,7 @@ template <Elem EL> __global__ void __launch_bounds__(TT, 2) k_mm_group(Args a, i
 
 // 16-bit experts: groups where their rounds of workgroups, each of which takes twice a round of single jobs, are fewer than half
 // of those; which the jobs themselves say.  Streamed and grouped (us; 2048 columns, 1024 rows, bf16, tokens / experts / top k):
-// 600 / 8 / 2 25 and 54; 1024 / 64 / 6 95 and 127; 2048 / 64 / 6 126 and 129; 4096 / 64 / 6 212 and 177; 4096 / 128 / 8 282 and 206.
+// 600 / 8 / 2 27 and 48; 1024 / 64 / 6 96 and 99; 2048 / 64 / 6 130 and 125; 4096 / 64 / 6 215 and 169; 4096 / 128 / 8 276 and 206.
 // The 8-bit products of experts are streamed: grouped, their steps' scales and conversions keep the matrix cores waiting, and
 // only experts of a thousand rows gain (gate|up of 4096 / 64 / 6 201 and 230, 1024 / 64 / 6 79 and 150).
 template <Elem EL> __global__ void __launch_bounds__(TT, 2) k_mm_experts(Args a, int cap) {
