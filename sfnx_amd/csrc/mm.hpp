@@ -179,6 +179,7 @@ struct Args {
     int ldo;
     int vec;                 // four consecutive outputs at a multiple of 4 are aligned to their size
     int slices = 0;          // of a matrix, 256 rows each
+    bool across = false;     // tiles: an XCD's are slices of all groups, not groups' slices
 };
 
 // workgroups of a launch: a job's slices for each job; a launch holds fewer than 2^32 threads

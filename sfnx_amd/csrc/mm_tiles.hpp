@@ -36,16 +36,23 @@ static_assert(T_LDS <= 160 * 1024 && T_LDS >= S1_LDS && 4 * WINDOW <= SG_LIST, "
 
 // Workgroup b runs on XCD b % 8: the slices of xg consecutive groups (an expert's jobs are consecutive) go to one XCD, so
 // an expert's weights come from HBM once for them; xg = XG, or 1 where there are too few to use all XCDs evenly (single jobs, few
-// of one expert, 2 for 4: down of 777 tokens 129 -> 124 us; groups 4 for 1: bf16 experts of 4096 tokens 307 -> 297).  false: no
-// such group
-template <int XG> __device__ __forceinline__ bool tile_at(int b, int nsl, int n, int& sl, int& i) {
-    const int xg = n >= 64 ? XG : 1;
-    const int x = b % XCDS, k = b / XCDS, m = k / nsl;
-    sl = k % nsl;
-    i = xg * (XCDS * (m / xg) + x) + m % xg;
-    return i < n;
+// of one expert, 2 for 4: down of 777 tokens 129 -> 124 us; groups 4 for 1: bf16 experts of 4096 tokens 307 -> 297).  A dense
+// product of few groups leaves XCDs idle that way: where fewer rounds of the compute units come of it, an XCD takes every 8th
+// slice of all groups (across; 128 rows, 4096 -> 8192: 41.5 -> 20.9 us).  false: no such group or slice
+template <int XG> __device__ __forceinline__ bool tile_at(int b, int nsl, int n, bool across, int& sl, int& i) {
+    const int p = across ? n : nsl, xg = n >= 64 ? XG : 1;
+    const int x = b % XCDS, k = b / XCDS, m = k / p, u = k % p, v = xg * (XCDS * (m / xg) + x) + m % xg;
+    sl = across ? v : u;
+    i = across ? u : v;
+    return v < (across ? nsl : n);
 }
-__host__ __device__ __forceinline__ int64_t tiles_of(int nsl, int n) { return (int64_t) nsl * ((n + 31) / 32) * 32; }
+inline bool across_of(int nsl, int n) {
+    const int64_t per = CUS / XCDS;   // an XCD's compute units
+    return n < 64 && ((nsl + XCDS - 1) / XCDS * n + per - 1) / per < ((n + XCDS - 1) / XCDS * nsl + per - 1) / per;
+}
+__host__ __device__ __forceinline__ int64_t tiles_of(int nsl, int n, bool across) {
+    return across ? (int64_t) (nsl + XCDS - 1) / XCDS * XCDS * n : (int64_t) nsl * ((n + 31) / 32) * 32;
+}
 
 // The place of a slice's weight row in LDS.  STORE: wavefronts' rows in order.  SWIGLU: of each W = 2 NT tiles of 16 that a
 // wavefront owns, the first NT are gate tiles and the others their up tiles.
@@ -121,13 +128,13 @@ template <Elem EL, Mode MODE, int NT> __device__ __forceinline__ void stream_til
     const int lane = threadIdx.x % WAVE, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
     const int r = lane % 16, q = lane / 16, r8 = lane / 8, p8 = (lane % 8) ^ r8;
     const int rb = a.n_in * ESZ<EL>, steps = (rb + STEP - 1) / STEP, nb = blocks_of(a.n_in);
-    const int nsl = (a.n_out + N - 1) / N, grid = (int) gridDim.x, tiles = (int) tiles_of(nsl, nj);
+    const int nsl = (a.n_out + N - 1) / N, grid = (int) gridDim.x, tiles = (int) tiles_of(nsl, nj, IS8<EL> && MODE == STORE && a.across);
     const bool dense = a.dense_c > 0;
     const sfnx_bigjob* jobs = (const sfnx_bigjob*) a.jobs;
 
     auto next_tile = [&](int b, int& sl, int& ji) {   // the first tile of this workgroup from b on; its number, or -1
         for (; b < tiles; b += grid)
-            if (tile_at<2>(b, nsl, nj, sl, ji)) return b;
+            if (tile_at<2>(b, nsl, nj, IS8<EL> && MODE == STORE && a.across, sl, ji)) return b;
         return -1;
     };
     auto slot_of = [&](int c) { return reinterpret_cast<const int*>(lds + Stream<NT>::JOBS + (c % S1_SLOTS) * S1_SLOT); };
@@ -534,10 +541,11 @@ __device__ __forceinline__ int list_groups(const sfnx_bigjob* jobs, int w0, int 
 
 // the tiles of the groups in list (or of a dense product's jobs [0, count), every GJ)
 template <Elem EL> __device__ __forceinline__ void group_tiles(const Args& a, int w0, int count, int n, const uint16_t* list, const Lds& L) {
-    const int tiles = (int) tiles_of(a.slices, n);
+    const bool across = IS8<EL> && a.across;
+    const int tiles = (int) tiles_of(a.slices, n, across);
     for (int b = blockIdx.x; b < tiles; b += gridDim.x) {
         int sl, i;
-        if (!tile_at<4>(b, a.slices, n, sl, i)) continue;
+        if (!tile_at<4>(b, a.slices, n, across, sl, i)) continue;
         i = n - 1 - i;   // the last group first: the shared expert's
         const int j0 = list ? list[i] : GJ * i, j1 = list ? (i + 1 < n ? list[i + 1] : count) : min(j0 + GJ, count);
         if (j1 - j0 > 2) group_tile<EL, 4>(a, sl, w0 + j0, j1 - j0, L);
@@ -579,21 +587,25 @@ template <Elem EL> __global__ void __launch_bounds__(TT, 2) k_mm_experts(Args a,
     if (!group) stream_tiles<EL, STORE, 2>(a, nj, L);
 }
 
-inline unsigned tile_grid(int slices, int jobs) {
-    const int64_t tiles = tiles_of(slices, jobs);
+inline unsigned tile_grid(int slices, int jobs, bool across) {
+    const int64_t tiles = tiles_of(slices, jobs, across);
     require(tiles < (1 << 30), "too many jobs for one launch");
     return (unsigned) std::min<int64_t>(tiles, CUS);
 }
-template <Elem EL, Mode MODE, int NT = 2> void launch_stream(const Args& a, int jobs, hipStream_t s) {
-    k_mm_stream<EL, MODE, NT><<<tile_grid((a.n_out + 128 * NT - 1) / (128 * NT), jobs), TT, Stream<NT>::LDS, s>>>(a, jobs);
+template <Elem EL, Mode MODE, int NT = 2> void launch_stream(Args a, int jobs, hipStream_t s) {
+    const int slices = (a.n_out + 128 * NT - 1) / (128 * NT);
+    a.across = a.dense_c > 0 && across_of(slices, jobs);
+    k_mm_stream<EL, MODE, NT><<<tile_grid(slices, jobs, a.across), TT, Stream<NT>::LDS, s>>>(a, jobs);
 }
 template <Elem EL> void launch_group(Args a, int jobs, hipStream_t s) {
+    const int groups = (jobs + GJ - 1) / GJ;
     a.slices = (a.n_out + BN - 1) / BN;
-    k_mm_group<EL><<<tile_grid(a.slices, (jobs + GJ - 1) / GJ), TT, T_LDS, s>>>(a, jobs);
+    a.across = across_of(a.slices, groups);
+    k_mm_group<EL><<<tile_grid(a.slices, groups, a.across), TT, T_LDS, s>>>(a, jobs);
 }
 template <Elem EL> void launch_experts(Args a, int njobs_cap, hipStream_t s) {
     a.slices = (a.n_out + BN - 1) / BN;
-    k_mm_experts<EL><<<tile_grid(a.slices, njobs_cap), TT, T_LDS, s>>>(a, njobs_cap);
+    k_mm_experts<EL><<<tile_grid(a.slices, njobs_cap, false), TT, T_LDS, s>>>(a, njobs_cap);
 }
 
 }  // namespace mm

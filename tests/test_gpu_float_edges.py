@@ -120,3 +120,16 @@ def test_offsets_past_32_bits(name):
     sc, v = hs[far.cuda()].cpu().double(), hq[far.cuda()].cpu().view(F8).double()
     lim = bound + (E4M3_HALF + 2 * ULP) * (want.abs() + bound) + E4M3_SUB * spread(sc, ff)
     assert ((v * spread(sc, ff) - want).abs() <= lim).all()
+
+
+@pytest.mark.parametrize("t", ["f16", "bf16"])
+@pytest.mark.parametrize("C, n_in, n_out", [(777, 2000, 1301), (600, 1024, 1600), (513, 144, 1937), (1000, 2032, 1185), (66, 1152, 16001), (128, 528, 8192), (300, 144, 20000)])
+def test_gemm_few_or_wide(C, n_in, n_out, t):
+    """dense sizes of few row tiles and many column tiles and between, with rows and columns past their last tiles"""
+    g = gen(C + n_out)
+    blob, W = matrices(g, 1, n_out, n_in)
+    q, s = quantize(torch.randn((C, n_in), generator=g))
+    out = torch.full((C, n_out), 77.0, dtype=OUT[t], device="cuda")
+    moe.f8_gemm(blob[0].cuda(), n_out, n_in, dev(q), dev(s), out)
+    want, bound = product(dequantize(q, s), W[0], True)
+    close(out, want, bound, OUT[t], many=True)
