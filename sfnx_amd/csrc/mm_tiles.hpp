@@ -38,7 +38,7 @@ static_assert(T_LDS <= 160 * 1024 && T_LDS >= S1_LDS && 4 * WINDOW <= SG_LIST, "
 // an expert's weights come from HBM once for them; xg = XG, or 1 where there are too few to use all XCDs evenly (single jobs, few
 // of one expert, 2 for 4: down of 777 tokens 129 -> 124 us; groups 4 for 1: bf16 experts of 4096 tokens 307 -> 297).  A dense
 // product of few groups leaves XCDs idle that way: where fewer rounds of the compute units come of it, an XCD takes every 8th
-// slice of all groups (across; 128 rows, 4096 -> 8192: 41.5 -> 20.9 us).  false: no such group or slice
+// slice of all groups (across; 128 rows, 4096 -> 8192: 41.8 -> 20.5 us).  false: no such group or slice
 template <int XG> __device__ __forceinline__ bool tile_at(int b, int nsl, int n, bool across, int& sl, int& i) {
     const int p = across ? n : nsl, xg = n >= 64 ? XG : 1;
     const int x = b % XCDS, k = b / XCDS, m = k / p, u = k % p, v = xg * (XCDS * (m / xg) + x) + m % xg;
@@ -54,8 +54,8 @@ __host__ __device__ __forceinline__ int64_t tiles_of(int nsl, int n, bool across
     return across ? (int64_t) (nsl + XCDS - 1) / XCDS * XCDS * n : (int64_t) nsl * ((n + 31) / 32) * 32;
 }
 
-// The place of a slice's weight row in LDS.  STORE: wavefronts' rows in order.  SWIGLU: of each W = 2 NT tiles of 16 that a
-// wavefront owns, the first NT are gate tiles and the others their up tiles.
+// The weight row at place i of a slice.  STORE: the rows in order.  SWIGLU: of the NT2 tiles of 16 that a wavefront owns, the
+// first half are gate tiles and the others their up tiles.
 template <Mode MODE, int NT2, int N = BN> __device__ __forceinline__ int weight_row(const Args& a, int sl, int i) {
     const int n_eff = MODE == SWIGLU ? a.n_out / 2 : a.n_out;
     if (MODE == STORE) return min(sl * N + i, a.n_out - 1);
