@@ -102,7 +102,7 @@ __device__ __forceinline__ const float* scales_of(const uint8_t* mat, int rows, 
 // fp32 quotient, at most 448 in size.  The floor of s keeps the quotient of a block of zeros (or of values below 448 2^-126) defined.  What is not
 // finite becomes the type's NaN.
 //
-// The quotient: with r = 1 / s rounded, x r is within a unit of x / s, and adding (x - (x r) s) r, both products fused, rounds
+// The quotient: with r = 1 / s rounded, x r is within a unit of x / s, and taking away ((x r) s - x) r, both products fused, rounds
 // it correctly (Markstein): three instructions for a division's ten.  The remainder has to stay above the smallest numbers,
 // so scales below 2^-90 divide; so do blocks with values that are not finite.
 __device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }   // not finite: 0x7f800000 on
@@ -123,7 +123,7 @@ __device__ __forceinline__ uint32_t f8_pack4(float a, float b, float c, float d,
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const float q = v[i] * k.r;
-            t[i] = fmaf(fmaf(-q, k.s, v[i]), k.r, q);
+            t[i] = fmaf(-fmaf(q, k.s, -v[i]), k.r, q);   // in this order a zero keeps its sign: -0 s + 0 = +0, then (-0) r + -0 = -0
         }
     } else {
 #pragma unroll
