@@ -227,6 +227,7 @@ def _fine(t, dtypes, shape, dev) -> bool:
 
 _F8_BYTES = (torch.uint8, torch.float8_e4m3fn)
 _F32, _I32 = (torch.float32,), (torch.int32,)
+_POINTERS = (torch.int64, torch.uint64)
 
 
 def _need_rows(q, s, qn: str, sn: str, cols: int, dev) -> None:
@@ -241,6 +242,28 @@ def _need_out(t, name: str, dtypes, cols: int, dev) -> None:
     """rows of cols values"""
     if not _fine(t, dtypes, (t.shape[0] if t.dim() else 0, cols), dev):
         _need(t, name, dtypes, (None, cols))
+
+
+def _need_experts(A, sa: int, matrix: int, dtypes) -> None:
+    """expert matrices of `matrix` bytes, sa bytes apart, or (sa 0) a table of their pointers: jobs name experts on the GPU, so
+    how many there are is not known here, but one there must be"""
+    if sa == 0:
+        if A.dtype not in _POINTERS:
+            raise ValueError(f"A: type {A.dtype}, expected a table of pointers (int64) where the stride is 0")
+        if A.numel() < 1:
+            raise ValueError("A: an empty table")
+        return
+    if A.dtype not in dtypes:
+        raise ValueError(f"A: type {A.dtype}, expected {' or '.join(str(d) for d in dtypes)}")
+    if sa < 0:
+        raise ValueError("A: stride below 0")
+    if A.numel() * A.element_size() < matrix:
+        raise ValueError("A: smaller than a matrix")
+
+
+def _f8_bytes(rows: int, cols: int) -> int:
+    """an 8-bit matrix without the store's padding"""
+    return rows * cols + 4 * ((rows + 127) // 128) * ((cols + 127) // 128)
 
 
 def _need_jobs(A, jobs, njobs, n: int, ints: int, dev) -> None:
@@ -284,7 +307,7 @@ def f8_gemm(W, rows: int, cols: int, xq, xs, out) -> None:
     dev = _current()
     if W.dtype is not torch.uint8 or W.get_device() != dev or not W.is_contiguous():
         _need(W, "W", (torch.uint8,))
-    if W.numel() < rows * cols + 4 * ((rows + 127) // 128) * ((cols + 127) // 128):
+    if W.numel() < _f8_bytes(rows, cols):
         raise ValueError("W: smaller than the matrix")
     _need_rows(xq, xs, "xq", "xs", cols, dev)
     C = xq.shape[0]
@@ -297,6 +320,7 @@ def f8_gemm(W, rows: int, cols: int, xq, xs, out) -> None:
 def moe_gate_up_swiglu_f8(A, sa, n_in, ff, jobs, njobs, njobs_max, xq, xs, h) -> None:
     """a window's h rows (f32) = silu(gate) * up of the 8-bit rows xq, xs, over jobs"""
     dev = _current()
+    _need_experts(A, sa, _f8_bytes(2 * ff, n_in), _F8_BYTES)
     _need_jobs(A, jobs, njobs, njobs_max, JOB_INTS, dev)
     _need_rows(xq, xs, "xq", "xs", n_in, dev)
     _need_out(h, "h", _F32, ff, dev)
@@ -307,6 +331,7 @@ def moe_gate_up_swiglu_f8(A, sa, n_in, ff, jobs, njobs, njobs_max, xq, xs, h) ->
 def moe_down_f8(A, sa, n_in, n_out, jobs, njobs, njobs_max, h, out) -> None:
     """a window's out rows = the experts' rows times h's (f32, quantized in the call), over jobs"""
     dev = _current()
+    _need_experts(A, sa, _f8_bytes(n_out, n_in), _F8_BYTES)
     _need_jobs(A, jobs, njobs, njobs_max, JOB_INTS, dev)
     _need_out(h, "h", _F32, n_in, dev)
     _need_out(out, "out", _TYPE_ID, n_out, dev)
@@ -317,6 +342,7 @@ def moe_down_f8(A, sa, n_in, n_out, jobs, njobs, njobs_max, h, out) -> None:
 def moe_gate_up_swiglu_f8_big(A, sa, n_in, ff, jobs, njobs, njobs_cap, xq, xs, hq, hs) -> None:
     """a chunk's 8-bit h rows hq, hs = silu(gate) * up of the 8-bit rows xq, xs, over BigJobs"""
     dev = _current()
+    _need_experts(A, sa, _f8_bytes(2 * ff, n_in), _F8_BYTES)
     _need_jobs(A, jobs, njobs, njobs_cap, BIGJOB_INTS, dev)
     _need_rows(xq, xs, "xq", "xs", n_in, dev)
     _need_rows(hq, hs, "hq", "hs", ff, dev)
@@ -327,6 +353,7 @@ def moe_gate_up_swiglu_f8_big(A, sa, n_in, ff, jobs, njobs, njobs_cap, xq, xs, h
 def moe_down_f8_big(A, sa, n_in, n_out, jobs, njobs, njobs_cap, hq, hs, out) -> None:
     """a chunk's out rows = the experts' rows times the 8-bit rows hq, hs, over BigJobs"""
     dev = _current()
+    _need_experts(A, sa, _f8_bytes(n_out, n_in), _F8_BYTES)
     _need_jobs(A, jobs, njobs, njobs_cap, BIGJOB_INTS, dev)
     _need_rows(hq, hs, "hq", "hs", n_in, dev)
     _need_out(out, "out", _TYPE_ID, n_out, dev)
@@ -336,11 +363,12 @@ def moe_down_f8_big(A, sa, n_in, n_out, jobs, njobs, njobs_cap, hq, hs, out) -> 
 
 def _mm_16(fn, ints, A, sa, n_in, n_out, jobs, njobs, n, x, out) -> None:
     dev = _current()
+    if sa != 0 and A.dtype is not x.dtype:
+        raise ValueError("A: another type than x")
+    _need_experts(A, sa, 2 * n_out * n_in, (torch.float16, torch.bfloat16))
     _need_jobs(A, jobs, njobs, n, ints, dev)
     _need_out(x, "x", (torch.float16, torch.bfloat16), n_in, dev)
     _need_out(out, "out", _TYPE_ID, n_out, dev)
-    if sa != 0 and A.dtype is not x.dtype:
-        raise ValueError("A: another type than x")
     check(fn(A.data_ptr(), sa, _TYPE_ID[x.dtype], n_in, n_out, jobs.data_ptr(), njobs.data_ptr(), n, x.data_ptr(),
              _TYPE_ID[out.dtype], out.data_ptr(), _st()))
 

@@ -1,0 +1,64 @@
+"""What the Python calls of the 8-bit and 16-bit experts refuse before anything is launched: expert matrices of another size,
+type or stride than the call's."""
+import pytest
+import torch
+
+from sfnx_amd import _abi, moe
+
+N_IN, N_OUT, ROWS = 256, 256, 5
+MAT8 = N_OUT * N_IN + 4 * 2 * 2
+U8, F16, BF16, I32, F32 = torch.uint8, torch.float16, torch.bfloat16, torch.int32, torch.float32
+
+
+def grouped(name, A, sa):
+    """one of the grouped calls, right but for its experts; on the CPU, where the right call is refused for its tensors' place"""
+    big = name.endswith("big")
+    jobs = torch.zeros(2 * (_abi.BIGJOB_INTS if big else _abi.JOB_INTS), dtype=I32), torch.zeros(2, dtype=I32), 2
+    q, s = torch.zeros((ROWS, N_IN), dtype=U8), torch.zeros((ROWS, 2))
+    out = torch.zeros((ROWS, N_OUT))
+    ff = N_OUT // 2
+    if name == "gate_up":
+        moe.moe_gate_up_swiglu_f8(A, sa, N_IN, ff, *jobs, q, s, torch.zeros((ROWS, ff)))
+    elif name == "gate_up_big":
+        moe.moe_gate_up_swiglu_f8_big(A, sa, N_IN, ff, *jobs, q, s, torch.zeros((ROWS, ff), dtype=U8), torch.zeros((ROWS, 1)))
+    elif name == "down":
+        moe.moe_down_f8(A, sa, N_IN, N_OUT, *jobs, torch.zeros((ROWS, N_IN)), out)
+    elif name == "down_big":
+        moe.moe_down_f8_big(A, sa, N_IN, N_OUT, *jobs, q, s, out)
+    else:
+        (moe.moe_mm_16_big if big else moe.moe_mm_16)(A, sa, N_IN, N_OUT, *jobs, torch.zeros((ROWS, N_IN), dtype=F16), out)
+
+
+F8_CALLS = ["gate_up", "gate_up_big", "down", "down_big"]
+MM_CALLS = ["mm", "mm_big"]
+
+
+@pytest.mark.parametrize("name", F8_CALLS + MM_CALLS)
+def test_experts_of_another_size(name):
+    """experts that do not hold one matrix of the call's, a negative stride, an empty table"""
+    f8 = name in F8_CALLS
+    t, size, n = (U8, 1, MAT8) if f8 else (F16, 2, N_OUT * N_IN)
+    sa = (n * size + 15) // 16 * 16
+    with pytest.raises(ValueError, match="A: smaller than a matrix"):
+        grouped(name, torch.zeros(n - 1, dtype=t), sa)
+    with pytest.raises(ValueError, match="A: stride"):
+        grouped(name, torch.zeros(n, dtype=t), -16)
+    with pytest.raises(ValueError, match="A: an empty table"):
+        grouped(name, torch.zeros(0, dtype=torch.int64), 0)
+    for A, stride in ((torch.zeros(n, dtype=t), sa), (torch.zeros(1, dtype=torch.int64), 0)):
+        with pytest.raises(ValueError, match="A: not on the current GPU"):   # nothing else is wrong
+            grouped(name, A, stride)
+
+
+@pytest.mark.parametrize("name", F8_CALLS + MM_CALLS)
+def test_experts_of_another_type(name):
+    """matrices of another type than the call's; matrices where their pointers are meant, and the other way about"""
+    f8 = name in F8_CALLS
+    t, other = (U8, F16) if f8 else (F16, BF16)
+    sa = 4 * N_OUT * N_IN
+    for wrong in (other, F32, torch.int64):
+        with pytest.raises(ValueError, match="A: type" if f8 else "A: another type than x"):
+            grouped(name, torch.zeros(8 * N_OUT * N_IN, dtype=wrong), sa)
+    for wrong in (t, I32, F32):
+        with pytest.raises(ValueError, match="A: type .* pointers"):
+            grouped(name, torch.zeros(8 * N_OUT * N_IN, dtype=wrong), 0)
