@@ -717,7 +717,7 @@ class FloatBuffers:
         s, big = shape, T > _abi.MAXT
         P = T * s.K
         NP = P + (T if s.shared else 0)
-        self.T, self.big = T, big
+        self.s, self.T, self.big = shape, T, big
         self.cap = P // PF_JOB + s.E + (T + PF_JOB - 1) // PF_JOB + 1 if big else P + 1
         i32 = dict(dtype=torch.int32, device=device)
         f32 = dict(dtype=torch.float32, device=device)
@@ -747,8 +747,15 @@ def _route(L, x, b) -> None:
 
 
 def _need_call(L, x, y, b) -> None:
+    """the routing checks no sizes of its own: buffers of the layer's shape, and the tensors it takes on the current GPU (the
+    later calls check theirs)"""
+    s, o = L.s, b.s
+    if (o.H, o.E, o.K, o.ff, o.shared) != (s.H, s.E, s.K, s.ff, s.shared):
+        raise ValueError("b: made for another shape than the layer's")
     _need(x, "x", (torch.float32,), (b.T, L.s.H))
     _need(y, "y", (torch.float32,), (b.T, L.s.H))
+    _need(L.W, "W", _F32)
+    _need(b.logits, "b.logits", _F32)
 
 
 def layer_f8(L: MoeLayerF8, x: torch.Tensor, y: torch.Tensor, b: FloatBuffers) -> None:

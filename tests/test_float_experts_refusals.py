@@ -62,3 +62,26 @@ def test_experts_of_another_type(name):
     for wrong in (t, I32, F32):
         with pytest.raises(ValueError, match="A: type .* pointers"):
             grouped(name, torch.zeros(8 * N_OUT * N_IN, dtype=wrong), 0)
+
+
+SHAPE = dict(H=1024, E=64, K=6, ff=256, shared=True)
+
+
+def layer_on_the_cpu(cls, shape):
+    L = cls.__new__(cls)   # the constructor asks for tensors on the GPU
+    L.s, L.W = shape, torch.zeros((shape.E + 1, shape.H))
+    return L
+
+
+@pytest.mark.parametrize("cls, call", [(moe.MoeLayerF8, moe.layer_f8), (moe.MoeLayer16, moe.layer_16)])
+@pytest.mark.parametrize("T", [3, 40])
+@pytest.mark.parametrize("other", [dict(H=2048), dict(E=32), dict(E=128), dict(K=4), dict(K=8), dict(ff=128), dict(shared=False)])
+def test_layer_with_buffers_of_another_shape(cls, call, T, other):
+    """the routing writes E + 1 logits and K picks a token, so smaller buffers would be written past their ends"""
+    s = moe.LayerShape(**SHAPE)
+    b = moe.FloatBuffers(moe.LayerShape(**{**SHAPE, **other}), T, device="cpu")
+    x, y = torch.zeros((T, s.H)), torch.zeros((T, s.H))
+    with pytest.raises(ValueError, match="b: made for another shape"):
+        call(layer_on_the_cpu(cls, s), x, y, b)
+    with pytest.raises(ValueError, match="x: not on the current GPU"):   # the right buffers: nothing else is wrong
+        call(layer_on_the_cpu(cls, s), x, y, moe.FloatBuffers(moe.LayerShape(**SHAPE, wtype=moe.Q8_0), T, device="cpu"))
