@@ -227,6 +227,7 @@ def _fine(t, dtypes, shape, dev) -> bool:
 
 _F8_BYTES = (torch.uint8, torch.float8_e4m3fn)
 _F32, _I32 = (torch.float32,), (torch.int32,)
+_INT_MAX = 2 ** 31 - 1
 _POINTERS = (torch.int64, torch.uint64)
 
 
@@ -244,9 +245,16 @@ def _need_out(t, name: str, dtypes, cols: int, dev) -> None:
         _need(t, name, dtypes, (None, cols))
 
 
-def _need_experts(A, sa: int, matrix: int, dtypes) -> None:
-    """expert matrices of `matrix` bytes, sa bytes apart, or (sa 0) a table of their pointers: jobs name experts on the GPU, so
-    how many there are is not known here, but one there must be"""
+def _too_large(name: str, shape) -> None:
+    """rows, columns and an output's stride are 32-bit integers at the library, which would cut larger ones"""
+    raise ValueError(f"{name}: {max(shape)} rows or columns, more than {_INT_MAX}")
+
+
+def _need_experts(A, sa: int, rows: int, cols: int, matrix: int, dtypes) -> None:
+    """expert matrices [rows][cols] of `matrix` bytes, sa bytes apart, or (sa 0) a table of their pointers: jobs name
+    experts on the GPU, so how many there are is not known here, but one there must be"""
+    if rows > _INT_MAX or cols > _INT_MAX:
+        _too_large("A", (rows, cols))
     if sa == 0:
         if A.dtype not in _POINTERS:
             raise ValueError(f"A: type {A.dtype}, expected a table of pointers (int64) where the stride is 0")
@@ -292,6 +300,8 @@ def f8_matrix_bytes(rows: int, cols: int) -> int:
 def quantize_f8(x, q, s) -> None:
     """rows of x (f32, f16 or bf16; rows may be strided) as e4m3 rows q with a scale s for each 128 values"""
     dev = _current()
+    if x.dim() == 2 and (x.shape[0] > _INT_MAX or x.shape[1] > _INT_MAX):
+        _too_large("x", x.shape)
     if x.dim() != 2 or not _fine(x, _TYPE_ID, x.shape, dev):
         _need(x, "x", tuple(_TYPE_ID), (None, None), rows_strided=True)
     rows, cols = x.shape
@@ -305,22 +315,29 @@ def quantize_f8(x, q, s) -> None:
 def f8_gemm(W, rows: int, cols: int, xq, xs, out) -> None:
     """out [C][rows] (f32, f16 or bf16; rows may be strided) = the 8-bit rows xq, xs [C][cols] times the 8-bit matrix W"""
     dev = _current()
+    if rows > _INT_MAX or cols > _INT_MAX:
+        _too_large("W", (rows, cols))
+    C = xq.shape[0] if xq.dim() else 0
+    if C > _INT_MAX:
+        _too_large("xq", xq.shape)
+    ldo = out.stride(0) if C > 1 and out.dim() else rows
+    if ldo > _INT_MAX:
+        raise ValueError(f"out: rows {ldo} values apart, more than {_INT_MAX}")
     if W.dtype is not torch.uint8 or W.get_device() != dev or not W.is_contiguous():
         _need(W, "W", (torch.uint8,))
     if W.numel() < _f8_bytes(rows, cols):
         raise ValueError("W: smaller than the matrix")
     _need_rows(xq, xs, "xq", "xs", cols, dev)
-    C = xq.shape[0]
     if not _fine(out, _TYPE_ID, (C, rows), dev):
         _need(out, "out", tuple(_TYPE_ID), (C, rows), rows_strided=True)
     check(lib().sfnx_f8_gemm(W.data_ptr(), rows, cols, xq.data_ptr(), xs.data_ptr(), C, _TYPE_ID[out.dtype], out.data_ptr(),
-                             out.stride(0) if C > 1 else rows, _st()))
+                             ldo, _st()))
 
 
 def moe_gate_up_swiglu_f8(A, sa, n_in, ff, jobs, njobs, njobs_max, xq, xs, h) -> None:
     """a window's h rows (f32) = silu(gate) * up of the 8-bit rows xq, xs, over jobs"""
     dev = _current()
-    _need_experts(A, sa, _f8_bytes(2 * ff, n_in), _F8_BYTES)
+    _need_experts(A, sa, 2 * ff, n_in, _f8_bytes(2 * ff, n_in), _F8_BYTES)
     _need_jobs(A, jobs, njobs, njobs_max, JOB_INTS, dev)
     _need_rows(xq, xs, "xq", "xs", n_in, dev)
     _need_out(h, "h", _F32, ff, dev)
@@ -331,7 +348,7 @@ def moe_gate_up_swiglu_f8(A, sa, n_in, ff, jobs, njobs, njobs_max, xq, xs, h) ->
 def moe_down_f8(A, sa, n_in, n_out, jobs, njobs, njobs_max, h, out) -> None:
     """a window's out rows = the experts' rows times h's (f32, quantized in the call), over jobs"""
     dev = _current()
-    _need_experts(A, sa, _f8_bytes(n_out, n_in), _F8_BYTES)
+    _need_experts(A, sa, n_out, n_in, _f8_bytes(n_out, n_in), _F8_BYTES)
     _need_jobs(A, jobs, njobs, njobs_max, JOB_INTS, dev)
     _need_out(h, "h", _F32, n_in, dev)
     _need_out(out, "out", _TYPE_ID, n_out, dev)
@@ -342,7 +359,7 @@ def moe_down_f8(A, sa, n_in, n_out, jobs, njobs, njobs_max, h, out) -> None:
 def moe_gate_up_swiglu_f8_big(A, sa, n_in, ff, jobs, njobs, njobs_cap, xq, xs, hq, hs) -> None:
     """a chunk's 8-bit h rows hq, hs = silu(gate) * up of the 8-bit rows xq, xs, over BigJobs"""
     dev = _current()
-    _need_experts(A, sa, _f8_bytes(2 * ff, n_in), _F8_BYTES)
+    _need_experts(A, sa, 2 * ff, n_in, _f8_bytes(2 * ff, n_in), _F8_BYTES)
     _need_jobs(A, jobs, njobs, njobs_cap, BIGJOB_INTS, dev)
     _need_rows(xq, xs, "xq", "xs", n_in, dev)
     _need_rows(hq, hs, "hq", "hs", ff, dev)
@@ -353,7 +370,7 @@ def moe_gate_up_swiglu_f8_big(A, sa, n_in, ff, jobs, njobs, njobs_cap, xq, xs, h
 def moe_down_f8_big(A, sa, n_in, n_out, jobs, njobs, njobs_cap, hq, hs, out) -> None:
     """a chunk's out rows = the experts' rows times the 8-bit rows hq, hs, over BigJobs"""
     dev = _current()
-    _need_experts(A, sa, _f8_bytes(n_out, n_in), _F8_BYTES)
+    _need_experts(A, sa, n_out, n_in, _f8_bytes(n_out, n_in), _F8_BYTES)
     _need_jobs(A, jobs, njobs, njobs_cap, BIGJOB_INTS, dev)
     _need_rows(hq, hs, "hq", "hs", n_in, dev)
     _need_out(out, "out", _TYPE_ID, n_out, dev)
@@ -365,7 +382,7 @@ def _mm_16(fn, ints, A, sa, n_in, n_out, jobs, njobs, n, x, out) -> None:
     dev = _current()
     if sa != 0 and A.dtype is not x.dtype:
         raise ValueError("A: another type than x")
-    _need_experts(A, sa, 2 * n_out * n_in, (torch.float16, torch.bfloat16))
+    _need_experts(A, sa, n_out, n_in, 2 * n_out * n_in, (torch.float16, torch.bfloat16))
     _need_jobs(A, jobs, njobs, n, ints, dev)
     _need_out(x, "x", (torch.float16, torch.bfloat16), n_in, dev)
     _need_out(out, "out", _TYPE_ID, n_out, dev)

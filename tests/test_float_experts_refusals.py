@@ -85,3 +85,27 @@ def test_layer_with_buffers_of_another_shape(cls, call, T, other):
         call(layer_on_the_cpu(cls, s), x, y, b)
     with pytest.raises(ValueError, match="x: not on the current GPU"):   # the right buffers: nothing else is wrong
         call(layer_on_the_cpu(cls, s), x, y, moe.FloatBuffers(moe.LayerShape(**SHAPE, wtype=moe.Q8_0), T, device="cpu"))
+
+
+def test_rows_and_strides_past_the_library_s_integers():
+    """the library takes rows and an output's stride as 32-bit integers: what does not fit is refused, not cut"""
+    far, rows = 1 << 32, (1 << 32) + 5
+    meta = dict(device="meta")   # sizes without memory
+    with pytest.raises(ValueError, match="x: .* rows"):
+        moe.quantize_f8(torch.empty((rows, 16), **meta), torch.empty((rows, 16), dtype=U8, **meta), torch.empty((rows, 1), **meta))
+    W = torch.empty(MAT8 + 16, dtype=U8, **meta)
+    q, s = torch.empty((2, N_IN), dtype=U8, **meta), torch.empty((2, 2), **meta)
+    with pytest.raises(ValueError, match="out: .* apart"):
+        moe.f8_gemm(W, N_OUT, N_IN, q, s, torch.empty_strided((2, N_OUT), (far + N_OUT, 1), **meta))
+    q, s = torch.empty((rows, N_IN), dtype=U8, **meta), torch.empty((rows, 2), **meta)
+    with pytest.raises(ValueError, match="xq: .* rows"):
+        moe.f8_gemm(W, N_OUT, N_IN, q, s, torch.empty((rows, N_OUT), **meta))
+    q, s = torch.empty((2, far + 16), dtype=U8, **meta), torch.empty((2, (far + 16 + 127) // 128), **meta)
+    with pytest.raises(ValueError, match="x: .* columns"):
+        moe.quantize_f8(torch.empty((2, far + 16), **meta), q, s)
+    with pytest.raises(ValueError, match="W: .* columns"):
+        moe.f8_gemm(torch.empty(far + (1 << 30), dtype=U8, **meta), 1, far + 16, q, s, torch.empty((2, 1), **meta))
+    jobs = torch.empty(2 * _abi.JOB_INTS, dtype=I32, **meta), torch.empty(2, dtype=I32, **meta), 2
+    with pytest.raises(ValueError, match="A: .* columns"):
+        moe.moe_mm_16(torch.empty(4 * far, dtype=F16, **meta), 4 * far, N_IN, far + 8, *jobs, torch.empty((2, N_IN), dtype=F16, **meta),
+                      torch.empty((2, far + 8), dtype=F16, **meta))
