@@ -6,7 +6,7 @@ from pathlib import Path
 
 HERE = Path(__file__).resolve().parent
 ROOT = HERE.parent.parent
-PROGRAMS = ["moe_window"]
+PROGRAMS = ["moe_window", "float_experts"]
 
 
 def build(verbose: bool = False) -> None:
