@@ -265,7 +265,7 @@ def _need_experts(A, sa: int, rows: int, cols: int, matrix: int, dtypes) -> None
         raise ValueError(f"A: type {A.dtype}, expected {' or '.join(str(d) for d in dtypes)}")
     if sa < 0:
         raise ValueError("A: stride below 0")
-    if A.numel() * A.element_size() < matrix:
+    if A.nbytes < matrix:
         raise ValueError("A: smaller than a matrix")
 
 
@@ -300,11 +300,13 @@ def f8_matrix_bytes(rows: int, cols: int) -> int:
 def quantize_f8(x, q, s) -> None:
     """rows of x (f32, f16 or bf16; rows may be strided) as e4m3 rows q with a scale s for each 128 values"""
     dev = _current()
-    if x.dim() == 2 and (x.shape[0] > _INT_MAX or x.shape[1] > _INT_MAX):
-        _too_large("x", x.shape)
-    if x.dim() != 2 or not _fine(x, _TYPE_ID, x.shape, dev):
-        _need(x, "x", tuple(_TYPE_ID), (None, None), rows_strided=True)
+    if x.dim() != 2:
+        _need(x, "x", tuple(_TYPE_ID), (None, None))
     rows, cols = x.shape
+    if rows > _INT_MAX or cols > _INT_MAX:
+        _too_large("x", (rows, cols))
+    if not _fine(x, _TYPE_ID, (rows, cols), dev):
+        _need(x, "x", tuple(_TYPE_ID), (None, None), rows_strided=True)
     if not _fine(q, _F8_BYTES, (rows, cols), dev) or not _fine(s, _F32, (rows, (cols + 127) // 128), dev):
         _need(q, "q", _F8_BYTES, (rows, cols))
         _need(s, "s", _F32, (rows, (cols + 127) // 128))
