@@ -188,13 +188,17 @@ int sfnx_pf_dense(const sfnx_q8s* W, int rows, int cols, const uint16_t* xh, int
  * 4 exponent and 3 mantissa bits without infinities, largest value 448) with an f32 scale for each block of 128.  A matrix
  * [rows][cols] of the 8-bit store is its values, row-major, then the scales of its 128 x 128 blocks
  * [ceil(rows / 128)][ceil(cols / 128)] (the last blocks of a row or column may be shorter); an activation row has a scale for
- * each 128 values, [rows][ceil(cols / 128)].  A product is the
- * sum over b of (xs_b ws_b) (sum over the block's k of xq[k] wq[k]), on the matrix cores: in fp32 where the result is kept
- * in 32 bits or quantized again, in a window's calls and in dense ones of up to 16 rows; where a larger call rounds it to 16
- * bits, sums of 8 consecutive products keep 13 bits of the largest, 1.5e-5 of the result's norm, and the rest is fp32.
+ * each 128 values, [rows][ceil(cols / 128)].  A product is the sum over b of (xs_b ws_b) (sum over the block's k of
+ * xq[k] wq[k]), on the matrix cores, the scales' product rounded to fp32.  It is summed in fp32 where the result is kept in 32
+ * bits or quantized again, in a window's calls and in dense ones of up to 16 rows.  Where a larger call rounds it to 16 bits,
+ * sums of 8 consecutive products keep 13 bits of the largest, and the rest is fp32: a product is off by at most 2^-13 of the
+ * largest of its 8, so an output by at most 7 2^-13 of the sum of its terms' sizes.  On normal data that measured 1.5e-5 of
+ * the result's norm; where large terms cancel it can be all of an output (and 16 and 17 dense rows then differ by as much):
+ * take such sums with out_type SFNX_F32.
  * cols % 16 == 0, rows and cols at most 2^20, a matrix smaller than 4 GiB; pointers 16-byte aligned (outputs and scales to
  * their type); expert strides a multiple of 16, or 0 for a table of expert pointers; out_type SFNX_F32, SFNX_F16 or SFNX_BF16.
- * jobs holds njobs_max (njobs_cap) entries, of which the first *njobs are jobs.  Rows that no job names are left as they were.
+ * jobs holds njobs_max (njobs_cap) entries, of which the first *njobs are jobs; a job may have no rows, its w is one of A's
+ * experts all the same.  Rows that no job names are left as they were.
  * A matrix's values and the activation rows are read as they are: a NaN reaches every output it belongs to. */
 /* bytes of a matrix of the 8-bit store, rounded up to 16 */
 size_t sfnx_f8_matrix_bytes(int rows, int cols);

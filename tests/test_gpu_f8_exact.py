@@ -135,3 +135,33 @@ def test_prompt_down_sums_in_32_bits(T, E, K, H, ff):
     moe.moe_down_f8_big(d, d.stride(0), ff, H, *job_tensors(a, n), dev(q), dev(s), out)
     want, _, where = grouped(x, W, flat, True)
     assert torch.equal(out[where.cuda()].double().cpu(), want)
+
+
+@pytest.mark.parametrize("t", ["f16", "bf16"])
+@pytest.mark.parametrize("C, n_in, n_out", [(17, 144, 40), (40, 1024, 200), (300, 528, 1301), (700, 1040, 2100), (1290, 2064, 4101), (3073, 2064, 4101)])
+def test_dense_16_bit_outputs_within_the_stated_bound(C, n_in, n_out, t):
+    """more rows into 16 bits: each output within 7 2^-13 of the sum of its terms' sizes, on sums that cancel too"""
+    g = gen(C + n_in)
+    blob, W = weights_of(g, 1, n_out, n_in)
+    q, s, x = rows_of(g, C, n_in)
+    out = torch.full((C, n_out), 77.0, dtype=OUT[t], device="cuda")
+    moe.f8_gemm(dev(blob), n_out, n_in, dev(q), dev(s), out)
+    x, W = dev(x), dev(W[0])
+    want, sizes = x @ W.t(), x.abs() @ W.abs().t()
+    bound = (COARSE + (128 + nb(n_in) + 3) * ULP) * sizes
+    assert ((out.double() - want).abs() <= bound + half_step(OUT[t], want.abs() + bound)).all()
+
+
+@pytest.mark.parametrize("t", ["f16", "bf16"])
+@pytest.mark.parametrize("T, E, K, H, ff", [(20, 8, 3, 256, 128), (300, 4, 2, 1043, 272)])
+def test_prompt_down_16_bit_outputs_within_the_stated_bound(T, E, K, H, ff, t):
+    g, rng = gen(T), np.random.default_rng(T)
+    blob, W = weights_of(g, E + 1, H, ff)
+    q, s, x = rows_of(g, T * K + T, ff)
+    a, n, flat = jobs(picks(rng, T, E, K), E, True, 64, False)
+    d, out = dev(blob), torch.full((T * K + T, H), 77.0, dtype=OUT[t], device="cuda")
+    moe.moe_down_f8_big(d, d.stride(0), ff, H, *job_tensors(a, n), dev(q), dev(s), out)
+    want, _, where = grouped(x, W, flat, True)
+    sizes, _, _ = grouped(x.abs(), W.abs(), flat, True)
+    bound = (COARSE + (128 + nb(ff) + 3) * ULP) * sizes
+    assert ((out[where.cuda()].double().cpu() - want).abs() <= bound + half_step(OUT[t], want.abs() + bound)).all()
