@@ -95,14 +95,15 @@ void check_f8_rows(const uint8_t* xq, const float* xs) {
 }
 
 // A dense product of more than 16 rows: the form of the least estimated time.  A form's tile takes `one` us for 4096 columns
-// when all tiles run at once, `more` in further rounds of 256 workgroups, and `fixed` us whatever the columns; measured with
-// matrices of 256 to 4096 rows, 512 to 4096 columns and 17 to 4096 rows of activations (us, into bf16; 4096 columns):
-//   rows x rows      32x16 mid  32x32 mid  32x64 mid  64x128 streamed  64x256 streamed  256x256 grouped
-//   128 x 256           9.4        11.3       15.5          27               31               52
-//   256 x 1024         16.8        11.8       15.6          27               33               64
-//   512 x 2048         58          37         30            28               33               65
-//   1024 x 4096       224         141        114            69               36               66
-//   4096 x 4096                                                             127               69
+// when all tiles run at once, `more` in further rounds of 256 workgroups, and `fixed` us whatever the columns; fitted to
+// matrices of 256 to 4096 rows, 512 to 4096 columns and 17 to 4096 rows of activations.  Of them, with 4096 columns, us in a
+// graph, into bf16 and (F8X) into f32, whose third form has 64 rows by 32:
+//   rows x rows      32x16 mid     32x32 mid     32x64 mid     64x128 streamed  64x256 streamed  256x256 grouped
+//   128 x 256         9.7   9.8    11.7  11.8    15.8  18.1     18.9  29.7       28.1  40.6       37.0  69.5
+//   256 x 1024       16.8  17.0    11.9  12.2    15.9  18.4     19.3  30.4       28.5  41.1       55.7 122
+//   512 x 2048       58.7  59.0    38.1  42.3    30.5  35.5     23.9  34.1       31.4  42.7       61.2 126
+//   1024 x 4096     226   226     143   162     114   134       46.7  66.1       34.8  47.5       66.0 128
+//   4096 x 4096                                                168   238        120   174         76.2 138
 struct DenseForm {
     int rows, cols;
     float one, more, fixed;

@@ -8,8 +8,9 @@
 //
 // e4m3 steps start their matrix instructions from zero and add the result times the block's two scales in fp32.  There are two
 // forms.  F8, v_mfma_f32_16x16x128_f8f6f4: measured, it adds the products of 8 consecutive k to a common unit of 2^-13 of
-// the largest (a product 2^-14 of a neighbour's size is lost) and these sums in fp32, which leaves normal data 1.5e-5 of the
-// result's norm off; it serves outputs that are rounded to 16 bits (2^-9, 2^-12) anyway.  F8X: the values converted to f16,
+// the largest (a product 2^-14 of a neighbour's size is lost) and these sums in fp32: an output is off by at most 7 2^-13 of the
+// sum of its terms' sizes, on normal data by 1.5e-5 of the result's norm, where large terms cancel by up to all of it.  It serves
+// outputs that are rounded to 16 bits (2^-9, 2^-12) anyway.  F8X: the values converted to f16,
 // exactly, and summed by four v_mfma_f32_16x16x32_f16, whose sums are fp32's (1e-8 on the same data), at half the rate; it
 // serves outputs kept in 32 bits, the scales of quantized ones, and products of few rows, which wait for the weights anyway.
 #pragma once
@@ -102,9 +103,12 @@ __device__ __forceinline__ const float* scales_of(const uint8_t* mat, int rows, 
 // fp32 quotient, at most 448 in size.  The floor of s keeps the quotient of a block of zeros (or of values below 448 2^-126) defined.  What is not
 // finite becomes the type's NaN.
 //
-// The quotient: with r = 1 / s rounded, x r is within a unit of x / s, and taking away ((x r) s - x) r, both products fused, rounds
-// it correctly (Markstein): three instructions for a division's ten.  The remainder has to stay above the smallest numbers,
-// so scales below 2^-90 divide; so do blocks with values that are not finite.
+// The quotient: with r = 1 / s rounded, x r is within 1.5 units of x / s, and ((x r) s - x) r, both products fused, is taken away
+// (Markstein's step): three instructions for a division's ten.  r is within 2^-24 of 1 / s, so what is rounded last is within
+// 1.5 2^-24 units of x / s; its rounding could be another one only beside a border of fp32, which matters to a code only at
+// e4m3's ties.  Compared there: all 2^23 scales of a binade with the seven values nearest to each of its ties, 940 million
+// quotients, every one the division's.  The remainder has to stay above the smallest numbers, so scales below 2^-90 divide; so
+// do blocks with values that are not finite.
 __device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }   // not finite: 0x7f800000 on
 struct F8Scale {
     float s, r;

@@ -1,6 +1,7 @@
 // Products of few rows (jobs of up to 16): the weight stream alone counts, each weight byte is used once.  Bound by HBM where
-// there are many jobs (16 tokens: 5.2 TB/s of gate|up weights, 4.5 of down's), by the chain of dependent loads (job, its
-// weights) and the launch where there are few (one token: 8 us, of which the host's call takes 6).
+// there are many jobs (16 tokens: 5.2 TB/s of gate|up weights, 4.2 of down's), by a chain of loads where there are few: the job,
+// then for each of a wavefront's steps x and the first row tile, and after their product the second (gate|up of one token, two
+// steps a wavefront: five round trips, the kernel 8.2 us for 23 MB; down 5.9 for 12; a dense row of 2048 by 1024 5.2).
 #pragma once
 
 #include "mm.hpp"
@@ -122,9 +123,9 @@ __global__ void __launch_bounds__(FEW_THREADS, EL == F8X && !QH ? 6 : 8) k_mm_fe
 }
 
 // WK: as many wavefronts along K as there are steps, for the shortest chain and the most blocks; where each block quantizes the
-// job's rows, half as many, for blocks of twice the rows.  gate|up (2048 columns, 16 steps) with 8, 4, 2 along K: one token 9.2,
-// 9.5, 12.3 us, 16 tokens (133 jobs) 53, 55, 58; down (512 columns, 4 steps) with 4, 2, 1: one token 8.0, 7.7, 8.2, 16 tokens 35,
-// 32, 32; f16 experts of 2048 columns as gate|up (101, 109, 112 us at 16 tokens, 5.4 TB/s of weights).
+// job's rows, half as many, for blocks of twice the rows.  In a graph, the weights in no cache: gate|up (2048 columns, 16 steps)
+// with 8, 4, 2 along K: one token 9.7, 11.3, 16.3 us, 16 tokens (133 jobs) 57, 59, 64; down (512 columns, 4 steps) with 4, 2, 1:
+// one token 7.2, 7.5, 10.2, 16 tokens 37, 34, 36; f16 experts of 2048 columns, 16 tokens, with 8, 4, 2: 108, 116, 123 (5.2 TB/s).
 template <Elem EL, Mode MODE, bool QH> void launch_few(const Args& a, int njobs_cap, hipStream_t s) {
     const int steps = (a.n_in * ESZ<EL> + STEP - 1) / STEP, n_eff = MODE == SWIGLU ? a.n_out / 2 : a.n_out;
     const int per = MODE == SWIGLU ? 16 : 32;

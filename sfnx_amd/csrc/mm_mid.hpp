@@ -1,6 +1,6 @@
 // Dense products of some tens to some hundreds of rows: too many rows for the weights to be all there is, too few tiles of
-// the large kind to fill the chip.  Bound by the latency of their loads: 128 rows of 4096 columns by a matrix of 256 rows 9.4 us
-// (27 streamed), 256 by 1024 11.8 (27).
+// the large kind to fill the chip.  Bound by the latency of their loads: 128 rows of 4096 columns by a matrix of 256 rows 9.7 us
+// (18.9 streamed), 256 by 1024 11.9 (19.3).
 #pragma once
 
 #include "mm_few.hpp"

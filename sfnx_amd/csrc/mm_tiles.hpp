@@ -115,11 +115,15 @@ template <typename Out> __device__ __forceinline__ void swiglu_out(const Args& a
 }
 
 // ------------------------------------------------------------------------------------------------ one job a tile
-// The tiles are one unbroken stream of stages: while one is multiplied the next two are on their way into LDS, across
-// the ends of tiles too, so no tile waits for its first weights.  The descriptions of later jobs come by asynchronous copies
-// as well: a load the compiler waits for would drain the stream.  A wavefront owns 32 of the tile's weight rows for all of
-// the job's rows.  Bound by memory: gate|up of 2048 tokens over 513 experts of 2048 x 1024, 1.07 GB of weights, 247 us, 4.4 TB/s
-// (a copy of that size 4.9, reads into LDS alone 6.0); the matrix cores are 21% busy.
+// The tiles are a stream of stages: while one is multiplied the next two are on their way into LDS, across the ends of tiles
+// too.  The descriptions of later jobs come by asynchronous copies as well.  Two places still drain the stream: enter(), once a
+// tile, where a table's entry is waited for after its branch (whether there is a table or not), and a tile's first wait, which
+// counts the stores of the tile before it among the copies (down of five steps a tile: every fifth step).  A wavefront owns 32
+// of the tile's weight rows for all of the job's rows.  Bound by memory where an expert has some tens of rows: gate|up of 2048
+// tokens over 513 experts of 2048 x 1024, 1.07 GB of weights, 245 us, 4.4 TB/s (a copy of that size 4.9, reads into LDS alone
+// 6.0); the matrix cores are 21% busy.  With hundreds of rows an expert by passing the weights through LDS and their conversion
+// once for each 64 rows, and by converting the activations in every wavefront: 4096 tokens over 65 experts, 120 GFLOP, gate|up
+// 187 us, down into bf16 108, into f32 131, the matrix cores 29% and 14% busy (gate|up, down into bf16).
 template <Elem EL, Mode MODE, int NT> __device__ __forceinline__ void stream_tiles(const Args& a, int nj, const Lds& L) {
     uint8_t* const lds = L.p;
     constexpr int KS = Stream<NT>::KS, D = Stream<NT>::STAGES, N = 128 * NT;
@@ -568,8 +572,10 @@ template <Elem EL> __global__ void __launch_bounds__(TT, 2) k_mm_group(Args a, i
 // 16-bit experts: groups where their rounds of workgroups, each of which takes twice a round of single jobs, are fewer than half
 // of those; which the jobs themselves say.  Streamed and grouped (us; 2048 columns, 1024 rows, bf16, tokens / experts / top k):
 // 600 / 8 / 2 27 and 48; 1024 / 64 / 6 96 and 99; 2048 / 64 / 6 130 and 125; 4096 / 64 / 6 215 and 169; 4096 / 128 / 8 276 and 206.
-// The 8-bit products of experts are streamed: grouped, their steps' scales and conversions keep the matrix cores waiting, and
-// only experts of a thousand rows gain (gate|up of 4096 / 64 / 6 201 and 230, 1024 / 64 / 6 79 and 150).
+// The 8-bit products of experts are streamed: grouped, their steps' scales and conversions keep the matrix cores waiting (gate|up
+// of 1024 / 64 / 6 streamed 79 us, grouped 150, of 4096 / 64 / 6 201 and 230).  Only down into 16 bits, whose sums are the matrix
+// instruction's own, gained from groups at 400 rows an expert (2048 rows, 1024 columns: 4096 / 64 / 6 159 us streamed, 144 grouped;
+// 512 columns 109 and 110).
 template <Elem EL> __global__ void __launch_bounds__(TT, 2) k_mm_experts(Args a, int cap) {
     extern __shared__ __align__(16) uint8_t lds[];
     const Lds L = lds_of(lds);
