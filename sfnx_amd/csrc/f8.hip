@@ -76,8 +76,8 @@ int vec_ok(const void* out, uint32_t out_type, int64_t ldo) {
     return ((uintptr_t) out & (4 * out_size(out_type) - 1)) == 0 && ldo % 4 == 0;
 }
 void check_jobs(const void* jobs, const int* njobs, int cap) {
-    require(jobs != nullptr && njobs != nullptr, "null pointer");
     require(cap >= 0 && cap <= (1 << 20), "njobs out of range");
+    require(cap == 0 || (jobs != nullptr && njobs != nullptr), "null pointer");
 }
 void check_f8_matrix(const void* A, size_t sa, int n_in, int n_out) {
     require(A != nullptr, "null pointer");

@@ -18,7 +18,7 @@ Args mm16_args(const void* A, size_t sa, uint32_t type, int n_in, int n_out, con
     require(stride_ok(sa, 2 * (size_t) n_out * n_in), "expert stride smaller than a matrix");
     require(sa % 16 == 0, "expert stride must be a multiple of 16");
     require(cap >= 0 && cap <= (1 << 20), "njobs out of range");
-    require(A != nullptr && jobs != nullptr && njobs != nullptr && x != nullptr && out != nullptr, "null pointer");
+    require(A != nullptr && (cap == 0 || (jobs != nullptr && njobs != nullptr && x != nullptr && out != nullptr)), "null pointer");
     require((((uintptr_t) A | (uintptr_t) x) & 15) == 0, "pointers must be 16-byte aligned");
     require(((uintptr_t) out & (out_size(out_type) - 1)) == 0, "out must be aligned to its type");
     const int vec = ((uintptr_t) out & (4 * out_size(out_type) - 1)) == 0 && n_out % 4 == 0;

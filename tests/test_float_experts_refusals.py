@@ -109,3 +109,29 @@ def test_rows_and_strides_past_the_library_s_integers():
     with pytest.raises(ValueError, match="A: .* columns"):
         moe.moe_mm_16(torch.empty(4 * far, dtype=F16, **meta), 4 * far, N_IN, far + 8, *jobs, torch.empty((2, N_IN), dtype=F16, **meta),
                       torch.empty((2, far + 8), dtype=F16, **meta))
+
+
+NO_JOBS = [
+    lambda L, *n: L.sfnx_moe_gate_up_swiglu_f8(4096, 1 << 40, 128, 128, *n, None, None, None, None),
+    lambda L, *n: L.sfnx_moe_down_f8(4096, 1 << 40, 128, 128, *n, None, 0, None, None),
+    lambda L, *n: L.sfnx_moe_gate_up_swiglu_f8_big(4096, 1 << 40, 128, 128, *n, None, None, None, None, None),
+    lambda L, *n: L.sfnx_moe_down_f8_big(4096, 1 << 40, 128, 128, *n, None, None, 0, None, None),
+    lambda L, *n: L.sfnx_moe_mm_16(4096, 1 << 40, 1, 128, 128, *n, None, 0, None, None),
+    lambda L, *n: L.sfnx_moe_mm_16_big(4096, 1 << 40, 30, 128, 128, *n, None, 0, None, None)]
+
+
+@pytest.mark.parametrize("call", NO_JOBS)
+def test_room_for_no_jobs(call):
+    """a list with room for no jobs has no address: nothing to do, as in the calls of the quantized experts; with room for one
+    it must have"""
+    L = _abi.lib()
+    # (without a GPU a call that has launched nothing still ends with the runtime's word that there is none)
+    assert call(L, None, None, 0) == 0 or b"no ROCm-capable device" in L.sfnx_last_error()
+    assert call(L, None, None, 1) == -1 and b"null pointer" in L.sfnx_last_error()
+    assert call(L, None, None, -1) == -1 and b"njobs out of range" in L.sfnx_last_error()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("call", NO_JOBS)
+def test_room_for_no_jobs_on_a_gpu(call):
+    assert call(_abi.lib(), None, None, 0) == 0
