@@ -245,3 +245,29 @@ def test_gemm_infinite_weight_scale(where):
         assert torch.isfinite(got[:, ~sick]).all()
         sure = d.abs() > 1e-3 * d.abs().mean()
         assert (got[:, rows].double() == torch.where(d > 0, float("inf"), float("-inf")))[sure].all()
+
+
+@pytest.mark.parametrize("t", ["f32", "bf16"])
+def test_down_window_of_rows_not_finite(t):
+    """h's rows of zeros, of small and large values, with infinities and NaN, quantized in the call: a value that is not finite
+    makes its row's outputs NaN, and no other's"""
+    T, E, K, H, ff = 10, 3, 2, 150, 272
+    g, rng = gen(8), np.random.default_rng(8)
+    blob, W = matrices(g, E + 1, H, ff)
+    P = T * K + T
+    h = torch.randn((P, ff), generator=g)
+    h[0], h[1, ::2], h[2], h[3] = 0, -0.0, h[2] * 1e-20, h[3] * 1e30
+    sick = {4: float("inf"), 9: float("nan"), 15: float("-inf"), 29: float("nan")}
+    for r, v in sick.items():
+        h[r, (37 * r) % ff] = v
+    a, n, flat = jobs(picks(rng, T, E, K), E, True, 16, False)
+    d, out = dev(blob), torch.full((P, H), 77.0, dtype=OUT[t], device="cuda")
+    moe.moe_down_f8(d, d.stride(0), ff, H, *job_tensors(a, n), dev(h), out)
+    bad = torch.zeros(P, dtype=torch.bool)
+    bad[list(sick)] = True
+    got = out.cpu()
+    assert torch.isnan(got[bad]).all() and not torch.isnan(got[~bad]).any()
+    h[bad] = 0
+    want, bound, where = grouped(dequantize(*quantize(h)), W, flat, True)
+    keep = ~bad[where]
+    close(out[where[keep].cuda()], want[keep], bound[keep], OUT[t])
