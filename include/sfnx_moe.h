@@ -233,6 +233,53 @@ int sfnx_moe_mm_16(const void* A, size_t sa, uint32_t type, int n_in, int n_out,
 int sfnx_moe_mm_16_big(const void* A, size_t sa, uint32_t type, int n_in, int n_out, const sfnx_bigjob* jobs,
                        const int* njobs, int njobs_cap, const uint16_t* x, uint32_t out_type, void* out, void* st);
 
+/* ---------------------------------------------------------------------------------------------- sorted rows
+ * No counterpart in the reference, whose experts gather their rows through job lists.  Tokens' rows in the order of their
+ * experts, as rows sent to experts elsewhere, or a product over each expert's consecutive rows, need them, and the way back with
+ * the router's weights, with the gradients of both.
+ *
+ * sfnx_group_rows groups rows 0 .. n - 1 by a number each carries (ids: picks topi [T][K], or a row's adapter); a row whose id
+ * is outside [0, n_groups) belongs to none.  offsets [n_groups + 1]: the rows of the groups before g (the last: of all);
+ * pos [n]: offsets[ids[i]] + the number of earlier rows with its id, -1 for a row without a group; order[pos[i]] = i, entries past
+ * offsets[n_groups] left as they were; jobs: a group's rows 64 a job in order, w the group, y and out the rows' numbers, pos (in_place
+ * 0, for products over sorted rows) or i (in_place 1, for sfnx_adapter_mm), entries past a job's n and jobs past njobs[0] left as they
+ * were; njobs[1] = 0.  pos and order may be null; jobs and njobs together too, else njobs_cap >= n / 64 + min(n, n_groups).
+ * 0 <= n <= 2^20, 1 <= n_groups <= 4096. */
+int sfnx_group_rows(const int* ids, int n, int n_groups, int* offsets, int* pos, int* order, sfnx_bigjob* jobs, int* njobs, int njobs_cap,
+                    int in_place, void* st);
+/* xs[pos[t][k]] = x[t] for rows of H values of elem (1, 2 or 4) bytes, pos [T][K] (of sfnx_group_rows), rows of x and xs ldx and ldxs
+ * values apart.  Here and below an entry of pos outside [0, rows) is left out (rows: of the sorted side), a sorted row that no entry names
+ * is left as it was, and K <= 64, H <= 2^20.  No two entries may be equal. */
+int sfnx_moe_sort_rows(int elem, const void* x, int64_t ldx, int T, int K, int H, const int* pos, void* xs, int64_t ldxs, int rows, void* st);
+/* dx[t] = sum_k dxs[pos[t][k]], summed in 32 bits in k order and rounded once (0 where every entry is left out).  Types SFNX_F32,
+ * SFNX_F16 or SFNX_BF16, each side its own. */
+int sfnx_moe_sort_rows_backward(uint32_t dxs_type, const void* dxs, int64_t lddxs, int rows, const int* pos, int T, int K, int H,
+                                uint32_t dx_type, void* dx, int64_t lddx, void* st);
+/* y[t] = sum_k topw[t][k] ys[pos[t][k]], fmaf in 32 bits in k order, rounded once: sfnx_moe_combine's sum over sorted rows (a shared
+ * expert is one more pick of each token, with its gate's value for a weight) */
+int sfnx_moe_combine_sorted(uint32_t ys_type, const void* ys, int64_t ldys, int rows, const float* topw, const int* pos, int T, int K, int H,
+                            uint32_t y_type, void* y, int64_t ldy, void* st);
+/* its gradient: dys[pos[t][k]] = topw[t][k] dy[t] (ys's type), dw[t][k] = sum_h dy[t][h] ys[pos[t][k]][h] ([T][K] f32, 0 where the entry
+ * is left out), summed in 32 bits.  dys or dw may be null; topw is read for dys, ys for dw only.  dys may be ys. */
+int sfnx_moe_combine_sorted_backward(uint32_t dy_type, const void* dy, int64_t lddy, uint32_t ys_type, const void* ys, int64_t ldys,
+                                     int rows, const float* topw, const int* pos, int T, int K, int H, void* dys, int64_t lddys, float* dw,
+                                     void* st);
+
+/* ---------------------------------------------------------------------------------------------- adapters
+ * Low-rank adapters of many requests beside a projection that all share (no counterpart in the reference):
+ * out[t] = base[t] + scale[a] B_a (A_a x[t]) over jobs of rows (w = a, y = the row of x, out = the row of base and out;
+ * sfnx_group_rows with in_place 1 makes them from each row's adapter).  A: n_adapters matrices [rank][n_in], B: [n_out][rank], f16 or
+ * bf16 (type), sa / sb bytes apart, or with a stride of 0 device tables of their pointers; adapters of a smaller rank are filled up with
+ * zeros.  scale [n_adapters] f32, or null (1).  x: f32 or of the adapters' type, rows ldx values apart.  base and out: f32, f16 or
+ * bf16, rows ldo values apart; base may be out (added in place) or null (zeros).  A job whose w is no adapter adds nothing: its
+ * out rows become base's (group n_adapters serves rows without one; in place they may also be in no job).  Rows of no job are left as
+ * they were, and so are rows outside [0, rows) in a job.  A row may be out of one job only.  A_a x and its product with B_a are summed and
+ * kept in 32 bits, and rounded once, with base, to out's type.
+ * rank % 8 == 0, at most 128; n_in % 8 == 0; n_in and n_out at most 2^20; A, B, x and their rows 16-byte aligned. */
+int sfnx_adapter_mm(const void* A, size_t sa, const void* B, size_t sb, uint32_t type, const float* scale, int n_adapters, int rank, int n_in,
+                    int n_out, const sfnx_bigjob* jobs, const int* njobs, int njobs_cap, uint32_t x_type, const void* x, int64_t ldx,
+                    const void* base, uint32_t out_type, void* out, int64_t ldo, int rows, void* st);
+
 /* ---------------------------------------------------------------------------------------------- fused decode */
 /* one layer's weights: router W [E + 1][H] fp32 (row E gates the shared expert), planar gate|up experts (E + 1 of
  * [2 ff][H], the shared expert last) and planar down experts (E + 1 of [H][ff]) */

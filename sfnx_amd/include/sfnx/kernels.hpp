@@ -252,6 +252,36 @@ inline void moe_mm_16_big(const DW& A, size_t sa, const BigJob* jobs, const int*
     ck(sfnx_moe_mm_16_big(detail::base_of(A), detail::stride_of(A, sa), A.type, A.n_in, A.n_out, jobs, njobs, njobs_cap, x, out_type, out, st));
 }
 
+// ------------------------------------------------------------------------------------------------ sorted rows and adapters
+// No counterpart in the reference (see sfnx_moe.h)
+inline void group_rows(const int* ids, int n, int n_groups, int* offsets, int* pos, int* order, BigJob* jobs, int* njobs, int njobs_cap,
+                       bool in_place, void* st) {
+    ck(sfnx_group_rows(ids, n, n_groups, offsets, pos, order, jobs, njobs, njobs_cap, in_place ? 1 : 0, st));
+}
+inline void moe_sort_rows(int elem, const void* x, int64_t ldx, int T, int K, int H, const int* pos, void* xs, int64_t ldxs, int rows, void* st) {
+    ck(sfnx_moe_sort_rows(elem, x, ldx, T, K, H, pos, xs, ldxs, rows, st));
+}
+inline void moe_sort_rows_backward(uint32_t dxs_type, const void* dxs, int64_t lddxs, int rows, const int* pos, int T, int K, int H,
+                                   uint32_t dx_type, void* dx, int64_t lddx, void* st) {
+    ck(sfnx_moe_sort_rows_backward(dxs_type, dxs, lddxs, rows, pos, T, K, H, dx_type, dx, lddx, st));
+}
+inline void moe_combine_sorted(uint32_t ys_type, const void* ys, int64_t ldys, int rows, const float* topw, const int* pos, int T, int K, int H,
+                               uint32_t y_type, void* y, int64_t ldy, void* st) {
+    ck(sfnx_moe_combine_sorted(ys_type, ys, ldys, rows, topw, pos, T, K, H, y_type, y, ldy, st));
+}
+inline void moe_combine_sorted_backward(uint32_t dy_type, const void* dy, int64_t lddy, uint32_t ys_type, const void* ys, int64_t ldys,
+                                        int rows, const float* topw, const int* pos, int T, int K, int H, void* dys, int64_t lddys, float* dw,
+                                        void* st) {
+    ck(sfnx_moe_combine_sorted_backward(dy_type, dy, lddy, ys_type, ys, ldys, rows, topw, pos, T, K, H, dys, lddys, dw, st));
+}
+// A and B as DWs (n_in, n_out and type of the adapters' matrices; p with a stride, or ep with 0)
+inline void adapter_mm(const DW& A, size_t sa, const DW& B, size_t sb, const float* scale, int n_adapters, const BigJob* jobs, const int* njobs,
+                       int njobs_cap, uint32_t x_type, const void* x, int64_t ldx, const void* base, uint32_t out_type, void* out, int64_t ldo,
+                       int rows, void* st) {
+    ck(sfnx_adapter_mm(detail::base_of(A), detail::stride_of(A, sa), detail::base_of(B), detail::stride_of(B, sb), A.type, scale, n_adapters,
+                       A.n_out, A.n_in, B.n_out, jobs, njobs, njobs_cap, x_type, x, ldx, base, out_type, out, ldo, rows, st));
+}
+
 static_assert(sizeof(Job) == 136 && sizeof(BigJob) == 520, "job layouts match the reference's");
 
 }  // namespace sfnx

@@ -402,6 +402,174 @@ def moe_mm_16_big(A, sa, n_in, n_out, jobs, njobs, njobs_cap, x, out) -> None:
     _mm_16(lib().sfnx_moe_mm_16_big, BIGJOB_INTS, A, sa, n_in, n_out, jobs, njobs, njobs_cap, x, out)
 
 
+# ---------------------------------------------------------------------------------------------------- sorted rows, adapters
+class RowGroups:
+    """What group_rows writes for up to n rows of n_groups groups: offsets [n_groups + 1], pos [n], order [n] (-1 where no call wrote) and
+    the job list jobs, njobs (of at most cap jobs), its rows' numbers pos (for products over sorted rows) or, in place, i (for adapter_mm)"""
+
+    def __init__(self, n: int, n_groups: int, in_place: bool = False, device="cuda"):
+        if n < 0 or n_groups < 1:
+            raise ValueError("n below 0, or no groups")
+        i32 = dict(dtype=torch.int32, device=device)
+        self.n, self.n_groups, self.in_place = n, n_groups, in_place
+        self.cap = n // PF_JOB + min(n, n_groups) + 1
+        self.offsets = torch.zeros(n_groups + 1, **i32)
+        self.pos, self.order = torch.full((n,), -1, **i32), torch.full((n,), -1, **i32)
+        self.jobs, self.njobs = torch.zeros(self.cap * BIGJOB_INTS, **i32), torch.zeros(2, **i32)
+
+
+def group_rows(ids, g: RowGroups) -> None:
+    """rows grouped by their ids (int32, any shape, at most g.n of them; those outside [0, g.n_groups) belong to no group)"""
+    n, dev = ids.numel(), _current()
+    if not _fine(ids, _I32, ids.shape, dev):
+        _need(ids, "ids", _I32)
+    if n > g.n:
+        raise ValueError(f"ids: {n} rows, g has room for {g.n}")
+    if g.offsets.get_device() != dev:
+        raise ValueError("g: not on the current GPU")
+    check(lib().sfnx_group_rows(ids.data_ptr(), n, g.n_groups, g.offsets.data_ptr(), g.pos.data_ptr(), g.order.data_ptr(),
+                                g.jobs.data_ptr(), g.njobs.data_ptr(), g.cap, int(g.in_place), _st()))
+
+
+_ELEM = {torch.uint8: 1, torch.int8: 1, torch.float8_e4m3fn: 1, torch.float16: 2, torch.bfloat16: 2, torch.float32: 4, torch.int32: 4}
+
+
+def _need_matrix(t, name: str, dtypes, cols, dev, rows=None) -> int:
+    """rows of cols (None: any) values, strided or not, none of whose sizes is cut by the library's 32-bit integers; the row stride in
+    values"""
+    if t.dim() != 2:
+        raise ValueError(f"{name}: {t.dim()} dimensions, expected rows of values")
+    n, c = t.shape
+    if not _fine(t, dtypes, (n if rows is None else rows, c if cols is None else cols), dev):
+        _need(t, name, dtypes, (rows, cols), rows_strided=True)
+        if n > 1 and t.stride(0) < c:
+            raise ValueError(f"{name}: rows overlap")
+    if n > _INT_MAX or c > _INT_MAX:
+        _too_large(name, t.shape)
+    return t.stride(0) if n > 1 else max(1, c)
+
+
+def _need_picks(pos, T: int, dev) -> int:
+    """pos [T][K] int32 (or flat, T K of them); K"""
+    K = pos.shape[1] if pos.dim() == 2 else pos.numel() // T if T else 1
+    if not _fine(pos, _I32, pos.shape, dev):
+        _need(pos, "pos", _I32)
+    if pos.numel() != T * K or (pos.dim() == 2 and pos.shape[0] != T):
+        raise ValueError(f"pos: {tuple(pos.shape)}, expected K for each of {T} tokens")
+    return K
+
+
+def moe_sort_rows(x, pos, xs) -> None:
+    """xs[pos[t][k]] = x[t]: the tokens' rows in the order of their experts (pos: group_rows of topi, [T][K] or flat); xs's rows that no pos
+    names are left as they were.  Rows of f32, f16, bf16, 8-bit or int32 values (8-bit rows and their scales are two calls)."""
+    dev = _current()
+    if x.dtype not in _ELEM or xs.dtype is not x.dtype:
+        raise ValueError(f"x: type {x.dtype}, xs {xs.dtype}: expected the same, of 1, 2 or 4 bytes")
+    ldx = _need_matrix(x, "x", (x.dtype,), None, dev)
+    ldxs = _need_matrix(xs, "xs", (x.dtype,), x.shape[1], dev)
+    T, H = x.shape
+    K = _need_picks(pos, T, dev)
+    check(lib().sfnx_moe_sort_rows(_ELEM[x.dtype], x.data_ptr(), ldx, T, K, H, pos.data_ptr(), xs.data_ptr(), ldxs, xs.shape[0], _st()))
+
+
+def moe_sort_rows_backward(dxs, pos, dx) -> None:
+    """dx[t] = sum_k dxs[pos[t][k]], the gradient of moe_sort_rows; each of f32, f16 or bf16"""
+    dev = _current()
+    lddxs = _need_matrix(dxs, "dxs", _TYPE_ID, None, dev)
+    lddx = _need_matrix(dx, "dx", _TYPE_ID, dxs.shape[1], dev)
+    T, H = dx.shape
+    K = _need_picks(pos, T, dev)
+    check(lib().sfnx_moe_sort_rows_backward(_TYPE_ID[dxs.dtype], dxs.data_ptr(), lddxs, dxs.shape[0], pos.data_ptr(), T, K, H,
+                                            _TYPE_ID[dx.dtype], dx.data_ptr(), lddx, _st()))
+
+
+def moe_combine_sorted(ys, topw, pos, y) -> None:
+    """y[t] = sum_k topw[t][k] ys[pos[t][k]]: moe_combine's sum over rows in the order of their experts; ys and y of f32, f16 or bf16"""
+    dev = _current()
+    ldys = _need_matrix(ys, "ys", _TYPE_ID, None, dev)
+    ldy = _need_matrix(y, "y", _TYPE_ID, ys.shape[1], dev)
+    T, H = y.shape
+    K = _need_picks(pos, T, dev)
+    if not _fine(topw, _F32, (T, K), dev):
+        _need(topw, "topw", _F32, (T, K))
+    check(lib().sfnx_moe_combine_sorted(_TYPE_ID[ys.dtype], ys.data_ptr(), ldys, ys.shape[0], topw.data_ptr(), pos.data_ptr(), T, K, H,
+                                        _TYPE_ID[y.dtype], y.data_ptr(), ldy, _st()))
+
+
+def moe_combine_sorted_backward(dy, ys, topw, pos, dys, dw) -> None:
+    """the gradient of moe_combine_sorted: dys[pos[t][k]] = topw[t][k] dy[t] (of ys's type; may be ys) and dw[t][k] = sum_h dy[t][h]
+    ys[pos[t][k]][h] (f32); either may be None.  dys's rows that no pos names are left as they were."""
+    dev = _current()
+    lddy = _need_matrix(dy, "dy", _TYPE_ID, None, dev)
+    ldys = _need_matrix(ys, "ys", _TYPE_ID, dy.shape[1], dev)
+    T, H = dy.shape
+    K = _need_picks(pos, T, dev)
+    if not _fine(topw, _F32, (T, K), dev):
+        _need(topw, "topw", _F32, (T, K))
+    lddys = _need_matrix(dys, "dys", (ys.dtype,), H, dev, ys.shape[0]) if dys is not None else H
+    if dw is not None and not _fine(dw, _F32, (T, K), dev):
+        _need(dw, "dw", _F32, (T, K))
+    check(lib().sfnx_moe_combine_sorted_backward(_TYPE_ID[dy.dtype], dy.data_ptr(), lddy, _TYPE_ID[ys.dtype], ys.data_ptr(), ldys,
+                                                 ys.shape[0], topw.data_ptr(), pos.data_ptr(), T, K, H, _p(dys), lddys, _p(dw), _st()))
+
+
+class Adapters:
+    """Low-rank adapters of one projection, of many requests: A [n][rank][n_in] and B [n][n_out][rank] (f16 or bf16), or lists of n
+    matrices that live apart (then reached through tables of their pointers), and scale [n] f32 (None: 1).  rank is a multiple of 8, at
+    most 128: an adapter of another rank is filled up with zeros."""
+
+    def __init__(self, A, B, scale: torch.Tensor | None = None):
+        self.A, self.B, self.scale = A, B, scale   # held: the tables point into them
+        if len(A) < 1 or len(A) != len(B):
+            raise ValueError("A and B: expected a matrix of each for every adapter")
+        self.n, t = len(A), A[0]
+        if t.dtype not in (torch.float16, torch.bfloat16):
+            raise ValueError(f"A: type {t.dtype}, expected torch.float16 or torch.bfloat16")
+        (self.rank, self.n_in), self.n_out, self.dtype, self.type = t.shape, B[0].shape[0], t.dtype, _TYPE_ID[t.dtype]
+        self.device = t.get_device()
+        self._a, self.sa, self._A = self._place("A", A, (self.rank, self.n_in))
+        self._b, self.sb, self._B = self._place("B", B, (self.n_out, self.rank))
+        if scale is not None:
+            _need(scale, "scale", _F32, (self.n,))
+        self._scale = _p(scale)
+
+    def _place(self, name: str, M, shape):
+        """(address, stride, the table if there is one)"""
+        if isinstance(M, torch.Tensor):
+            _need(M, name, (self.dtype,), (self.n, *shape))
+            return M.data_ptr(), 2 * shape[0] * shape[1], None
+        for m in M:
+            _need(m, name, (self.dtype,), shape)
+            if m.data_ptr() % 16:
+                raise ValueError(f"{name}: a matrix is not 16-byte aligned")
+        table = torch.tensor([m.data_ptr() for m in M], dtype=torch.int64, device=M[0].device)
+        return table.data_ptr(), 0, table
+
+
+def adapter_mm(ad: Adapters, jobs, njobs, njobs_cap: int, x, base, out) -> None:
+    """out[t] = base[t] + scale[a] B_a (A_a x[t]) over jobs of the rows' adapters (group_rows in place over each row's adapter; rows of
+    group ad.n or above have none, and become base's).  x: f32 or the adapters' type; base: out itself (added in place), None (zeros) or
+    of out's type and strides.  Rows of no job are left as they were."""
+    dev = _current()
+    if ad.device != dev:
+        raise ValueError("ad: not on the current GPU")
+    ldx = _need_matrix(x, "x", (torch.float32, ad.dtype), ad.n_in, dev)
+    rows = x.shape[0]
+    ldo = _need_matrix(out, "out", _TYPE_ID, ad.n_out, dev, rows)
+    if base is not None and base is not out:
+        ldb = _need_matrix(base, "base", (out.dtype,), ad.n_out, dev, rows)
+        if ldb != ldo:
+            raise ValueError(f"base: rows {ldb} values apart, out's {ldo}")
+    if not (_fine(jobs, _I32, jobs.shape, dev) and _fine(njobs, _I32, njobs.shape, dev)):
+        _need(jobs, "jobs", _I32)
+        _need(njobs, "njobs", _I32)
+    if njobs_cap < 0 or jobs.numel() < njobs_cap * BIGJOB_INTS or njobs.numel() < 1:
+        raise ValueError("jobs: smaller than the jobs announced, or njobs empty")
+    check(lib().sfnx_adapter_mm(ad._a, ad.sa, ad._b, ad.sb, ad.type, ad._scale, ad.n, ad.rank, ad.n_in, ad.n_out, jobs.data_ptr(),
+                                njobs.data_ptr(), njobs_cap, _TYPE_ID[x.dtype], x.data_ptr(), ldx, _p(base), _TYPE_ID[out.dtype],
+                                out.data_ptr(), ldo, rows, _st()))
+
+
 # ---------------------------------------------------------------------------------------------------- a layer
 @dataclass
 class LayerShape:
