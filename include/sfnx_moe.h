@@ -275,10 +275,13 @@ int sfnx_moe_combine_sorted_backward(uint32_t dy_type, const void* dy, int64_t l
  * out rows become base's (group n_adapters serves rows without one; in place they may also be in no job).  Rows of no job are left as
  * they were, and so are rows outside [0, rows) in a job.  A row may be out of one job only.  A_a x and its product with B_a are summed and
  * kept in 32 bits, and rounded once, with base, to out's type.
- * rank % 8 == 0, at most 128; n_in % 8 == 0; n_in and n_out at most 2^20; A, B, x and their rows 16-byte aligned. */
+ * rank % 8 == 0, at most 128; n_in % 8 == 0; n_in and n_out at most 2^20; A, B, x and their rows 16-byte aligned.
+ * Few rows of small ranks are one launch, others two, which need a workspace of sfnx_adapter_workspace bytes (0: none), 16-byte aligned,
+ * whose contents do not matter; calls that may overlap need one each. */
+size_t sfnx_adapter_workspace(int rows, int rank, int n_in, uint32_t x_type);
 int sfnx_adapter_mm(const void* A, size_t sa, const void* B, size_t sb, uint32_t type, const float* scale, int n_adapters, int rank, int n_in,
                     int n_out, const sfnx_bigjob* jobs, const int* njobs, int njobs_cap, uint32_t x_type, const void* x, int64_t ldx,
-                    const void* base, uint32_t out_type, void* out, int64_t ldo, int rows, void* st);
+                    const void* base, uint32_t out_type, void* out, int64_t ldo, int rows, void* ws, size_t ws_bytes, void* st);
 
 /* ---------------------------------------------------------------------------------------------- fused decode */
 /* one layer's weights: router W [E + 1][H] fp32 (row E gates the shared expert), planar gate|up experts (E + 1 of

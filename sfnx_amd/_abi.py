@@ -70,7 +70,8 @@ SIGNATURES = {
     "sfnx_moe_sort_rows_backward": (i32, [u32, vp, i64, i32, vp, i32, i32, i32, u32, vp, i64, vp]),
     "sfnx_moe_combine_sorted": (i32, [u32, vp, i64, i32, vp, vp, i32, i32, i32, u32, vp, i64, vp]),
     "sfnx_moe_combine_sorted_backward": (i32, [u32, vp, i64, u32, vp, i64, i32, vp, vp, i32, i32, i32, vp, i64, vp, vp]),
-    "sfnx_adapter_mm": (i32, [vp, sz, vp, sz, u32, vp, i32, i32, i32, i32, vp, vp, i32, u32, vp, i64, vp, u32, vp, i64, i32, vp]),
+    "sfnx_adapter_workspace": (sz, [i32, i32, i32, u32]),
+    "sfnx_adapter_mm": (i32, [vp, sz, vp, sz, u32, vp, i32, i32, i32, i32, vp, vp, i32, u32, vp, i64, vp, u32, vp, i64, i32, vp, sz, vp]),
     "sfnx_hc_workspace": (sz, [i32, i32, i32, vp]),
     "sfnx_pf_dense": (i32, [vp, i32, i32, vp, i32, vp, i32, vp, sz, vp]),
     "sfnx_hc_read": (i32, [vp, vp, vp, vp, vp, vp, vp, vp, vp, f32, vp, vp, vp, i32, i32, i32, i32, vp, sz, vp]),

@@ -565,9 +565,12 @@ def adapter_mm(ad: Adapters, jobs, njobs, njobs_cap: int, x, base, out) -> None:
         _need(njobs, "njobs", _I32)
     if njobs_cap < 0 or jobs.numel() < njobs_cap * BIGJOB_INTS or njobs.numel() < 1:
         raise ValueError("jobs: smaller than the jobs announced, or njobs empty")
+    ws, need = None, lib().sfnx_adapter_workspace(rows, ad.rank, ad.n_in, _TYPE_ID[x.dtype])
+    if need:   # of the stream's allocator: freed here, it goes to later work of this stream only
+        ws = torch.empty(need, dtype=torch.uint8, device=x.device)
     check(lib().sfnx_adapter_mm(ad._a, ad.sa, ad._b, ad.sb, ad.type, ad._scale, ad.n, ad.rank, ad.n_in, ad.n_out, jobs.data_ptr(),
                                 njobs.data_ptr(), njobs_cap, _TYPE_ID[x.dtype], x.data_ptr(), ldx, _p(base), _TYPE_ID[out.dtype],
-                                out.data_ptr(), ldo, rows, _st()))
+                                out.data_ptr(), ldo, rows, _p(ws), need, _st()))
 
 
 # ---------------------------------------------------------------------------------------------------- a layer

@@ -111,6 +111,76 @@ def test_rows_that_are_not_finite(T, x_t):
     assert torch.isfinite(out[((ids == 0) & (torch.arange(T) > 1)).cuda()]).all()
 
 
+@pytest.mark.parametrize("t, x_t, out_t", [("bf16", "bf16", "bf16"), ("f16", "f32", "f32"), ("f16", "f16", "f16"), ("bf16", "f32", "f32")])
+@pytest.mark.parametrize("T, n, R, n_in, n_out", [(1025, 4, 8, 264, 145), (1100, 9, 32, 1000, 520), (1500, 2, 24, 2048, 333), (17, 3, 32, 512, 256), (2000, 40, 16, 136, 128)])
+def test_many_rows(T, n, R, n_in, n_out, t, x_t, out_t):
+    test_product(T, n, R, n_in, n_out, t, x_t, out_t)
+
+
+@pytest.mark.parametrize("T, R", [(7, 16), (7, 48), (130, 64), (1100, 16), (90, 128)])
+@pytest.mark.parametrize("t", ["f16", "bf16"])
+def test_matrices_that_are_not_finite(T, R, t):
+    """infinities and NaN in A and B, of adapters of their own: each output is the formula's, the other adapters' are untouched"""
+    n, n_in, n_out, t = 5, 264, 200, TYPES[t]
+    A, B, scale = matrices(n, R, n_in, n_out, t)
+    A[1, R - 1, 3], A[2, 0, 263] = float("-inf"), float("nan")
+    B[3, 7, R - 1], B[3, 199, 0], B[4, 100, 2] = float("inf"), float("-inf"), float("nan")
+    ids = adapter_ids(T, n, T, 0.1)
+    ids[:5] = torch.arange(5)
+    x, base = rand(gen(1), (T, n_in), t), rand(gen(2), (T, n_out), torch.float32)
+    x[3] = 0
+    x[3, 8] = 1.0   # so that most of this row's s has few bits
+    out = base.cuda()
+    call(moe.Adapters(A.cuda(), B.cuda(), scale.cuda()), plan(ids, n), x.cuda(), out, out)
+    want, bound = adapted(x, A, B, scale, ids, base)
+    within(out, want, bound, torch.float32)
+    assert torch.isfinite(out[(ids == 0).cuda()]).all() and torch.isinf(out[3, [7, 199]]).all()
+
+
+def test_past_32_bit_offsets_of_few_rows():
+    """rows 2^22 values apart, 700 of them"""
+    T, n_in, n_out, R, ld = 700, 256, 264, 8, 1 << 22
+    x = torch.zeros(T * ld, dtype=torch.float16, device="cuda").as_strided((T, n_in), (ld, 1))
+    out = torch.zeros(T * ld, dtype=torch.float16, device="cuda").as_strided((T, n_out), (ld, 1))
+    A, B = torch.zeros((2, R, n_in), dtype=torch.float16), torch.zeros((2, n_out, R), dtype=torch.float16)
+    A[1, 3, 255], B[1, :, 3] = 2.0, (torch.arange(n_out) % 100).half()
+    x[T - 1, 255] = 3.0
+    ids = torch.full((T,), -1, dtype=torch.int32)
+    ids[T - 1], ids[5] = 1, 0
+    call(moe.Adapters(A.cuda(), B.cuda()), plan(ids, 2), x, out, out)
+    assert torch.equal(out[T - 1].cpu(), 6 * B[1, :, 3]) and not out[:T - 1].any()
+
+
+def test_two_forms_at_once_and_one_workspace_each():
+    """calls with a workspace on two streams at once, and replayed beside each other"""
+    T, n, R, n_in, n_out = 500, 3, 64, 1024, 512
+    A, B, scale = matrices(n, R, n_in, n_out, torch.bfloat16)
+    ad, ids = moe.Adapters(A.cuda(), B.cuda(), scale.cuda()), adapter_ids(T, n, 1)
+    g = plan(ids, n, True)
+    xs = [rand(gen(k), (T, n_in), torch.bfloat16).cuda() for k in range(2)]
+    base, outs = rand(gen(9), (T, n_out), torch.float32).cuda(), [torch.zeros((T, n_out)).cuda() for _ in range(2)]
+    want = []
+    for x, out in zip(xs, outs):
+        call(ad, g, x, base, out)
+        want.append(out.clone())
+    streams, graphs = [torch.cuda.Stream(), torch.cuda.Stream()], []
+    for x, out in zip(xs, outs):
+        torch.cuda.synchronize()
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            call(ad, g, x, base, out)
+    for k in range(4):
+        for out in outs:
+            out.zero_()
+        torch.cuda.synchronize()
+        for st, gr, x, out in zip(streams, graphs, xs, outs):
+            with torch.cuda.stream(st):
+                for _ in range(3):
+                    gr.replay() if k % 2 else call(ad, g, x, base, out)
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(outs, want))
+
+
 def test_sums_that_only_32_bits_hold():
     """s of two large terms that cancel and a small one, and s itself beside a base of another size: 16 bits anywhere on the way would lose them"""
     n_in, n_out, R = 64, 32, 8

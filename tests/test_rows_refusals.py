@@ -25,8 +25,8 @@ def backward(L, b=1, dy=P, lddy=64, a=1, ys=P, ldys=64, rows=8, w=P, pos=P, T=4,
 
 
 def adapter(L, A=P, sa=BIG, B=P, sb=BIG, t=30, scale=P, n=2, R=16, ni=64, no=64, jobs=P, njobs=P, cap=2, xt=30, x=P, ldx=64, base=P, ot=0, out=P, ldo=64,
-            rows=4):
-    return L.sfnx_adapter_mm(A, sa, B, sb, t, scale, n, R, ni, no, jobs, njobs, cap, xt, x, ldx, base, ot, out, ldo, rows, None)
+            rows=4, ws=None, wb=0):
+    return L.sfnx_adapter_mm(A, sa, B, sb, t, scale, n, R, ni, no, jobs, njobs, cap, xt, x, ldx, base, ot, out, ldo, rows, ws, wb, None)
 
 
 @pytest.mark.parametrize("fn, args, msg", [
@@ -55,6 +55,7 @@ def adapter(L, A=P, sa=BIG, B=P, sb=BIG, t=30, scale=P, n=2, R=16, ni=64, no=64,
     (adapter, dict(A=None), "null pointer"), (adapter, dict(jobs=None), "null pointer"), (adapter, dict(out=None), "null pointer"),
     (adapter, dict(B=P + 8), "16-byte aligned"), (adapter, dict(x=P + 2), "16-byte aligned"), (adapter, dict(ldx=63), "ldx must be"), (adapter, dict(ldx=68), "ldx must be"),
     (adapter, dict(ldo=63), "ldo smaller"), (adapter, dict(out=P + 2), "aligned to their type"), (adapter, dict(base=P + 2), "aligned to their type"),
+    (adapter, dict(R=40), "workspace smaller"), (adapter, dict(R=40, ws=P, wb=1023), "workspace smaller"), (adapter, dict(R=40, ws=P + 4, wb=BIG), "workspace must be"),
     (adapter, dict(scale=P + 2), "4-byte aligned"), (adapter, dict(jobs=P + 2), "4-byte aligned"),
 ])
 def test_library_refuses(fn, args, msg):
