@@ -244,9 +244,11 @@ int sfnx_moe_mm_16_big(const void* A, size_t sa, uint32_t type, int n_in, int n_
  * offsets[n_groups] left as they were; jobs: a group's rows 64 a job in order, w the group, y and out the rows' numbers, pos (in_place
  * 0, for products over sorted rows) or i (in_place 1, for sfnx_adapter_mm), entries past a job's n and jobs past njobs[0] left as they
  * were; njobs[1] = 0.  pos and order may be null; jobs and njobs together too, else njobs_cap >= n / 64 + min(n, n_groups).
- * 0 <= n <= 2^20, 1 <= n_groups <= 4096. */
+ * 0 <= n <= 2^24, 1 <= n_groups <= 4096.  ws: sfnx_group_rows_workspace bytes (0 for few rows; 4-byte aligned, contents do not matter), one for
+ * each of calls that may overlap. */
 int sfnx_group_rows(const int* ids, int n, int n_groups, int* offsets, int* pos, int* order, sfnx_bigjob* jobs, int* njobs, int njobs_cap,
-                    int in_place, void* st);
+                    int in_place, void* ws, size_t ws_bytes, void* st);
+size_t sfnx_group_rows_workspace(int n, int n_groups);
 /* xs[pos[t][k]] = x[t] for rows of H values of elem (1, 2 or 4) bytes, pos [T][K] (of sfnx_group_rows), rows of x and xs ldx and ldxs
  * values apart.  Here and below an entry of pos outside [0, rows) is left out (rows: of the sorted side), a sorted row that no entry names
  * is left as it was, and K <= 64, H <= 2^20.  No two entries may be equal. */

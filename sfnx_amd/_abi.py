@@ -65,7 +65,8 @@ SIGNATURES = {
     "sfnx_moe_down_f8_big": (i32, [vp, sz, i32, i32, vp, vp, i32, vp, vp, u32, vp, vp]),
     "sfnx_moe_mm_16": (i32, [vp, sz, u32, i32, i32, vp, vp, i32, vp, u32, vp, vp]),
     "sfnx_moe_mm_16_big": (i32, [vp, sz, u32, i32, i32, vp, vp, i32, vp, u32, vp, vp]),
-    "sfnx_group_rows": (i32, [vp, i32, i32, vp, vp, vp, vp, vp, i32, i32, vp]),
+    "sfnx_group_rows": (i32, [vp, i32, i32, vp, vp, vp, vp, vp, i32, i32, vp, sz, vp]),
+    "sfnx_group_rows_workspace": (sz, [i32, i32]),
     "sfnx_moe_sort_rows": (i32, [i32, vp, i64, i32, i32, i32, vp, vp, i64, i32, vp]),
     "sfnx_moe_sort_rows_backward": (i32, [u32, vp, i64, i32, vp, i32, i32, i32, u32, vp, i64, vp]),
     "sfnx_moe_combine_sorted": (i32, [u32, vp, i64, i32, vp, vp, i32, i32, i32, u32, vp, i64, vp]),

@@ -635,10 +635,13 @@ void split_columns(int64_t jobs, int n_in, int& parts, int& steps) {
 // Ranks above 32 are two launches: each slice would read 256 KB of A for itself.
 bool two_launches(int rows, int rank, bool x32) { return rank > 32 || rows > 1024 || (x32 && rank > 16 && rows > SFNX_MAXT); }
 
-template <typename K> void launch_lds(K kern, unsigned grid, int threads, int lds, const AdapterArgs& a, hipStream_t st) {
-    if (lds > 64 * 1024)
-        check(hipFuncSetAttribute((const void*) kern, hipFuncAttributeMaxDynamicSharedMemorySize, lds), "hipFuncSetAttribute");
-    kern<<<grid, threads, lds, st>>>(a);
+// more than 64 KB of LDS are asked for once
+template <auto KERN, int LDS> void launch_lds(unsigned grid, int threads, const AdapterArgs& a, hipStream_t st) {
+    if (LDS > 64 * 1024) {
+        static const hipError_t allowed = hipFuncSetAttribute((const void*) KERN, hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
+        check(allowed, "hipFuncSetAttribute");
+    }
+    KERN<<<grid, threads, LDS, st>>>(a);
 }
 
 template <Elem EL, bool X32, int RT> void launch(AdapterArgs a, uint32_t out_type, int cap, hipStream_t st) {
@@ -654,7 +657,7 @@ template <Elem EL, bool X32, int RT> void launch(AdapterArgs a, uint32_t out_typ
             slice(std::max<int64_t>(1, CUS / tiles), AD_UNIT * AW_WAVES);   // one workgroup a compute unit runs at once
             a.units *= AW_WAVES;
             const unsigned grid = grid_of(a.slices * a.subs, cap, AW_THREADS);
-            by_type(out_type, [&](auto ot) { launch_lds(k_adapter_mm<EL, X32, RT, decltype(ot)::value>, grid, AW_THREADS, Few<X32, RT>::LDS, a, st); });
+            by_type(out_type, [&](auto ot) { launch_lds<k_adapter_mm<EL, X32, RT, decltype(ot)::value>, Few<X32, RT>::LDS>(grid, AW_THREADS, a, st); });
         }
         return;
     }
@@ -662,9 +665,9 @@ template <Elem EL, bool X32, int RT> void launch(AdapterArgs a, uint32_t out_typ
     const int64_t jobs = std::min<int64_t>(cap, a.rows / SFNX_PF_JOB + std::min(a.rows, a.n + 1));
     split_columns(jobs, a.n_in, a.parts, a.steps);
     slice(std::max<int64_t>(1, 2 * CUS / jobs), AE_COLS);   // two workgroups a compute unit run at once
-    launch_lds(k_adapter_shrink<EL, X32, RT>, grid_of(a.parts, cap, A2_THREADS), A2_THREADS, Many<X32, RT>::LDS, a, st);
+    launch_lds<k_adapter_shrink<EL, X32, RT>, Many<X32, RT>::LDS>(grid_of(a.parts, cap, A2_THREADS), A2_THREADS, a, st);
     const unsigned grid = grid_of(a.slices, cap, A2_THREADS);
-    by_type(out_type, [&](auto ot) { launch_lds(k_adapter_expand<EL, RT, decltype(ot)::value>, grid, A2_THREADS, Expand<RT>::LDS, a, st); });
+    by_type(out_type, [&](auto ot) { launch_lds<k_adapter_expand<EL, RT, decltype(ot)::value>, Expand<RT>::LDS>(grid, A2_THREADS, a, st); });
 }
 
 }  // namespace

@@ -7,13 +7,31 @@ namespace {
 using namespace mm;
 
 // ------------------------------------------------------------------------------------------------ group_rows
-// A stable counting sort: pos[i] = offsets[g] + the rows of g = ids[i] before i.  A workgroup places 256 rows.  It counts the
-// rows before its own and all others by group in LDS from a read of all of them, which gives every group's offset, its first
-// job (the prefix over groups of ceil(cnt / 64)) and the rank its own rows start from.
-constexpr int GR_THREADS = 256, GR_MAX = 4096;
+// A stable counting sort: pos[i] = offsets[g] + the rows of g = ids[i] before i.  A workgroup places a chunk of rows.  It needs how many rows
+// of each group come before its chunk and how many there are: every group's offset and first job are prefixes over groups of the
+// counts and of ceil(count / 64).  Few rows are one launch, whose workgroups count all rows for themselves; many are two, the first of
+// which counts each chunk into a table.  Within a round of GR_THREADS rows a wavefront's lanes find those before them in the same group by
+// ballots of the ids' bits, and the wavefronts before theirs from a byte each of the group's 16.
+constexpr int GR_THREADS = 1024, GR_WAVES = GR_THREADS / WAVE, GR_MAX = 4096, GR_PER = GR_MAX / GR_THREADS, GR_CHUNKS = 128;
+// Rows up to which one launch is used.  us of the kernels, 512 groups: 4096 rows 6.5 and (two launches) 2.2 + 6.5, 16384 8.0 and 2.4 + 7.1, 40960
+// 10.6 and 2.4 + 8.9 and a launch more; 2^20 rows 5 + 38.
+constexpr int GR_ALONE = 65536;
+
+__global__ void __launch_bounds__(GR_THREADS) k_group_count(const int* __restrict__ ids, int n, int G, int chunk, int* __restrict__ table) {
+    extern __shared__ int hist[];
+    const int c0 = blockIdx.x * chunk, c1 = min(n, c0 + chunk);
+    for (int g = threadIdx.x; g < G; g += GR_THREADS) hist[g] = 0;
+    __syncthreads();
+    for (int i = c0 + (int) threadIdx.x; i < c1; i += GR_THREADS) {
+        const int g = ids[i];
+        if ((unsigned) g < (unsigned) G) atomicAdd(&hist[g], 1);
+    }
+    __syncthreads();
+    for (int g = threadIdx.x; g < G; g += GR_THREADS) table[(size_t) blockIdx.x * G + g] = hist[g];
+}
 
 // exclusive prefix sums of two counts over the workgroup's threads
-__device__ __forceinline__ void block_prefix(int& a, int& b, int (&sums)[2][GR_THREADS / WAVE]) {
+__device__ __forceinline__ void block_prefix(int& a, int& b, int (&sums)[2][GR_WAVES]) {
     const int lane = threadIdx.x % WAVE, wave = threadIdx.x / WAVE, a0 = a, b0 = b;
 #pragma unroll
     for (int o = 1; o < WAVE; o *= 2) {
@@ -23,71 +41,141 @@ __device__ __forceinline__ void block_prefix(int& a, int& b, int (&sums)[2][GR_T
     if (lane == WAVE - 1) sums[0][wave] = a, sums[1][wave] = b;
     __syncthreads();
 #pragma unroll
-    for (int w = 0; w < GR_THREADS / WAVE; ++w)
-        if (w < wave) a += sums[0][w], b += sums[1][w];
+    for (int w = 0; w < GR_WAVES - 1; ++w) {
+        a += w < wave ? sums[0][w] : 0;
+        b += w < wave ? sums[1][w] : 0;
+    }
     a -= a0, b -= b0;
 }
 
-__global__ void __launch_bounds__(GR_THREADS) k_group_rows(const int* __restrict__ ids, int n, int G, int* __restrict__ offsets,
-                                                          int* __restrict__ pos, int* __restrict__ order, sfnx_bigjob* __restrict__ jobs,
-                                                          int* __restrict__ njobs, int in_place) {
-    extern __shared__ int sh[];
-    int *before = sh, *total = sh + G, *first = sh + 2 * G;   // first: a group's first job
-    __shared__ int mine[GR_THREADS], sums[2][GR_THREADS / WAVE], all;   // all: rows that have a group
-    const int tid = threadIdx.x, c0 = blockIdx.x * GR_THREADS, i = c0 + tid;
-    for (int g = tid; g < G; g += GR_THREADS) before[g] = total[g] = 0;
-    __syncthreads();
-    for (int j = tid; j < n; j += GR_THREADS) {
-        const int g = ids[j];
-        if ((unsigned) g < (unsigned) G) atomicAdd(j < c0 ? &before[g] : &total[g], 1);
+// table: the chunks' counts, or null
+__global__ void __launch_bounds__(GR_THREADS) k_group_rows(const int* __restrict__ ids, int n, int G, int chunk, const int* __restrict__ table,
+                                                          int* __restrict__ offsets, int* __restrict__ pos, int* __restrict__ order,
+                                                          sfnx_bigjob* __restrict__ jobs, int* __restrict__ njobs, int in_place) {
+    extern __shared__ __align__(16) int sh[];
+    uint4* const of_wave = reinterpret_cast<uint4*>(sh);                     // a group's rows of this round, a byte a wavefront
+    int *run = sh + 4 * G, *off = sh + 5 * G, *first = sh + 6 * G;           // its rows so far, offset and first job
+    __shared__ int sums[2][GR_WAVES], all;                // all: rows that have a group
+    const int tid = threadIdx.x, lane = tid % WAVE, wave = tid / WAVE, c0 = blockIdx.x * chunk, c1 = min(n, c0 + chunk);
+    const int per = (G + GR_THREADS - 1) / GR_THREADS, g0 = tid * per;   // this thread's groups
+    int before[GR_PER] = {}, total[GR_PER] = {};
+    if (table) {
+        constexpr int AT = 16;   // chunks requested at once
+        const int nb = gridDim.x, mine = blockIdx.x;
+#pragma unroll
+        for (int k = 0; k < GR_PER; ++k)
+            if (k < per && g0 + k < G)
+                for (int b0 = 0; b0 < nb; b0 += AT) {
+                    int c[AT];
+#pragma unroll
+                    for (int e = 0; e < AT; ++e) c[e] = b0 + e < nb ? table[(size_t) (b0 + e) * G + g0 + k] : 0;
+#pragma unroll
+                    for (int e = 0; e < AT; ++e) {
+                        total[k] += c[e];
+                        before[k] += b0 + e < mine ? c[e] : 0;
+                    }
+                }
+    } else {
+        for (int g = tid; g < G; g += GR_THREADS) run[g] = off[g] = 0;
+        __syncthreads();
+        for (int i0 = tid; i0 < n; i0 += 8 * GR_THREADS) {
+            int g[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) g[e] = i0 + e * GR_THREADS < n ? ids[i0 + e * GR_THREADS] : -1;
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if ((unsigned) g[e] < (unsigned) G) atomicAdd(i0 + e * GR_THREADS < c0 ? &run[g[e]] : &off[g[e]], 1);
+        }
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < GR_PER; ++k)
+            if (k < per && g0 + k < G) {
+                before[k] = run[g0 + k];
+                total[k] = before[k] + off[g0 + k];
+            }
+        __syncthreads();
     }
-    const int g = i < n ? ids[i] : -1;
-    const bool in = (unsigned) g < (unsigned) G;
-    mine[tid] = in ? g : -1;
-    __syncthreads();
-    int rank = 0;
-    for (int j = 0; j < tid; ++j) rank += mine[j] == g;
-    // the prefix over groups, PER consecutive ones a thread
-    const int per = (G + GR_THREADS - 1) / GR_THREADS;
     int rows = 0, nj = 0;
-    for (int k = 0, h = tid * per; k < per && h < G; ++k, ++h) {
-        const int c = before[h] + total[h];
-        rows += c, nj += (c + SFNX_PF_JOB - 1) / SFNX_PF_JOB;
-    }
+#pragma unroll
+    for (int k = 0; k < GR_PER; ++k) rows += total[k], nj += (total[k] + SFNX_PF_JOB - 1) / SFNX_PF_JOB;
     block_prefix(rows, nj, sums);
-    for (int k = 0, h = tid * per; k < per && h < G; ++k, ++h) {
-        const int c = before[h] + total[h];
-        if (blockIdx.x == 0) offsets[h] = rows;
-        first[h] = nj;
-        total[h] = rows;   // its offset from here on
-        rows += c, nj += (c + SFNX_PF_JOB - 1) / SFNX_PF_JOB;
-        if (h == G - 1) {
-            all = rows;
-            if (blockIdx.x == 0) {
-                offsets[G] = rows;
-                if (njobs) njobs[0] = nj, njobs[1] = 0;
+#pragma unroll
+    for (int k = 0; k < GR_PER; ++k)
+        if (k < per && g0 + k < G) {
+            const int g = g0 + k;
+            if (blockIdx.x == 0) offsets[g] = rows;
+            run[g] = before[k];
+            of_wave[g] = uint4{0, 0, 0, 0};
+            off[g] = rows;
+            first[g] = nj;
+            rows += total[k], nj += (total[k] + SFNX_PF_JOB - 1) / SFNX_PF_JOB;
+            if (g == G - 1) {
+                all = rows;
+                if (blockIdx.x == 0) {
+                    offsets[G] = rows;
+                    if (njobs) njobs[0] = nj, njobs[1] = 0;
+                }
+            }
+        }
+    __syncthreads();
+    const int bits = 32 - __clz(G - 1);   // of an id (G = 1: __clz(0) is 32)
+    const auto bytes = [](const uint4& v) {
+        unsigned n = 0;
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) n = __builtin_amdgcn_udot4(w[e], 0x01010101u, n, false);
+        return (int) n;
+    };
+    int next = c0 + tid < c1 ? ids[c0 + tid] : -1;
+    for (int i0 = c0; i0 < c1; i0 += GR_THREADS) {
+        const int i = i0 + tid, g = next;
+        const bool in = (unsigned) g < (unsigned) G, more = i0 + GR_THREADS < c1;
+        if (more) next = i + GR_THREADS < c1 ? ids[i + GR_THREADS] : -1;
+        uint64_t same = __ballot(in);
+        for (int b = 0; b < bits; ++b) {
+            const uint64_t m = __ballot(g >> b & 1);
+            same &= g >> b & 1 ? m : ~m;
+        }
+        const int mine = __popcll(same & ((1ull << lane) - 1));   // of the same group, before this lane
+        if (in && mine == 0) reinterpret_cast<uint8_t*>(of_wave + g)[wave] = (uint8_t) __popcll(same);
+        lds_barrier();
+        int r = 0;
+        if (in) {
+            uint4 v = of_wave[g];   // of the wavefronts before this one
+            const uint64_t lo = wave >= 8 ? ~0ull : (1ull << 8 * wave) - 1, hi = wave > 8 ? (1ull << 8 * (wave - 8)) - 1 : 0;
+            v.x &= (uint32_t) lo, v.y &= (uint32_t) (lo >> 32), v.z &= (uint32_t) hi, v.w &= (uint32_t) (hi >> 32);
+            r = run[g] + bytes(v) + mine;
+        }
+        if (more) {   // the round's rows join those before the next
+            lds_barrier();
+            for (int k = 0; k < per && g0 + k < G; ++k) {
+                run[g0 + k] += bytes(of_wave[g0 + k]);
+                of_wave[g0 + k] = uint4{0, 0, 0, 0};
+            }
+            lds_barrier();
+        }
+        if (i >= c1) continue;
+        if (!in) {
+            if (pos) pos[i] = -1;
+            continue;
+        }
+        const int p = off[g] + r;
+        if (pos) pos[i] = p;
+        if (order) order[p] = i;
+        if (jobs) {
+            sfnx_bigjob& j = jobs[first[g] + r / SFNX_PF_JOB];
+            const int s = r % SFNX_PF_JOB, v = in_place ? i : p;
+            j.y[s] = j.out[s] = v;
+            if (s == 0) {
+                j.w = g;
+                j.n = min(SFNX_PF_JOB, (g + 1 < G ? off[g + 1] : all) - p);
             }
         }
     }
-    __syncthreads();
-    if (i >= n) return;
-    if (!in) {
-        if (pos) pos[i] = -1;
-        return;
-    }
-    const int r = before[g] + rank, p = total[g] + r;
-    if (pos) pos[i] = p;
-    if (order) order[p] = i;
-    if (jobs) {
-        sfnx_bigjob& j = jobs[first[g] + r / SFNX_PF_JOB];
-        const int s = r % SFNX_PF_JOB, v = in_place ? i : p;
-        j.y[s] = j.out[s] = v;
-        if (s == 0) {
-            j.w = g;
-            j.n = min(SFNX_PF_JOB, (g + 1 < G ? total[g + 1] : all) - p);
-        }
-    }
 }
+
+// rows of a chunk, a multiple of GR_THREADS
+int group_chunk(int n) { return (n + GR_THREADS * GR_CHUNKS - 1) / (GR_THREADS * GR_CHUNKS) * GR_THREADS; }
 
 // ------------------------------------------------------------------------------------------------ rows of 16- and 32-bit values
 // E consecutive values of a row
@@ -117,11 +205,12 @@ template <int TYPE, int E> __device__ __forceinline__ void store_pack(void* p, i
 constexpr int RW_THREADS = 256, RW_GROUP = 8;   // rows requested before the first is used
 
 // ------------------------------------------------------------------------------------------------ sort_rows
-// xs[pos[t][k]] = x[t]: a token's row is read once and written K times.  PIECE: the bytes a thread moves.
+// xs[pos[t][k]] = x[t]: a token's row is read once and written K times.  PIECE: the bytes a thread moves.  Bound by its writes: 2048 tokens, 10 picks,
+// 2048 bf16 columns, 92 MB, 18.7 us (4.9 TB/s).
 template <typename PIECE>
 __global__ void __launch_bounds__(RW_THREADS) k_sort_rows(const uint8_t* __restrict__ x, int64_t ldx, int K, int pieces, int blocks,
                                                          const int* __restrict__ pos, uint8_t* __restrict__ xs, int64_t ldxs, int rows) {
-    const int t = blockIdx.x / blocks, c = (blockIdx.x % blocks) * RW_THREADS + threadIdx.x;
+    const int t = blockIdx.x / blocks, c = (blockIdx.x % blocks) * blockDim.x + threadIdx.x;
     if (c >= pieces) return;
     const PIECE v = *(reinterpret_cast<const PIECE*>(x + (int64_t) t * ldx) + c);
     for (int k = 0; k < K; ++k) {
@@ -132,12 +221,12 @@ __global__ void __launch_bounds__(RW_THREADS) k_sort_rows(const uint8_t* __restr
 
 // ------------------------------------------------------------------------------------------------ combine
 // y[t] = sum_k w[t][k] ys[pos[t][k]] in k order, fmaf in 32 bits, one rounding to y's type; w null: 1 (the gradient of
-// sort_rows).
+// sort_rows).  Bound by its reads: 4096 tokens, 10 picks, 2048 bf16 columns, 185 MB, 40.6 us (4.6 TB/s; 12 rows requested at once 44.5).
 template <int YS, int Y, int E>
 __global__ void __launch_bounds__(RW_THREADS) k_combine_sorted(const void* __restrict__ ys, int64_t ldys, int rows, const float* __restrict__ w,
                                                               const int* __restrict__ pos, int K, int H, int blocks, void* __restrict__ y,
                                                               int64_t ldy) {
-    const int t = blockIdx.x / blocks, c = ((blockIdx.x % blocks) * RW_THREADS + threadIdx.x) * E;
+    const int t = blockIdx.x / blocks, c = ((blockIdx.x % blocks) * blockDim.x + threadIdx.x) * E;
     if (c >= H) return;
     float s[E] = {};
     for (int k0 = 0; k0 < K; k0 += RW_GROUP) {
@@ -160,57 +249,51 @@ __global__ void __launch_bounds__(RW_THREADS) k_combine_sorted(const void* __res
     store_pack<Y, E>(y, t * ldy + c, s);
 }
 
-// dys[pos[t][k]] = w[t][k] dy[t], dw[t][k] = sum_h dy[t][h] ys[pos[t][k]][h]: a workgroup takes RW_GROUP picks of a token.  A
-// thread's products of a row are summed in 32 bits in column order, then the threads by a tree.
+// dys[pos[t][k]] = w[t][k] dy[t], dw[t][k] = sum_h dy[t][h] ys[pos[t][k]][h]: a workgroup a token, a wavefront a pick (the 17th on go to
+// the first again), so that dy's row is in the L1 for all but the first and a pick's sum stays in its wavefront: a lane's products in column
+// order by fmaf, then the lanes by a tree.  Bound by memory: 4096 tokens, 6 picks, 2048 bf16 columns, 218 MB, 48.7 us (4.5 TB/s; 42 at a large copy's
+// rate); 10 picks of 1024 columns 42 us, where four pieces at once leave room for fewer wavefronts: 56.  With all of a token's
+// picks in one thread's registers and their sums joined in LDS 52 and 84.
+constexpr int CB_WAVES = 16, CB_AT = 2;   // pieces of a row requested at once
 template <int YS, int DY, int E>
-__global__ void __launch_bounds__(RW_THREADS) k_combine_sorted_backward(const void* __restrict__ dy, int64_t lddy, const void* __restrict__ ys,
-                                                                       int64_t ldys, int rows, const float* __restrict__ w,
-                                                                       const int* __restrict__ pos, int K, int H, int groups,
-                                                                       void* __restrict__ dys, int64_t lddys, float* __restrict__ dw) {
-    const int t = blockIdx.x / groups, k0 = (blockIdx.x % groups) * RW_GROUP;
-    __shared__ float part[RW_THREADS / WAVE][RW_GROUP];
-    int p[RW_GROUP];
-    float wk[RW_GROUP], s[RW_GROUP] = {};
+__global__ void __launch_bounds__(CB_WAVES * WAVE) k_combine_sorted_backward(const void* __restrict__ dy, int64_t lddy, const void* ys, int64_t ldys,
+                                                                            int rows, const float* __restrict__ w, const int* __restrict__ pos,
+                                                                            int K, int H, void* dys, int64_t lddys, float* __restrict__ dw) {
+    const int t = blockIdx.x, lane = threadIdx.x % WAVE, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE), nw = blockDim.x / WAVE;
+    for (int k = wave; k < K; k += nw) {
+        const int64_t at = (int64_t) t * K + k;
+        const int p = pos[at];
+        float s = 0.f;
+        if ((unsigned) p < (unsigned) rows) {
+            const float wk = dys ? w[at] : 0.f;
+            for (int c0 = lane * E; c0 < H; c0 += CB_AT * WAVE * E) {
+                Pack<DY, E> d[CB_AT];
+                Pack<YS, E> v[CB_AT];
 #pragma unroll
-    for (int k = 0; k < RW_GROUP; ++k) {
-        p[k] = k0 + k < K ? pos[(int64_t) t * K + k0 + k] : -1;
-        if ((unsigned) p[k] >= (unsigned) rows) p[k] = -1;
-        wk[k] = dys && p[k] >= 0 ? w[(int64_t) t * K + k0 + k] : 0.f;
-    }
-    for (int c = threadIdx.x * E; c < H; c += RW_THREADS * E) {
-        const Pack<DY, E> d = pack_at<DY, E>(dy, t * lddy + c);
-        Pack<YS, E> v[RW_GROUP];
-        if (dw) {
-#pragma unroll
-            for (int k = 0; k < RW_GROUP; ++k)
-                if (p[k] >= 0) v[k] = pack_at<YS, E>(ys, p[k] * ldys + c);
-        }
-#pragma unroll
-        for (int k = 0; k < RW_GROUP; ++k)
-            if (p[k] >= 0) {
-                float o[E];
-#pragma unroll
-                for (int e = 0; e < E; ++e) {
-                    const float g = to_float<DY>(d.v[e]);
-                    o[e] = wk[k] * g;
-                    if (dw) s[k] = fmaf(g, to_float<YS>(v[k].v[e]), s[k]);
+                for (int u = 0; u < CB_AT; ++u) {
+                    const int c = c0 + u * WAVE * E;
+                    if (c < H) {
+                        d[u] = pack_at<DY, E>(dy, t * lddy + c);
+                        if (dw) v[u] = pack_at<YS, E>(ys, p * ldys + c);
+                    }
                 }
-                if (dys) store_pack<YS, E>(dys, p[k] * lddys + c, o);
+#pragma unroll
+                for (int u = 0; u < CB_AT; ++u) {
+                    const int c = c0 + u * WAVE * E;
+                    if (c >= H) continue;
+                    float o[E];
+#pragma unroll
+                    for (int e = 0; e < E; ++e) {
+                        const float g = to_float<DY>(d[u].v[e]);
+                        o[e] = wk * g;
+                        if (dw) s = fmaf(g, to_float<YS>(v[u].v[e]), s);
+                    }
+                    if (dys) store_pack<YS, E>(dys, p * lddys + c, o);
+                }
             }
-    }
-    if (!dw) return;
-    const int lane = threadIdx.x % WAVE, wave = threadIdx.x / WAVE;
-#pragma unroll
-    for (int k = 0; k < RW_GROUP; ++k) {
-        const float v = group_sum<WAVE>(s[k]);
-        if (lane == 0) part[wave][k] = v;
-    }
-    __syncthreads();
-    if (threadIdx.x < RW_GROUP && k0 + (int) threadIdx.x < K) {
-        float v = 0.f;
-#pragma unroll
-        for (int q = 0; q < RW_THREADS / WAVE; ++q) v += part[q][threadIdx.x];
-        dw[(int64_t) t * K + k0 + threadIdx.x] = v;
+            s = group_sum<WAVE>(s);
+        }
+        if (dw && lane == 0) dw[at] = s;
     }
 }
 
@@ -231,9 +314,17 @@ void check_rows(const void* p, int64_t ld, int H, int size, bool used) {
 }
 void check_type(uint32_t type) { require(out_type_ok(type), "type must be F32 (0), F16 (1) or BF16 (30)"); }
 bool wide(const void* p, int64_t ld, int size, int bytes) { return ((uintptr_t) p & (bytes - 1)) == 0 && ld * size % bytes == 0; }
-unsigned grid_rows(int T, int blocks) {
-    require((int64_t) T * blocks * RW_THREADS < ((int64_t) 1 << 32), "too many rows for one launch");
-    return (unsigned) (T * blocks);
+unsigned grid_rows(int T, int blocks, int threads) {
+    require((int64_t) T * blocks * threads < ((int64_t) 1 << 32), "too many rows for one launch");
+    return (unsigned) T * (unsigned) blocks;
+}
+// a row's pieces over workgroups of at most RW_THREADS, about the same for each
+struct RowSplit {
+    int blocks, threads;
+};
+RowSplit row_split(int pieces) {
+    const int blocks = (pieces + RW_THREADS - 1) / RW_THREADS, each = (pieces + blocks - 1) / blocks;
+    return RowSplit{blocks, (each + WAVE - 1) / WAVE * WAVE};
 }
 
 template <typename F> void by_type(uint32_t type, F&& f) {
@@ -257,11 +348,11 @@ void combine_sorted(uint32_t ys_type, const void* ys, int64_t ldys, int rows, co
             constexpr int YS = decltype(a)::value, Y = decltype(b)::value, E = wide_of(YS);
             const int yb = E * out_size(Y) < 16 ? E * out_size(Y) : 16;
             if (H % E == 0 && wide(ys, ldys, out_size(YS), 16) && wide(y, ldy, out_size(Y), yb)) {
-                const int blocks = (H / E + RW_THREADS - 1) / RW_THREADS;
-                k_combine_sorted<YS, Y, E><<<grid_rows(T, blocks), RW_THREADS, 0, st>>>(ys, ldys, rows, w, pos, K, H, blocks, y, ldy);
+                const RowSplit r = row_split(H / E);
+                k_combine_sorted<YS, Y, E><<<grid_rows(T, r.blocks, r.threads), r.threads, 0, st>>>(ys, ldys, rows, w, pos, K, H, r.blocks, y, ldy);
             } else {
-                const int blocks = (H + RW_THREADS - 1) / RW_THREADS;
-                k_combine_sorted<YS, Y, 1><<<grid_rows(T, blocks), RW_THREADS, 0, st>>>(ys, ldys, rows, w, pos, K, H, blocks, y, ldy);
+                const RowSplit r = row_split(H);
+                k_combine_sorted<YS, Y, 1><<<grid_rows(T, r.blocks, r.threads), r.threads, 0, st>>>(ys, ldys, rows, w, pos, K, H, r.blocks, y, ldy);
             }
         });
     });
@@ -272,19 +363,31 @@ void combine_sorted(uint32_t ys_type, const void* ys, int64_t ldys, int rows, co
 
 using namespace sfnx;
 
+extern "C" size_t sfnx_group_rows_workspace(int n, int n_groups) {
+    if (n <= GR_ALONE || n_groups <= 0) return 0;
+    const int chunk = group_chunk(n);
+    return (size_t) ((n + chunk - 1) / chunk) * n_groups * sizeof(int);
+}
+
 extern "C" int sfnx_group_rows(const int* ids, int n, int n_groups, int* offsets, int* pos, int* order, sfnx_bigjob* jobs, int* njobs,
-                               int njobs_cap, int in_place, void* st) {
+                               int njobs_cap, int in_place, void* ws, size_t ws_bytes, void* st) {
     return guarded("sfnx_group_rows", [&] {
-        require(n >= 0 && n <= (1 << 20), "n out of range (0..2^20)");
+        require(n >= 0 && n <= (1 << 24), "n out of range (0..2^24)");
         require(n_groups >= 1 && n_groups <= GR_MAX, "n_groups out of range (1..4096)");
         require((n == 0 || ids != nullptr) && offsets != nullptr, "null pointer");
         require((jobs == nullptr) == (njobs == nullptr), "jobs and njobs go together");
-        require((((uintptr_t) ids | (uintptr_t) offsets | (uintptr_t) pos | (uintptr_t) order | (uintptr_t) jobs | (uintptr_t) njobs) & 3) == 0,
+        require((((uintptr_t) ids | (uintptr_t) offsets | (uintptr_t) pos | (uintptr_t) order | (uintptr_t) jobs | (uintptr_t) njobs | (uintptr_t) ws) & 3) == 0,
                 "pointers must be 4-byte aligned");
         require(jobs == nullptr || njobs_cap >= n / SFNX_PF_JOB + std::min(n, n_groups), "njobs_cap smaller than n / 64 + min(n, n_groups)");
-        const int blocks = std::max(1, (n + GR_THREADS - 1) / GR_THREADS);
-        k_group_rows<<<blocks, GR_THREADS, 3 * n_groups * sizeof(int), stream_of(st)>>>(ids, n, n_groups, offsets, pos, order, jobs, njobs,
-                                                                                       in_place);
+        const size_t need = sfnx_group_rows_workspace(n, n_groups);
+        require(need == 0 || (ws != nullptr && ws_bytes >= need), "workspace smaller than sfnx_group_rows_workspace");
+        const int chunk = need ? group_chunk(n) : GR_THREADS, blocks = std::max(1, (n + chunk - 1) / chunk);
+        int* const table = need ? (int*) ws : nullptr;
+        if (table) k_group_count<<<blocks, GR_THREADS, n_groups * sizeof(int), stream_of(st)>>>(ids, n, n_groups, chunk, table);
+        static const hipError_t allowed = hipFuncSetAttribute((const void*) k_group_rows, hipFuncAttributeMaxDynamicSharedMemorySize, 28 * GR_MAX);
+        check(allowed, "hipFuncSetAttribute");
+        k_group_rows<<<blocks, GR_THREADS, 28 * (size_t) n_groups, stream_of(st)>>>(ids, n, n_groups, chunk, table, offsets, pos, order, jobs,
+                                                                                       njobs, in_place);
     });
 }
 
@@ -298,9 +401,10 @@ extern "C" int sfnx_moe_sort_rows(int elem, const void* x, int64_t ldx, int T, i
         if (T == 0) return;
         const auto go = [&](auto piece) {
             typedef decltype(piece) P;
-            const int pieces = (int) ((int64_t) H * elem / sizeof(P)), blocks = (pieces + RW_THREADS - 1) / RW_THREADS;
-            k_sort_rows<P><<<grid_rows(T, blocks), RW_THREADS, 0, stream_of(st)>>>((const uint8_t*) x, ldx * elem, K, pieces, blocks, pos,
-                                                                                  (uint8_t*) xs, ldxs * elem, rows);
+            const int pieces = (int) ((int64_t) H * elem / sizeof(P));
+            const RowSplit r = row_split(pieces);
+            k_sort_rows<P><<<grid_rows(T, r.blocks, r.threads), r.threads, 0, stream_of(st)>>>((const uint8_t*) x, ldx * elem, K, pieces, r.blocks, pos,
+                                                                                             (uint8_t*) xs, ldxs * elem, rows);
         };
         if (H * elem % 16 == 0 && wide(x, ldx, elem, 16) && wide(xs, ldxs, elem, 16)) go(uint4{});
         else if (elem == 4) go(uint32_t{});
@@ -337,17 +441,15 @@ extern "C" int sfnx_moe_combine_sorted_backward(uint32_t dy_type, const void* dy
         require(T <= 0 || topw != nullptr || dys == nullptr, "null pointer");
         require((((uintptr_t) topw | (uintptr_t) dw) & 3) == 0, "weights must be 4-byte aligned");
         if (T == 0 || (dys == nullptr && dw == nullptr)) return;
+        const unsigned grid = grid_rows(T, 1, CB_WAVES * WAVE);
         by_type(ys_type, [&](auto a) {
             by_type(dy_type, [&](auto b) {
                 constexpr int YS = decltype(a)::value, DY = decltype(b)::value, E = wide_of(YS);
-                const int db = E * out_size(DY) < 16 ? E * out_size(DY) : 16, groups = (K + RW_GROUP - 1) / RW_GROUP;
-                const unsigned grid = grid_rows(T, groups);
+                const int db = E * out_size(DY) < 16 ? E * out_size(DY) : 16, threads = std::min(K, CB_WAVES) * WAVE;
                 if (H % E == 0 && wide(ys, ldys, out_size(YS), 16) && (!dys || wide(dys, lddys, out_size(YS), 16)) && wide(dy, lddy, out_size(DY), db))
-                    k_combine_sorted_backward<YS, DY, E><<<grid, RW_THREADS, 0, stream_of(st)>>>(dy, lddy, ys, ldys, rows, topw, pos, K, H,
-                                                                                               groups, dys, lddys, dw);
+                    k_combine_sorted_backward<YS, DY, E><<<grid, threads, 0, stream_of(st)>>>(dy, lddy, ys, ldys, rows, topw, pos, K, H, dys, lddys, dw);
                 else
-                    k_combine_sorted_backward<YS, DY, 1><<<grid, RW_THREADS, 0, stream_of(st)>>>(dy, lddy, ys, ldys, rows, topw, pos, K, H,
-                                                                                               groups, dys, lddys, dw);
+                    k_combine_sorted_backward<YS, DY, 1><<<grid, threads, 0, stream_of(st)>>>(dy, lddy, ys, ldys, rows, topw, pos, K, H, dys, lddys, dw);
             });
         });
     });

@@ -255,8 +255,8 @@ inline void moe_mm_16_big(const DW& A, size_t sa, const BigJob* jobs, const int*
 // ------------------------------------------------------------------------------------------------ sorted rows and adapters
 // No counterpart in the reference (see sfnx_moe.h)
 inline void group_rows(const int* ids, int n, int n_groups, int* offsets, int* pos, int* order, BigJob* jobs, int* njobs, int njobs_cap,
-                       bool in_place, void* st) {
-    ck(sfnx_group_rows(ids, n, n_groups, offsets, pos, order, jobs, njobs, njobs_cap, in_place ? 1 : 0, st));
+                       bool in_place, void* ws, size_t ws_bytes, void* st) {
+    ck(sfnx_group_rows(ids, n, n_groups, offsets, pos, order, jobs, njobs, njobs_cap, in_place ? 1 : 0, ws, ws_bytes, st));
 }
 inline void moe_sort_rows(int elem, const void* x, int64_t ldx, int T, int K, int H, const int* pos, void* xs, int64_t ldxs, int rows, void* st) {
     ck(sfnx_moe_sort_rows(elem, x, ldx, T, K, H, pos, xs, ldxs, rows, st));

@@ -416,6 +416,7 @@ class RowGroups:
         self.offsets = torch.zeros(n_groups + 1, **i32)
         self.pos, self.order = torch.full((n,), -1, **i32), torch.full((n,), -1, **i32)
         self.jobs, self.njobs = torch.zeros(self.cap * BIGJOB_INTS, **i32), torch.zeros(2, **i32)
+        self.ws = torch.empty(lib().sfnx_group_rows_workspace(n, n_groups), dtype=torch.uint8, device=device)
 
 
 def group_rows(ids, g: RowGroups) -> None:
@@ -428,7 +429,7 @@ def group_rows(ids, g: RowGroups) -> None:
     if g.offsets.get_device() != dev:
         raise ValueError("g: not on the current GPU")
     check(lib().sfnx_group_rows(ids.data_ptr(), n, g.n_groups, g.offsets.data_ptr(), g.pos.data_ptr(), g.order.data_ptr(),
-                                g.jobs.data_ptr(), g.njobs.data_ptr(), g.cap, int(g.in_place), _st()))
+                                g.jobs.data_ptr(), g.njobs.data_ptr(), g.cap, int(g.in_place), g.ws.data_ptr(), g.ws.numel(), _st()))
 
 
 _ELEM = {torch.uint8: 1, torch.int8: 1, torch.float8_e4m3fn: 1, torch.float16: 2, torch.bfloat16: 2, torch.float32: 4, torch.int32: 4}
@@ -459,58 +460,84 @@ def _need_picks(pos, T: int, dev) -> int:
     return K
 
 
+def _usual(dev, *ts) -> bool:
+    """all contiguous and on the current GPU"""
+    for t in ts:
+        if not t.is_contiguous() or t.get_device() != dev:
+            return False
+    return True
+
+
+# The calls below first ask for their usual case at once (a small call's launch is 3 us, each check of a tensor by itself 0.6); where it is
+# false, the checks say why or allow it.
 def moe_sort_rows(x, pos, xs) -> None:
     """xs[pos[t][k]] = x[t]: the tokens' rows in the order of their experts (pos: group_rows of topi, [T][K] or flat); xs's rows that no pos
     names are left as they were.  Rows of f32, f16, bf16, 8-bit or int32 values (8-bit rows and their scales are two calls)."""
-    dev = _current()
-    if x.dtype not in _ELEM or xs.dtype is not x.dtype:
-        raise ValueError(f"x: type {x.dtype}, xs {xs.dtype}: expected the same, of 1, 2 or 4 bytes")
-    ldx = _need_matrix(x, "x", (x.dtype,), None, dev)
-    ldxs = _need_matrix(xs, "xs", (x.dtype,), x.shape[1], dev)
-    T, H = x.shape
-    K = _need_picks(pos, T, dev)
-    check(lib().sfnx_moe_sort_rows(_ELEM[x.dtype], x.data_ptr(), ldx, T, K, H, pos.data_ptr(), xs.data_ptr(), ldxs, xs.shape[0], _st()))
+    dev, dt = _current(), x.dtype
+    if dt not in _ELEM or xs.dtype is not dt:
+        raise ValueError(f"x: type {dt}, xs {xs.dtype}: expected the same, of 1, 2 or 4 bytes")
+    s, d, p = x.shape, xs.shape, pos.shape
+    if (len(s) == len(d) == len(p) == 2 and s[1] == d[1] and s[0] == p[0] and pos.dtype is torch.int32 and _usual(dev, x, xs, pos)
+            and max(s[0], d[0], s[1]) <= _INT_MAX):
+        K, ldx, ldxs = p[1], s[1], d[1]
+    else:
+        ldx = _need_matrix(x, "x", (dt,), None, dev)
+        ldxs = _need_matrix(xs, "xs", (dt,), s[1], dev)
+        K = _need_picks(pos, s[0], dev)
+    check(lib().sfnx_moe_sort_rows(_ELEM[dt], x.data_ptr(), ldx, s[0], K, s[1], pos.data_ptr(), xs.data_ptr(), ldxs, d[0], _st()))
 
 
 def moe_sort_rows_backward(dxs, pos, dx) -> None:
     """dx[t] = sum_k dxs[pos[t][k]], the gradient of moe_sort_rows; each of f32, f16 or bf16"""
-    dev = _current()
-    lddxs = _need_matrix(dxs, "dxs", _TYPE_ID, None, dev)
-    lddx = _need_matrix(dx, "dx", _TYPE_ID, dxs.shape[1], dev)
-    T, H = dx.shape
-    K = _need_picks(pos, T, dev)
-    check(lib().sfnx_moe_sort_rows_backward(_TYPE_ID[dxs.dtype], dxs.data_ptr(), lddxs, dxs.shape[0], pos.data_ptr(), T, K, H,
+    dev, s, d, p = _current(), dxs.shape, dx.shape, pos.shape
+    if (len(s) == len(d) == len(p) == 2 and s[1] == d[1] and d[0] == p[0] and pos.dtype is torch.int32 and dxs.dtype in _TYPE_ID
+            and dx.dtype in _TYPE_ID and _usual(dev, dxs, dx, pos) and max(s[0], d[0], s[1]) <= _INT_MAX):
+        K, lddxs, lddx = p[1], s[1], d[1]
+    else:
+        lddxs = _need_matrix(dxs, "dxs", _TYPE_ID, None, dev)
+        lddx = _need_matrix(dx, "dx", _TYPE_ID, s[1], dev)
+        K = _need_picks(pos, d[0], dev)
+    check(lib().sfnx_moe_sort_rows_backward(_TYPE_ID[dxs.dtype], dxs.data_ptr(), lddxs, s[0], pos.data_ptr(), d[0], K, s[1],
                                             _TYPE_ID[dx.dtype], dx.data_ptr(), lddx, _st()))
 
 
 def moe_combine_sorted(ys, topw, pos, y) -> None:
     """y[t] = sum_k topw[t][k] ys[pos[t][k]]: moe_combine's sum over rows in the order of their experts; ys and y of f32, f16 or bf16"""
-    dev = _current()
-    ldys = _need_matrix(ys, "ys", _TYPE_ID, None, dev)
-    ldy = _need_matrix(y, "y", _TYPE_ID, ys.shape[1], dev)
-    T, H = y.shape
-    K = _need_picks(pos, T, dev)
-    if not _fine(topw, _F32, (T, K), dev):
-        _need(topw, "topw", _F32, (T, K))
-    check(lib().sfnx_moe_combine_sorted(_TYPE_ID[ys.dtype], ys.data_ptr(), ldys, ys.shape[0], topw.data_ptr(), pos.data_ptr(), T, K, H,
+    dev, s, d, p = _current(), ys.shape, y.shape, pos.shape
+    if (len(s) == len(d) == len(p) == 2 and s[1] == d[1] and d[0] == p[0] and p == topw.shape and pos.dtype is torch.int32
+            and topw.dtype is torch.float32 and ys.dtype in _TYPE_ID and y.dtype in _TYPE_ID and _usual(dev, ys, y, pos, topw)
+            and max(s[0], d[0], s[1]) <= _INT_MAX):
+        K, ldys, ldy = p[1], s[1], d[1]
+    else:
+        ldys = _need_matrix(ys, "ys", _TYPE_ID, None, dev)
+        ldy = _need_matrix(y, "y", _TYPE_ID, s[1], dev)
+        K = _need_picks(pos, d[0], dev)
+        _need(topw, "topw", _F32, (d[0], K))
+    check(lib().sfnx_moe_combine_sorted(_TYPE_ID[ys.dtype], ys.data_ptr(), ldys, s[0], topw.data_ptr(), pos.data_ptr(), d[0], K, s[1],
                                         _TYPE_ID[y.dtype], y.data_ptr(), ldy, _st()))
 
 
 def moe_combine_sorted_backward(dy, ys, topw, pos, dys, dw) -> None:
     """the gradient of moe_combine_sorted: dys[pos[t][k]] = topw[t][k] dy[t] (of ys's type; may be ys) and dw[t][k] = sum_h dy[t][h]
     ys[pos[t][k]][h] (f32); either may be None.  dys's rows that no pos names are left as they were."""
-    dev = _current()
-    lddy = _need_matrix(dy, "dy", _TYPE_ID, None, dev)
-    ldys = _need_matrix(ys, "ys", _TYPE_ID, dy.shape[1], dev)
-    T, H = dy.shape
-    K = _need_picks(pos, T, dev)
-    if not _fine(topw, _F32, (T, K), dev):
-        _need(topw, "topw", _F32, (T, K))
-    lddys = _need_matrix(dys, "dys", (ys.dtype,), H, dev, ys.shape[0]) if dys is not None else H
-    if dw is not None and not _fine(dw, _F32, (T, K), dev):
-        _need(dw, "dw", _F32, (T, K))
+    dev, d, s, p = _current(), dy.shape, ys.shape, pos.shape
+    if (len(s) == len(d) == len(p) == 2 and s[1] == d[1] and d[0] == p[0] and p == topw.shape and pos.dtype is torch.int32
+            and topw.dtype is torch.float32 and ys.dtype in _TYPE_ID and dy.dtype in _TYPE_ID and _usual(dev, dy, ys, pos, topw)
+            and max(s[0], d[0], s[1]) <= _INT_MAX
+            and (dys is None or (dys.dtype is ys.dtype and dys.shape == s and _usual(dev, dys)))
+            and (dw is None or (dw.dtype is torch.float32 and dw.shape == p and _usual(dev, dw)))):
+        K = p[1]
+        lddy = ldys = lddys = s[1]
+    else:
+        lddy = _need_matrix(dy, "dy", _TYPE_ID, None, dev)
+        ldys = _need_matrix(ys, "ys", _TYPE_ID, d[1], dev)
+        K = _need_picks(pos, d[0], dev)
+        _need(topw, "topw", _F32, (d[0], K))
+        lddys = _need_matrix(dys, "dys", (ys.dtype,), d[1], dev, s[0]) if dys is not None else d[1]
+        if dw is not None:
+            _need(dw, "dw", _F32, (d[0], K))
     check(lib().sfnx_moe_combine_sorted_backward(_TYPE_ID[dy.dtype], dy.data_ptr(), lddy, _TYPE_ID[ys.dtype], ys.data_ptr(), ldys,
-                                                 ys.shape[0], topw.data_ptr(), pos.data_ptr(), T, K, H, _p(dys), lddys, _p(dw), _st()))
+                                                 s[0], topw.data_ptr(), pos.data_ptr(), d[0], K, d[1], _p(dys), lddys, _p(dw), _st()))
 
 
 class Adapters:
@@ -550,17 +577,22 @@ def adapter_mm(ad: Adapters, jobs, njobs, njobs_cap: int, x, base, out) -> None:
     """out[t] = base[t] + scale[a] B_a (A_a x[t]) over jobs of the rows' adapters (group_rows in place over each row's adapter; rows of
     group ad.n or above have none, and become base's).  x: f32 or the adapters' type; base: out itself (added in place), None (zeros) or
     of out's type and strides.  Rows of no job are left as they were."""
-    dev = _current()
-    if ad.device != dev:
-        raise ValueError("ad: not on the current GPU")
-    ldx = _need_matrix(x, "x", (torch.float32, ad.dtype), ad.n_in, dev)
-    rows = x.shape[0]
-    ldo = _need_matrix(out, "out", _TYPE_ID, ad.n_out, dev, rows)
-    if base is not None and base is not out:
-        ldb = _need_matrix(base, "base", (out.dtype,), ad.n_out, dev, rows)
-        if ldb != ldo:
-            raise ValueError(f"base: rows {ldb} values apart, out's {ldo}")
-    if not (_fine(jobs, _I32, jobs.shape, dev) and _fine(njobs, _I32, njobs.shape, dev)):
+    dev, s, d = _current(), x.shape, out.shape
+    if (len(s) == len(d) == 2 and s[1] == ad.n_in and d[1] == ad.n_out and s[0] == d[0] and s[0] <= _INT_MAX and ad.device == dev
+            and (x.dtype is ad.dtype or x.dtype is torch.float32) and out.dtype in _TYPE_ID and jobs.dtype is torch.int32
+            and njobs.dtype is torch.int32 and _usual(dev, x, out, jobs, njobs)
+            and (base is None or base is out or (base.dtype is out.dtype and base.shape == d and _usual(dev, base)))):
+        rows, ldx, ldo = s[0], s[1], d[1]
+    else:
+        if ad.device != dev:
+            raise ValueError("ad: not on the current GPU")
+        ldx = _need_matrix(x, "x", (torch.float32, ad.dtype), ad.n_in, dev)
+        rows = s[0]
+        ldo = _need_matrix(out, "out", _TYPE_ID, ad.n_out, dev, rows)
+        if base is not None and base is not out:
+            ldb = _need_matrix(base, "base", (out.dtype,), ad.n_out, dev, rows)
+            if ldb != ldo:
+                raise ValueError(f"base: rows {ldb} values apart, out's {ldo}")
         _need(jobs, "jobs", _I32)
         _need(njobs, "njobs", _I32)
     if njobs_cap < 0 or jobs.numel() < njobs_cap * BIGJOB_INTS or njobs.numel() < 1:

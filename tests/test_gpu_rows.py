@@ -67,8 +67,30 @@ def test_group_fewer_rows_and_no_lists():
     assert (g.pos[300:] == 5).all() and (g.order[300:] == -1).all()
     off = torch.full((10,), -1, dtype=torch.int32).cuda()
     d = ids.cuda()
-    _abi.check(_abi.lib().sfnx_group_rows(d.data_ptr(), 300, 9, off.data_ptr(), None, None, None, None, 0, 0, moe._st()))
+    _abi.check(_abi.lib().sfnx_group_rows(d.data_ptr(), 300, 9, off.data_ptr(), None, None, None, None, 0, 0, None, 0, moe._st()))
     assert torch.equal(off, g.offsets)
+
+
+@pytest.mark.parametrize("n, G", [(4096, 64), (65536, 64), (65537, 64), (131072, 512), (131073, 4096), (300001, 1), (1 << 20, 700)])
+def test_group_many(n, G):
+    """both forms' ends, chunks of several rounds; against a stable sort"""
+    ids = torch.randint(-1, G, (n,), generator=gen(n), dtype=torch.int32)
+    ids[n // 3:n // 3 + 3000] = G - 1
+    g = moe.RowGroups(n, G, in_place=True)
+    moe.group_rows(ids.cuda(), g)
+    by = torch.argsort(torch.where(ids < 0, G, ids), stable=True)
+    cnt = torch.bincount(ids[ids >= 0], minlength=G)
+    m = int(cnt.sum())
+    assert torch.equal(g.offsets.cpu(), torch.cat([torch.zeros(1, dtype=torch.int64), torch.cumsum(cnt, 0)]).int())
+    assert torch.equal(g.order.cpu()[:m], by[:m].int()) and (g.order[m:] == -1).all()
+    pos = torch.full((n,), -1, dtype=torch.int32)
+    pos[by[:m]] = torch.arange(m, dtype=torch.int32)
+    assert torch.equal(g.pos.cpu(), pos)
+    a, nj = g.jobs.cpu().view(-1, 2 + 2 * JOB), int(g.njobs[0])
+    assert nj == int(((cnt + JOB - 1) // JOB).sum()) and int(a[:nj, 1].sum()) == m and not a[nj:].any()
+    there = torch.arange(JOB) < a[:nj, 1:2]
+    assert torch.equal(a[:nj, 2:2 + JOB][there], by[:m].int()) and torch.equal(a[:nj, 2 + JOB:][there], by[:m].int())
+    assert torch.equal(torch.repeat_interleave(a[:nj, 0], a[:nj, 1]), ids[by[:m]])
 
 
 def test_group_in_a_graph():

@@ -8,8 +8,8 @@ P = 4096   # a device pointer that is never dereferenced
 BIG = 1 << 40
 
 
-def group(L, ids=P, n=10, G=4, off=P, pos=P, order=P, jobs=P, njobs=P, cap=10):
-    return L.sfnx_group_rows(ids, n, G, off, pos, order, jobs, njobs, cap, 0, None)
+def group(L, ids=P, n=10, G=4, off=P, pos=P, order=P, jobs=P, njobs=P, cap=10, ws=None, wb=0):
+    return L.sfnx_group_rows(ids, n, G, off, pos, order, jobs, njobs, cap, 0, ws, wb, None)
 
 
 def sort(L, elem=2, x=P, ldx=64, T=4, K=2, H=64, pos=P, xs=P, ldxs=64, rows=8):
@@ -30,7 +30,8 @@ def adapter(L, A=P, sa=BIG, B=P, sb=BIG, t=30, scale=P, n=2, R=16, ni=64, no=64,
 
 
 @pytest.mark.parametrize("fn, args, msg", [
-    (group, dict(n=-1), "n out of range"), (group, dict(n=(1 << 20) + 1, cap=1 << 20), "n out of range"),
+    (group, dict(n=-1), "n out of range"), (group, dict(n=(1 << 24) + 1, cap=1 << 20), "n out of range"), (group, dict(n=70000, cap=2000), "workspace smaller"),
+    (group, dict(n=70000, cap=2000, ws=P, wb=4 * 4 * 69 - 1), "workspace smaller"), (group, dict(n=70000, cap=2000, ws=P + 2, wb=BIG), "4-byte aligned"),
     (group, dict(G=0), "n_groups out of range"), (group, dict(G=4097), "n_groups out of range"),
     (group, dict(ids=None), "null pointer"), (group, dict(off=None), "null pointer"),
     (group, dict(njobs=None), "go together"), (group, dict(jobs=None), "go together"),
