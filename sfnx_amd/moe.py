@@ -597,7 +597,7 @@ def adapter_mm(ad: Adapters, jobs, njobs, njobs_cap: int, x, base, out) -> None:
         _need(njobs, "njobs", _I32)
     if njobs_cap < 0 or jobs.numel() < njobs_cap * BIGJOB_INTS or njobs.numel() < 1:
         raise ValueError("jobs: smaller than the jobs announced, or njobs empty")
-    ws, need = None, lib().sfnx_adapter_workspace(rows, ad.rank, ad.n_in, _TYPE_ID[x.dtype])
+    ws, need = None, 0 if ad.rank <= 32 and rows <= _abi.MAXT else lib().sfnx_adapter_workspace(rows, ad.rank, ad.n_in, _TYPE_ID[x.dtype])
     if need:   # of the stream's allocator: freed here, it goes to later work of this stream only
         ws = torch.empty(need, dtype=torch.uint8, device=x.device)
     check(lib().sfnx_adapter_mm(ad._a, ad.sa, ad._b, ad.sb, ad.type, ad._scale, ad.n, ad.rank, ad.n_in, ad.n_out, jobs.data_ptr(),
@@ -996,17 +996,48 @@ def layer_f8(L: MoeLayerF8, x: torch.Tensor, y: torch.Tensor, b: FloatBuffers) -
     moe_combine(b.part, b.topw, b.topi, b.logits, y, s.E, s.K, s.shared)
 
 
-def layer_16(L: MoeLayer16, x: torch.Tensor, y: torch.Tensor, b: FloatBuffers) -> None:
+@dataclass
+class SharedAdapters:
+    """The requests' low-rank adapters of a layer's shared expert (any of the three may be None; f16, gate and up H -> ff, down ff -> H) and
+    groups, group_rows in place over each row's adapter (rows of none are left out or of a group past the adapters).  One groups serves
+    all layers of a window."""
+    gate: Adapters | None
+    up: Adapters | None
+    down: Adapters | None
+    groups: RowGroups
+
+
+def _need_adapters(s: LayerShape, ad: SharedAdapters) -> None:
+    if not s.shared:
+        raise ValueError("adapters: the layer has no shared expert")
+    for name, a, n_in, n_out in (("gate", ad.gate, s.H, s.ff), ("up", ad.up, s.H, s.ff), ("down", ad.down, s.ff, s.H)):
+        if a is not None and (a.n_in, a.n_out, a.dtype) != (n_in, n_out, torch.float16):
+            raise ValueError(f"adapters.{name}: {a.n_in} -> {a.n_out} of {a.dtype}, expected {n_in} -> {n_out} of torch.float16")
+    if not ad.groups.in_place:
+        raise ValueError("adapters.groups: made for sorted rows, not in place")
+
+
+def layer_16(L: MoeLayer16, x: torch.Tensor, y: torch.Tensor, b: FloatBuffers, adapters: SharedAdapters | None = None) -> None:
     """A decode window or a prompt chunk through a layer of f16 experts: routing, f16 activations, gate|up, SwiGLU to f16,
-    down, the combine"""
+    down, the combine; adapters are added to the shared expert's products"""
     s = L.s
     _need_call(L, x, y, b)
+    if adapters is not None:
+        _need_adapters(s, adapters)
     _route(L, x, b)
     to_f16(x, b.xh)
     mm = moe_mm_16_big if b.big else moe_mm_16
     mm(L.gu_w, L.gu_stride, s.H, 2 * s.ff, b.jobs_gu, b.njobs, b.cap, b.xh, b.gu)
+    if adapters is not None:
+        g, gu = adapters.groups, b.gu[b.T * s.K:]   # the shared expert's rows follow the pairs'
+        for a, out in ((adapters.gate, gu[:, : s.ff]), (adapters.up, gu[:, s.ff:])):
+            if a is not None:
+                adapter_mm(a, g.jobs, g.njobs, g.cap, b.xh, out, out)
     swiglu_h16(b.gu, b.h16, s.ff)
     mm(L.dn_w, L.dn_stride, s.ff, s.H, b.jobs_dn, b.njobs, b.cap, b.h16, b.part)
+    if adapters is not None and adapters.down is not None:
+        out = b.part[b.T * s.K:]
+        adapter_mm(adapters.down, g.jobs, g.njobs, g.cap, b.h16[b.T * s.K:], out, out)
     moe_combine(b.part, b.topw, b.topi, b.logits, y, s.E, s.K, s.shared)
 
 
