@@ -278,6 +278,7 @@ inline void moe_combine_sorted_backward(uint32_t dy_type, const void* dy, int64_
 inline void adapter_mm(const DW& A, size_t sa, const DW& B, size_t sb, const float* scale, int n_adapters, const BigJob* jobs, const int* njobs,
                        int njobs_cap, uint32_t x_type, const void* x, int64_t ldx, const void* base, uint32_t out_type, void* out, int64_t ldo,
                        int rows, void* ws, size_t ws_bytes, void* st) {
+    if (A.type != B.type || A.n_out != B.n_in) throw std::runtime_error("adapter_mm: A and B of different types or ranks");
     ck(sfnx_adapter_mm(detail::base_of(A), detail::stride_of(A, sa), detail::base_of(B), detail::stride_of(B, sb), A.type, scale, n_adapters,
                        A.n_out, A.n_in, B.n_out, jobs, njobs, njobs_cap, x_type, x, ldx, base, out_type, out, ldo, rows, ws, ws_bytes, st));
 }

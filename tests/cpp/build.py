@@ -6,7 +6,7 @@ from pathlib import Path
 
 HERE = Path(__file__).resolve().parent
 ROOT = HERE.parent.parent
-PROGRAMS = ["moe_window", "float_experts"]
+PROGRAMS = ["moe_window", "float_experts", "sorted_rows"]
 
 
 def build(verbose: bool = False) -> None:
