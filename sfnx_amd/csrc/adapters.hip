@@ -97,7 +97,12 @@ template <int OT> __device__ __forceinline__ Eight<OT> pack(const float (&v)[8])
     } else {
         uint32_t w[4];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) w[k] = half_bits(OT, v[2 * k]) | half_bits(OT, v[2 * k + 1]) << 16;
+        for (int k = 0; k < 4; ++k) {   // two at once
+            typedef float float2v __attribute__((ext_vector_type(2)));
+            typedef typename std::conditional<OT == SFNX_F16, _Float16, __bf16>::type T;
+            typedef T pair __attribute__((ext_vector_type(2)));
+            w[k] = __builtin_bit_cast(uint32_t, __builtin_convertvector(float2v{v[2 * k], v[2 * k + 1]}, pair));
+        }
         e.v[0] = uint4{w[0], w[1], w[2], w[3]};
     }
     return e;
@@ -422,19 +427,24 @@ __device__ __forceinline__ uint32_t top16(uint32_t top, const uint4& v) {
     return __builtin_bit_cast(uint32_t, t);
 }
 
-constexpr int AE_COLS = 128, AE_PITCH = AE_COLS + 4;   // columns of a unit, 32 a wavefront; floats of a row of results in LDS
 template <int RT> struct Expand {
-    static constexpr int KB = RT <= 2 ? 1 : RT / 2;    // blocks of 32 ranks
-    static constexpr int SP = 32 * KB + 8;             // values of a token's s in LDS
+    static constexpr int KB = RT <= 2 ? 1 : RT / 2;                 // blocks of 32 ranks
+    // two workgroups of four wavefronts a compute unit, or one of eight where s takes much of its LDS (4096 rows, 4096 -> 4096, us of the
+    // call, four and eight: rank 64 43 and 47; rank 128, 2048 -> 2048, 48 and 39)
+    static constexpr int WAVES = RT == 8 ? 8 : 4, EACH = 8 / WAVES, THREADS = WAVES * WAVE;
+    static constexpr int COLS = 32 * WAVES, PITCH = COLS + 4;       // columns of a unit, 32 a wavefront; floats of a row of results in LDS
+    static constexpr int SP = 32 * KB + 8;                          // values of a token's s in LDS
     static constexpr int S = 3 * SFNX_PF_JOB * SP * 2;
-    static constexpr int LDS = S + SFNX_PF_JOB * AE_PITCH * 4;
+    static constexpr int LDS = S + SFNX_PF_JOB * PITCH * 4;
+    static_assert(EACH * LDS <= 160 * 1024, "");
 };
 template <Elem EL, int RT, int OT>
-__global__ void __launch_bounds__(A2_THREADS) k_adapter_expand(const AdapterArgs a) {
+__global__ void __launch_bounds__(Expand<RT>::THREADS) k_adapter_expand(const AdapterArgs a) {
     typedef Expand<RT> X;
-    // a thread's rows are tid / 16 + 16 i: base and out 8 columns each, s 2 KB ranks
-    constexpr int KB = X::KB, RP = 16 * RT, LANES = AE_COLS / 8, PASSES = SFNX_PF_JOB * LANES / A2_THREADS, RK = 2 * KB;
-    static_assert(LANES == 16, "");
+    constexpr int AE_WAVES = X::WAVES, AE_COLS = X::COLS, AE_PITCH = X::PITCH;
+    // a thread's rows are tid / LANES + 16 i: base and out 8 columns each, s RK ranks
+    constexpr int KB = X::KB, RP = 16 * RT, LANES = AE_COLS / 8, PASSES = SFNX_PF_JOB * LANES / X::THREADS, RK = 32 * KB / LANES;
+    static_assert(PASSES == SFNX_PF_JOB / 16, "");
     extern __shared__ __align__(16) uint8_t lds_[];
     uint16_t* const sp = reinterpret_cast<uint16_t*>(lds_);                  // [3][64][SP]
     float* const res = reinterpret_cast<float*>(lds_ + X::S);                // [64][AE_PITCH]
@@ -444,8 +454,12 @@ __global__ void __launch_bounds__(A2_THREADS) k_adapter_expand(const AdapterArgs
     const sfnx_bigjob& job = a.jobs[j];
     const int nj = *a.njobs, n = min(job.n, SFNX_PF_JOB), w = job.w;
     int o[PASSES];
+    int64_t row[PASSES];
 #pragma unroll
-    for (int i = 0; i < PASSES; ++i) o[i] = job_row(job, n, 16 * i + m0, a.rows).o;
+    for (int i = 0; i < PASSES; ++i) {
+        o[i] = job_row(job, n, 16 * i + m0, a.rows).o;
+        row[i] = o[i] * a.ldo + col;
+    }
     if (j >= nj || n <= 0) return;
     if ((unsigned) w >= (unsigned) a.n) {
 #pragma unroll 1
@@ -489,28 +503,41 @@ __global__ void __launch_bounds__(A2_THREADS) k_adapter_expand(const AdapterArgs
                 }
             constexpr uint32_t INF16 = EL == F16 ? 0x7c00u : 0x7f80u;
             const bool fin = __all(plain && (top & 0xffffu) < INF16 && top >> 16 < INF16);
+            // tiles of 16 rows at once: all four, or the first of a job that has no more, without branches between them
+            const auto tiles = [&](auto count) {
+                constexpr int MT = decltype(count)::value;
+                float4v d[MT][2] = {};
 #pragma unroll
-            for (int m = 0; m < A2_TILES; ++m) {
-                if (16 * m >= n) continue;
-                float4v d[2] = {};
-                if (fin) {
+                for (int p = 2; p >= 0; --p)
 #pragma unroll
-                    for (int p = 2; p >= 0; --p)
+                    for (int k = 0; k < KB; ++k)
 #pragma unroll
-                        for (int k = 0; k < KB; ++k) {
+                        for (int m = 0; m < MT; ++m) {
                             const bf8v s = __builtin_bit_cast(bf8v, lds16((const uint8_t*) (sp + (p * SFNX_PF_JOB + 16 * m + r) * X::SP + 32 * k + 8 * q)));
 #pragma unroll
                             for (int h = 0; h < 2; ++h) {
                                 if constexpr (EL == F16)
-                                    if (p < 2) d[h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(lo[h][k], s, d[h], 0, 0, 0);
-                                d[h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(hi[h][k], s, d[h], 0, 0, 0);
+                                    if (p < 2) d[m][h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(lo[h][k], s, d[m][h], 0, 0, 0);
+                                d[m][h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(hi[h][k], s, d[m][h], 0, 0, 0);
                             }
                         }
-                } else {
+#pragma unroll
+                for (int m = 0; m < MT; ++m)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) *reinterpret_cast<float4v*>(res + (16 * m + r) * AE_PITCH + 32 * wave + 16 * h + 4 * q) = d[m][h];
+            };
+            if (fin && n <= 16) {
+                tiles(std::integral_constant<int, 1>());
+            } else if (fin) {
+                tiles(std::integral_constant<int, A2_TILES>());
+            } else {
+#pragma unroll 1
+                for (int m = 0; 16 * m < n; ++m) {
+                    float4v d[2] = {};
+                    const int om = job_row(job, n, 16 * m + r, a.rows).o;
 #pragma unroll 1
                     for (int k = 0; k < a.rank; ++k) {
                         float f = 0.f;
-                        const int om = job_row(job, n, 16 * m + r, a.rows).o;
                         for (int p = 0; om >= 0 && p < a.parts; ++p) f += a.part[((int64_t) p * a.rows + om) * RP + k];
                         f *= sc;
 #pragma unroll
@@ -519,9 +546,9 @@ __global__ void __launch_bounds__(A2_THREADS) k_adapter_expand(const AdapterArgs
                             d[e / 4][e % 4] = fmaf(f, wide16(EL == F16, reinterpret_cast<const uint16_t*>(Bw)[(size_t) c * a.rank + k]), d[e / 4][e % 4]);
                         }
                     }
-                }
 #pragma unroll
-                for (int h = 0; h < 2; ++h) *reinterpret_cast<float4v*>(res + (16 * m + r) * AE_PITCH + 32 * wave + 16 * h + 4 * q) = d[h];
+                    for (int h = 0; h < 2; ++h) *reinterpret_cast<float4v*>(res + (16 * m + r) * AE_PITCH + 32 * wave + 16 * h + 4 * q) = d[h];
+                }
             }
             lds_barrier();
         }
@@ -540,10 +567,10 @@ __global__ void __launch_bounds__(A2_THREADS) k_adapter_expand(const AdapterArgs
             if (a.base && v + col + 8 <= c1)
 #pragma unroll
                 for (int i = 0; i < PASSES; ++i)
-                    if (o[i] >= 0) next.base[i] = load_eight<OT>(a.base, o[i] * a.ldo + v + col, 8);
+                    if (o[i] >= 0) next.base[i] = load_eight<OT>(a.base, row[i] + v, 8);
         }
         if (t == 0) {   // s: the parts' sum times the scale, zeros for missing rows and beyond the rank
-            constexpr int AT = KB == 1 ? 4 : KB == 2 ? 4 : 2;   // parts requested at once
+            constexpr int AT = KB == 1 ? 4 : 2;   // parts requested at once
             float s[PASSES][RK] = {};
             uint32_t size = 0;
             const int64_t step = (int64_t) a.rows * RP;
@@ -575,8 +602,11 @@ __global__ void __launch_bounds__(A2_THREADS) k_adapter_expand(const AdapterArgs
 #pragma unroll
                     for (int k = 0; k < 3; ++k) *reinterpret_cast<uint32_t*>(sp + (k * SFNX_PF_JOB + 16 * i + m0) * X::SP + rk + c) = p[k];
                 }
-            plain = size < 0x7f800000u;
-            plain = __syncthreads_and(plain);
+            const int fin = __all(size < 0x7f800000u);
+            if (lane == 0) reinterpret_cast<int*>(res)[wave * AE_PITCH + AE_COLS] = fin;   // beside the results
+            lds_barrier();
+#pragma unroll
+            for (int k = 0; k < AE_WAVES; ++k) plain = plain && reinterpret_cast<const int*>(res)[k * AE_PITCH + AE_COLS];
         } else {
             if (u + col + 8 <= c1) {
 #pragma unroll
@@ -588,7 +618,7 @@ __global__ void __launch_bounds__(A2_THREADS) k_adapter_expand(const AdapterArgs
                         const float4v x = reinterpret_cast<const float4v*>(p)[0], y = reinterpret_cast<const float4v*>(p)[1];
 #pragma unroll
                         for (int e = 0; e < 4; ++e) v[e] += x[e], v[4 + e] += y[e];
-                        store_eight<OT>(a.out, o[i] * a.ldo + u + col, 8, pack<OT>(v));
+                        store_eight<OT>(a.out, row[i] + u, 8, pack<OT>(v));
                     }
             } else {   // the row's last columns
 #pragma unroll 1
@@ -635,6 +665,14 @@ void split_columns(int64_t jobs, int n_in, int& parts, int& steps) {
 // Ranks above 32 are two launches: each slice would read 256 KB of A for itself.
 bool two_launches(int rows, int rank, bool x32) { return rank > 32 || rows > 1024 || (x32 && rank > 16 && rows > SFNX_MAXT); }
 
+// Jobs that are not full, as launches take them: one for each adapter, and for the rows without; of a long list a chunk's rows are taken to use a
+// quarter.  More are a second round of workgroups, fewer leave compute units idle (4096 rows of 16 of 64 adapters, 2048 -> 2048, rank 32, f32:
+// 38 us, with all 64 counted 71).
+int64_t short_jobs(const AdapterArgs& a) {
+    const int most = std::min(a.rows, a.n + 1);
+    return a.rows <= 256 ? most : (most + 3) / 4;
+}
+
 // more than 64 KB of LDS are asked for once
 template <auto KERN, int LDS> void launch_lds(unsigned grid, int threads, const AdapterArgs& a, hipStream_t st) {
     if (LDS > 64 * 1024) {
@@ -653,7 +691,7 @@ template <Elem EL, bool X32, int RT> void launch(AdapterArgs a, uint32_t out_typ
     if (a.part == nullptr) {
         if constexpr (RT <= 2) {
             a.subs = std::min(SFNX_PF_JOB / AD_ROWS, (a.rows + AD_ROWS - 1) / AD_ROWS);
-            const int64_t tiles = std::min<int64_t>((int64_t) cap * a.subs, (int64_t) cap + a.rows / AD_ROWS);
+            const int64_t tiles = std::max<int64_t>(1, std::min<int64_t>((int64_t) cap * a.subs, a.rows / AD_ROWS + short_jobs(a)));
             slice(std::max<int64_t>(1, CUS / tiles), AD_UNIT * AW_WAVES);   // one workgroup a compute unit runs at once
             a.units *= AW_WAVES;
             const unsigned grid = grid_of(a.slices * a.subs, cap, AW_THREADS);
@@ -661,13 +699,12 @@ template <Elem EL, bool X32, int RT> void launch(AdapterArgs a, uint32_t out_typ
         }
         return;
     }
-    // the most jobs there may be: a short one for each adapter, and for the rows without one
-    const int64_t jobs = std::min<int64_t>(cap, a.rows / SFNX_PF_JOB + std::min(a.rows, a.n + 1));
+    const int64_t jobs = std::max<int64_t>(1, std::min<int64_t>(cap, a.rows / SFNX_PF_JOB + short_jobs(a)));
     split_columns(jobs, a.n_in, a.parts, a.steps);
-    slice(std::max<int64_t>(1, 2 * CUS / jobs), AE_COLS);   // two workgroups a compute unit run at once
+    slice(std::max<int64_t>(1, Expand<RT>::EACH * CUS / jobs), Expand<RT>::COLS);
     launch_lds<k_adapter_shrink<EL, X32, RT>, Many<X32, RT>::LDS>(grid_of(a.parts, cap, A2_THREADS), A2_THREADS, a, st);
-    const unsigned grid = grid_of(a.slices, cap, A2_THREADS);
-    by_type(out_type, [&](auto ot) { launch_lds<k_adapter_expand<EL, RT, decltype(ot)::value>, Expand<RT>::LDS>(grid, A2_THREADS, a, st); });
+    const unsigned grid = grid_of(a.slices, cap, Expand<RT>::THREADS);
+    by_type(out_type, [&](auto ot) { launch_lds<k_adapter_expand<EL, RT, decltype(ot)::value>, Expand<RT>::LDS>(grid, Expand<RT>::THREADS, a, st); });
 }
 
 }  // namespace
