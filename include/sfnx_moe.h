@@ -244,14 +244,14 @@ int sfnx_moe_mm_16_big(const void* A, size_t sa, uint32_t type, int n_in, int n_
  * offsets[n_groups] left as they were; jobs: a group's rows 64 a job in order, w the group, y and out the rows' numbers, pos (in_place
  * 0, for products over sorted rows) or i (in_place 1, for sfnx_adapter_mm), entries past a job's n and jobs past njobs[0] left as they
  * were; njobs[1] = 0.  pos and order may be null; jobs and njobs together too, else njobs_cap >= n / 64 + min(n, n_groups).
- * 0 <= n <= 2^24, 1 <= n_groups <= 4096.  ws: sfnx_group_rows_workspace bytes (0 for few rows; 4-byte aligned, contents do not matter), one for
- * each of calls that may overlap. */
+ * 0 <= n <= 2^24, 1 <= n_groups <= 4096.  ws: sfnx_group_rows_workspace bytes (0 for few rows, never less for more; 4-byte aligned, contents do not
+ * matter), one for each of calls that may overlap. */
 int sfnx_group_rows(const int* ids, int n, int n_groups, int* offsets, int* pos, int* order, sfnx_bigjob* jobs, int* njobs, int njobs_cap,
                     int in_place, void* ws, size_t ws_bytes, void* st);
 size_t sfnx_group_rows_workspace(int n, int n_groups);
 /* xs[pos[t][k]] = x[t] for rows of H values of elem (1, 2 or 4) bytes, pos [T][K] (of sfnx_group_rows), rows of x and xs ldx and ldxs
  * values apart.  Here and below an entry of pos outside [0, rows) is left out (rows: of the sorted side), a sorted row that no entry names
- * is left as it was, and K <= 64, H <= 2^20.  No two entries may be equal. */
+ * is left as it was, and K <= 64, H <= 2^20.  No two entries may be equal, and outputs overlap no input but where it is said. */
 int sfnx_moe_sort_rows(int elem, const void* x, int64_t ldx, int T, int K, int H, const int* pos, void* xs, int64_t ldxs, int rows, void* st);
 /* dx[t] = sum_k dxs[pos[t][k]], summed in 32 bits in k order and rounded once (0 where every entry is left out).  Types SFNX_F32,
  * SFNX_F16 or SFNX_BF16, each side its own. */
@@ -278,8 +278,9 @@ int sfnx_moe_combine_sorted_backward(uint32_t dy_type, const void* dy, int64_t l
  * they were, and so are rows outside [0, rows) in a job.  A row may be out of one job only.  A_a x and its product with B_a are summed and
  * kept in 32 bits, and rounded once, with base, to out's type.
  * rank % 8 == 0, at most 128; n_in % 8 == 0; n_in and n_out at most 2^20; A, B, x and their rows 16-byte aligned.
- * Few rows of small ranks are one launch, others two, which need a workspace of sfnx_adapter_workspace bytes (0: none), 16-byte aligned,
- * whose contents do not matter; calls that may overlap need one each. */
+ * Few rows of small ranks are one launch, others two, which need a workspace of sfnx_adapter_workspace bytes (0: none; never less for more
+ * rows), 16-byte aligned, whose contents do not matter; calls that may overlap need one each.  out overlaps neither x nor, unless it is base,
+ * base. */
 size_t sfnx_adapter_workspace(int rows, int rank, int n_in, uint32_t x_type);
 int sfnx_adapter_mm(const void* A, size_t sa, const void* B, size_t sb, uint32_t type, const float* scale, int n_adapters, int rank, int n_in,
                     int n_out, const sfnx_bigjob* jobs, const int* njobs, int njobs_cap, uint32_t x_type, const void* x, int64_t ldx,

@@ -673,11 +673,11 @@ int64_t short_jobs(const AdapterArgs& a) {
     return a.rows <= 256 ? most : (most + 3) / 4;
 }
 
-// more than 64 KB of LDS are asked for once
+// more than 64 KB of LDS are asked for once a GPU
 template <auto KERN, int LDS> void launch_lds(unsigned grid, int threads, const AdapterArgs& a, hipStream_t st) {
     if (LDS > 64 * 1024) {
-        static const hipError_t allowed = hipFuncSetAttribute((const void*) KERN, hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
-        check(allowed, "hipFuncSetAttribute");
+        static std::atomic<uint64_t> asked{0};
+        allow_lds((const void*) KERN, LDS, asked);
     }
     KERN<<<grid, threads, LDS, st>>>(a);
 }
@@ -714,9 +714,11 @@ using namespace sfnx;
 
 extern "C" size_t sfnx_adapter_workspace(int rows, int rank, int n_in, uint32_t x_type) {
     if (rows <= 0 || rank <= 0 || n_in <= 0 || !two_launches(rows, rank, x_type == SFNX_F32)) return 0;
-    int parts, steps;
-    split_columns(rows / SFNX_PF_JOB, n_in, parts, steps);   // the fewest jobs have the most parts
-    return (size_t) parts * rows * rank_up(rank) * sizeof(float);
+    // Rows times parts, as more than the split gives for any number of jobs and not less for more rows: at most 8 parts, and with j >= 32 jobs 256 / j for fewer
+    // than 64 (j + 1) rows
+    const int64_t all = (n_in + A2_KC - 1) / A2_KC;
+    const int64_t n = std::max<int64_t>(rows, std::min<int64_t>(std::min<int64_t>(8, all) * rows, (int64_t) CUS * SFNX_PF_JOB * 33 / 32));
+    return (size_t) n * rank_up(rank) * sizeof(float);
 }
 
 extern "C" int sfnx_adapter_mm(const void* A, size_t sa, const void* B, size_t sb, uint32_t type, const float* scale, int n_adapters, int rank,

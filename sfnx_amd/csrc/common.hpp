@@ -4,6 +4,7 @@
 #include <hip/hip_fp16.h>
 #include <hip/hip_runtime.h>
 
+#include <atomic>
 #include <cstdint>
 #include <stdexcept>
 #include <string>
@@ -44,6 +45,15 @@ inline void require(bool ok, const char* msg) {
 }
 inline void check(hipError_t e, const char* what) {
     if (e != hipSuccess) throw std::runtime_error(std::string(what) + ": " + hipGetErrorString(e));
+}
+// lets a kernel have `bytes` of dynamic LDS on the current GPU; asked: the GPUs on which it has been asked for
+inline void allow_lds(const void* kern, int bytes, std::atomic<uint64_t>& asked) {
+    int dev = 0;
+    check(hipGetDevice(&dev), "hipGetDevice");
+    const uint64_t bit = 1ull << (dev & 63);
+    if (asked.load(std::memory_order_relaxed) & bit) return;
+    check(hipFuncSetAttribute(kern, hipFuncAttributeMaxDynamicSharedMemorySize, bytes), "hipFuncSetAttribute");
+    asked.fetch_or(bit, std::memory_order_relaxed);
 }
 inline hipStream_t stream_of(void* st) { return reinterpret_cast<hipStream_t>(st); }
 

@@ -365,8 +365,7 @@ using namespace sfnx;
 
 extern "C" size_t sfnx_group_rows_workspace(int n, int n_groups) {
     if (n <= GR_ALONE || n_groups <= 0) return 0;
-    const int chunk = group_chunk(n);
-    return (size_t) ((n + chunk - 1) / chunk) * n_groups * sizeof(int);
+    return (size_t) GR_CHUNKS * n_groups * sizeof(int);   // a table of all chunks: for more rows never less
 }
 
 extern "C" int sfnx_group_rows(const int* ids, int n, int n_groups, int* offsets, int* pos, int* order, sfnx_bigjob* jobs, int* njobs,
@@ -384,8 +383,8 @@ extern "C" int sfnx_group_rows(const int* ids, int n, int n_groups, int* offsets
         const int chunk = need ? group_chunk(n) : GR_THREADS, blocks = std::max(1, (n + chunk - 1) / chunk);
         int* const table = need ? (int*) ws : nullptr;
         if (table) k_group_count<<<blocks, GR_THREADS, n_groups * sizeof(int), stream_of(st)>>>(ids, n, n_groups, chunk, table);
-        static const hipError_t allowed = hipFuncSetAttribute((const void*) k_group_rows, hipFuncAttributeMaxDynamicSharedMemorySize, 28 * GR_MAX);
-        check(allowed, "hipFuncSetAttribute");
+        static std::atomic<uint64_t> asked{0};
+        if (28 * n_groups > 64 * 1024) allow_lds((const void*) k_group_rows, 28 * GR_MAX, asked);
         k_group_rows<<<blocks, GR_THREADS, 28 * (size_t) n_groups, stream_of(st)>>>(ids, n, n_groups, chunk, table, offsets, pos, order, jobs,
                                                                                        njobs, in_place);
     });

@@ -93,6 +93,14 @@ def test_group_many(n, G):
     assert torch.equal(torch.repeat_interleave(a[:nj, 0], a[:nj, 1]), ids[by[:m]])
 
 
+def test_group_fewer_rows_in_chunks_of_another_size():
+    """131072 rows take 128 chunks, one row more 65: a g for the latter serves the former"""
+    g, ids = moe.RowGroups(131073, 40), torch.randint(0, 40, (131072,), generator=gen(4), dtype=torch.int32)
+    moe.group_rows(ids.cuda(), g)
+    by = torch.argsort(ids, stable=True).int()
+    assert torch.equal(g.order[:131072].cpu(), by) and int(g.order[131072]) == -1
+
+
 def test_group_in_a_graph():
     """captured and replayed on other ids, with eager calls between"""
     ids = torch.zeros(3000, dtype=torch.int32).cuda()

@@ -31,7 +31,7 @@ def adapter(L, A=P, sa=BIG, B=P, sb=BIG, t=30, scale=P, n=2, R=16, ni=64, no=64,
 
 @pytest.mark.parametrize("fn, args, msg", [
     (group, dict(n=-1), "n out of range"), (group, dict(n=(1 << 24) + 1, cap=1 << 20), "n out of range"), (group, dict(n=70000, cap=2000), "workspace smaller"),
-    (group, dict(n=70000, cap=2000, ws=P, wb=4 * 4 * 69 - 1), "workspace smaller"), (group, dict(n=70000, cap=2000, ws=P + 2, wb=BIG), "4-byte aligned"),
+    (group, dict(n=70000, cap=2000, ws=P, wb=4 * 4 * 128 - 1), "workspace smaller"), (group, dict(n=70000, cap=2000, ws=P + 2, wb=BIG), "4-byte aligned"),
     (group, dict(G=0), "n_groups out of range"), (group, dict(G=4097), "n_groups out of range"),
     (group, dict(ids=None), "null pointer"), (group, dict(off=None), "null pointer"),
     (group, dict(njobs=None), "go together"), (group, dict(jobs=None), "go together"),
@@ -87,3 +87,21 @@ def test_python_refuses():
     for k, (call, msg) in enumerate(cases):
         with pytest.raises(ValueError, match=msg):
             call()
+
+
+def test_workspaces_grow_with_rows():
+    """a workspace for the most rows serves fewer; none where one launch is used"""
+    L = _abi.lib()
+    for args in ((16, 1 << 20, 30), (40, 4096, 30), (128, 64, 0), (32, 2048, 0)):
+        last = 0
+        for rows in list(range(0, 9000, 7)) + [1 << 16, 1 << 20]:
+            now = L.sfnx_adapter_workspace(rows, *args)
+            assert now >= last
+            last = now
+    assert L.sfnx_adapter_workspace(1024, 32, 4096, 30) == 0 and L.sfnx_adapter_workspace(16, 32, 4096, 0) == 0 and L.sfnx_adapter_workspace(1, 40, 4096, 0) > 0
+    last = 0
+    for n in list(range(0, 300000, 997)) + [1 << 24]:
+        now = L.sfnx_group_rows_workspace(n, 512)
+        assert now >= last
+        last = now
+    assert L.sfnx_group_rows_workspace(65536, 4096) == 0 and last == 4 * 128 * 512
