@@ -162,7 +162,8 @@ template <Elem EL, bool X32> __device__ __forceinline__ float4v shrink_mma(const
 __device__ __forceinline__ uint4 lds16(const uint8_t* p) { return *reinterpret_cast<const uint4*>(p); }
 
 // ------------------------------------------------------------------------------------------------ one launch
-// For few rows and small ranks.  Each wavefront copies its own chunks of columns and multiplies them, so that none waits for another
+// For few rows and small ranks.  Bound by a chain of reads: the job, its rows of x and A, B's tail, a launch's start (1 row, rank 16, 2048 -> 1024, f32: 5.3 us; 16 rows of
+// 16 adapters, 2048 -> 2048, bf16: 6.1).  Each wavefront copies its own chunks of columns and multiplies them, so that none waits for another
 // before the sum; base and B are on their way meanwhile.  Loops stay rolled: a launch of few workgroups runs its code once, and fetching it is
 // part of its time (f32 x, 16 ranks, 2048 columns, unrolled to one pass: 12.7 us a launch).
 constexpr int AW_WAVES = 8, AW_THREADS = AW_WAVES * WAVE;
@@ -304,7 +305,8 @@ __global__ void __launch_bounds__(AW_THREADS) k_adapter_mm(const AdapterArgs a) 
 
 // ------------------------------------------------------------------------------------------------ two launches
 // The first: a workgroup takes a job's rows and a part of the input columns, 128 columns a stage, stages in flight while one is multiplied;
-// each wavefront takes 32 of a stage's columns, all rows and all ranks.
+// each wavefront takes 32 of a stage's columns, all rows and all ranks.  Bound by what a compute unit takes in, x and A for each 64 rows again: 4096
+// rows, rank 64, 4096 columns, bf16, 34 MB of x and as much of A out of the L2, 14.5 us.
 constexpr int A2_WAVES = 4, A2_THREADS = A2_WAVES * WAVE, A2_TILES = SFNX_PF_JOB / AD_ROWS, A2_KC = 128;
 template <bool X32, int RT> struct Many {
     static constexpr int XROW = A2_KC * (X32 ? 4 : 2), AROW = A2_KC * 2;
@@ -406,6 +408,8 @@ __global__ void __launch_bounds__(A2_THREADS) k_adapter_shrink(const AdapterArgs
 // last (truncated, so that none overflows).  Their products with B's values are exact; f16 values of B are two bf16 parts (the product of
 // both lowest, 2^-25 of the whole, is left out).  A part that is 0 times an infinity would be NaN where the product is not: jobs with such
 // an s, and columns with such a B, are computed value by value.  The results pass through LDS, so that base and out go by whole rows' pieces.
+// 4096 rows, rank 64, 4096 columns, bf16, 67 MB of base and out: 24.6 us, of which 6 pass before the first product (the job, then the parts of s, which
+// every slice sums and splits for itself), and 2.6 for each unit of 128 columns: reads of LDS and products 1.5, the way out 1.
 // the same for two values, packed; of finite ones
 __device__ __forceinline__ void split3(float f, float g, uint32_t (&p)[3]) {
     constexpr uint32_t HI = 0xffff0000u;
@@ -656,13 +660,13 @@ void split_columns(int64_t jobs, int n_in, int& parts, int& steps) {
 
 // The form.  One launch computes s in each slice and holds 128 KB of LDS, two have a launch more and pass s through memory.  us in a graph, one
 // and two launches, 4 adapters of a list of 8, 2048 -> 2048 columns, bf16:
-//   rows                       16          128         512         1024        2048        4096
-//   rank 16, bf16 x            5.9  8.5    7.0  9.9    8.5  11.3   10.4  12.9  17.3  17.1  33    22.6
-//   rank 32, bf16 x            8.0  8.8    8.2  10.6   9.7  12.1   12.0  14.2  20.1  18.9
-//   rank 16, f32 x             8.7  9.8    10.2 11.4   11.3 12.7   13.1  14.6  21.0  20.2
-//   rank 32, f32 x            12.6  10.8   13.8 12.9   15.4 14.1   17.6  16.5  26.3  22.8
-// A window's rows are mostly one to an adapter, which one launch multiplies without the matrix cores' empty rows (1 row, rank 16, f32: 5.5 and 9.6).
-// Ranks above 32 are two launches: each slice would read 256 KB of A for itself.
+//   rows                 1          16          128         512         1024        2048        4096
+//   rank 16, bf16 x      4.6  7.9   6.3  8.2    7.0  9.4    8.4  10.7   10.1 12.4   17.0 16.7   32.9 21.9
+//   rank 32, bf16 x      6.0  8.3   7.9  8.4    8.1  10.3   9.6  11.6   11.8 13.9   19.7 18.5   37.7 23.2
+//   rank 16, f32 x       5.3  9.1   9.6  9.5    10.7 11.2   11.9 12.2   13.9 14.2   21.6 19.8   40.5 25.6
+//   rank 32, f32 x       6.7  10.3  12.6 10.4   13.7 12.4   15.1 13.6   17.4 16.1   25.9 22.4   48.9 28.7
+// A window's rows are mostly one to an adapter, which one launch multiplies as the first column does.  Ranks above 32 are two launches: each slice would
+// read 256 KB of A for itself, of which a compute unit takes in about 35 KB/us.
 bool two_launches(int rows, int rank, bool x32) { return rank > 32 || rows > 1024 || (x32 && rank > 16 && rows > SFNX_MAXT); }
 
 // Jobs that are not full, as launches take them: one for each adapter, and for the rows without; of a long list a chunk's rows are taken to use a
