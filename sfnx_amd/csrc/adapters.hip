@@ -410,7 +410,7 @@ __global__ void __launch_bounds__(A2_THREADS) k_adapter_shrink(const AdapterArgs
 // an s, and columns with such a B, are computed value by value.  The results pass through LDS, so that base and out go by whole rows' pieces.
 // 4096 rows, rank 64, 4096 columns, bf16, 67 MB of base and out: 24.6 us, of which 6 pass before the first product (the job, then the parts of s, which
 // every slice sums and splits for itself), and 2.6 for each unit of 128 columns: reads of LDS and products 1.5, the way out 1.
-// the same for two values, packed; of finite ones
+// the parts of two finite values, packed
 __device__ __forceinline__ void split3(float f, float g, uint32_t (&p)[3]) {
     constexpr uint32_t HI = 0xffff0000u;
     const uint32_t a = __float_as_uint(f), b = __float_as_uint(g);
@@ -704,7 +704,7 @@ template <Elem EL, bool X32, int RT> void launch(AdapterArgs a, uint32_t out_typ
         return;
     }
     const int64_t jobs = std::max<int64_t>(1, std::min<int64_t>(cap, a.rows / SFNX_PF_JOB + short_jobs(a)));
-    split_columns(jobs, a.n_in, a.parts, a.steps);
+    split_columns(std::max<int64_t>(jobs, a.rows / SFNX_PF_JOB), a.n_in, a.parts, a.steps);   // a short list of many rows' jobs: the workspace goes by rows
     slice(std::max<int64_t>(1, Expand<RT>::EACH * CUS / jobs), Expand<RT>::COLS);
     launch_lds<k_adapter_shrink<EL, X32, RT>, Many<X32, RT>::LDS>(grid_of(a.parts, cap, A2_THREADS), A2_THREADS, a, st);
     const unsigned grid = grid_of(a.slices, cap, Expand<RT>::THREADS);

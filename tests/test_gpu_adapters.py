@@ -137,6 +137,28 @@ def test_matrices_that_are_not_finite(T, R, t):
     assert torch.isfinite(out[(ids == 0).cuda()]).all() and torch.isinf(out[3, [7, 199]]).all()
 
 
+@pytest.mark.parametrize("T, R", [(5000, 16), (3000, 64), (700, 128)])
+def test_few_jobs_of_many_rows(T, R):
+    """a list shorter than the rows would fill: the rows' workspace, whose guard behind it stays, and rows of no job"""
+    n, n_in, n_out = 2, 2048, 96
+    A, B, scale = matrices(n, R, n_in, n_out, torch.bfloat16)
+    x, base = rand(gen(1), (T, n_in), torch.bfloat16), rand(gen(2), (T, n_out), torch.float32)
+    rows = torch.tensor([0, 5, T - 1, T // 2], dtype=torch.int32)
+    a = torch.zeros((1, 130), dtype=torch.int32)
+    a[0, 0], a[0, 1], a[0, 2:6], a[0, 66:70] = 1, 4, rows, rows
+    ids = torch.full((T,), -1, dtype=torch.int32)
+    ids[rows.long()] = 1
+    d = dict(A=A.cuda(), B=B.cuda(), f=scale.cuda(), x=x.cuda(), out=base.cuda(), jobs=a.view(-1).cuda(), njobs=torch.tensor([1, 0], dtype=torch.int32).cuda())
+    need = _abi.lib().sfnx_adapter_workspace(T, R, n_in, _abi.BF16)
+    ws = torch.full((need + 4096,), 0xAB, dtype=torch.uint8, device="cuda")
+    p = {k: v.data_ptr() for k, v in d.items()}
+    _abi.check(_abi.lib().sfnx_adapter_mm(p["A"], 2 * R * n_in, p["B"], 2 * n_out * R, _abi.BF16, p["f"], n, R, n_in, n_out, p["jobs"], p["njobs"], 1,
+                                          _abi.BF16, p["x"], n_in, p["out"], _abi.F32, p["out"], n_out, T, ws.data_ptr(), need, moe._st()))
+    want, bound = adapted(x, A, B, scale, ids, base)
+    within(d["out"], want, bound, torch.float32)
+    assert torch.equal(d["out"][(ids < 0).cuda()].cpu(), base[ids < 0]) and need and (ws[need:] == 0xAB).all()
+
+
 def test_past_32_bit_offsets_of_few_rows():
     """rows 2^22 values apart, 700 of them"""
     T, n_in, n_out, R, ld = 700, 256, 264, 8, 1 << 22

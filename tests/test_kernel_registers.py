@@ -51,3 +51,9 @@ def test_window_gate_up_two_workgroups(kernels, wtype, G):
     registers"""
     v = [v[0] for n, v in kernels.items() if f"k_dec_expertsILi{wtype}ELi{G}E" in n]
     assert v and max(v) <= 64
+
+
+def test_row_and_adapter_kernels_do_not_spill(kernels):
+    new = {n: v for n, v in kernels.items() if any(k in n for k in ("k_adapter", "k_group", "k_sort_rows", "k_combine_sorted"))}
+    assert len(new) > 60
+    assert not {n: v for n, v in new.items() if v[1]}
