@@ -193,60 +193,78 @@ template <int TYPE> __device__ __forceinline__ typename ElemOf<TYPE>::type from_
 template <int TYPE, int E> struct alignas((TYPE == SFNX_F32 ? 4 : 2) * E < 16 ? (TYPE == SFNX_F32 ? 4 : 2) * E : 16) Pack {
     typename ElemOf<TYPE>::type v[E];
 };
-template <int TYPE, int E> __device__ __forceinline__ const Pack<TYPE, E>& pack_at(const void* p, int64_t i) {
-    return *reinterpret_cast<const Pack<TYPE, E>*>((const typename ElemOf<TYPE>::type*) p + i);
+// ALIGNED: aligned to the piece's size (16 bytes at most); else to the type's, which is enough for wide accesses
+template <int TYPE, int E, bool ALIGNED> __device__ __forceinline__ Pack<TYPE, E> load_pack(const void* p, int64_t i) {
+    typedef typename ElemOf<TYPE>::type T;
+    Pack<TYPE, E> r;
+    __builtin_memcpy(&r, __builtin_assume_aligned((const T*) p + i, ALIGNED ? alignof(Pack<TYPE, E>) : sizeof(T)), E * sizeof(T));
+    return r;
 }
-template <int TYPE, int E> __device__ __forceinline__ void store_pack(void* p, int64_t i, const float (&v)[E]) {
+template <int TYPE, int E, bool ALIGNED> __device__ __forceinline__ void store_pack(void* p, int64_t i, const float (&v)[E]) {
+    typedef typename ElemOf<TYPE>::type T;
     Pack<TYPE, E> o;
 #pragma unroll
     for (int e = 0; e < E; ++e) o.v[e] = from_float<TYPE>(v[e]);
-    *reinterpret_cast<Pack<TYPE, E>*>((typename ElemOf<TYPE>::type*) p + i) = o;
+    __builtin_memcpy(__builtin_assume_aligned((T*) p + i, ALIGNED ? alignof(Pack<TYPE, E>) : sizeof(T)), &o, E * sizeof(T));
 }
+// A row of n values is n / E pieces and, one by one, the values behind them (none of aligned rows); 2048 tokens with 10 picks of
+// 2047 bf16 columns take 27 us to sort, 31 to combine and 58 in the gradient; all value by value 40, 45 and 70.
+template <int E> constexpr int pieces_of(int n) { return n / E + n % E; }
 constexpr int RW_THREADS = 256, RW_GROUP = 8;   // rows requested before the first is used
 
 // ------------------------------------------------------------------------------------------------ sort_rows
-// xs[pos[t][k]] = x[t]: a token's row is read once and written K times.  PIECE: the bytes a thread moves.  Bound by its writes: 2048 tokens, 10 picks,
-// 2048 bf16 columns, 92 MB, 18.7 us (4.9 TB/s).
-template <typename PIECE>
-__global__ void __launch_bounds__(RW_THREADS) k_sort_rows(const uint8_t* __restrict__ x, int64_t ldx, int K, int pieces, int blocks,
+// xs[pos[t][k]] = x[t]: a token's row is read once and written K times, 16 bytes a thread (ELEM: the bytes of a value).  Bound by its writes: 2048
+// tokens, 10 picks, 2048 bf16 columns, 92 MB, 18.7 us (4.9 TB/s).
+template <int ELEM, bool ALIGNED>
+__global__ void __launch_bounds__(RW_THREADS) k_sort_rows(const uint8_t* __restrict__ x, int64_t ldx, int K, int H, int blocks,
                                                          const int* __restrict__ pos, uint8_t* __restrict__ xs, int64_t ldxs, int rows) {
-    const int t = blockIdx.x / blocks, c = (blockIdx.x % blocks) * blockDim.x + threadIdx.x;
-    if (c >= pieces) return;
-    const PIECE v = *(reinterpret_cast<const PIECE*>(x + (int64_t) t * ldx) + c);
-    for (int k = 0; k < K; ++k) {
-        const int p = pos[(int64_t) t * K + k];
-        if ((unsigned) p < (unsigned) rows) *(reinterpret_cast<PIECE*>(xs + (int64_t) p * ldxs) + c) = v;
-    }
+    constexpr int E = 16 / ELEM;
+    const int t = blockIdx.x / blocks, i = (blockIdx.x % blocks) * blockDim.x + threadIdx.x, full = H / E;
+    const auto move = [&](int64_t at, auto v) {
+        constexpr int AL = ALIGNED ? 16 : ELEM;
+        __builtin_memcpy(&v, __builtin_assume_aligned(x + t * ldx + at, AL), sizeof(v));
+        for (int k = 0; k < K; ++k) {
+            const int p = pos[(int64_t) t * K + k];
+            if ((unsigned) p < (unsigned) rows) __builtin_memcpy(__builtin_assume_aligned(xs + p * ldxs + at, AL), &v, sizeof(v));
+        }
+    };
+    typedef typename std::conditional<ELEM == 4, uint32_t, typename std::conditional<ELEM == 2, uint16_t, uint8_t>::type>::type One;
+    if (i < full) move(i * 16, uint4{});
+    else if (!ALIGNED && i < pieces_of<E>(H)) move((full * E + i - full) * ELEM, One{});
 }
 
 // ------------------------------------------------------------------------------------------------ combine
 // y[t] = sum_k w[t][k] ys[pos[t][k]] in k order, fmaf in 32 bits, one rounding to y's type; w null: 1 (the gradient of
 // sort_rows).  Bound by its reads: 4096 tokens, 10 picks, 2048 bf16 columns, 185 MB, 40.6 us (4.6 TB/s; 12 rows requested at once 44.5).
-template <int YS, int Y, int E>
+template <int YS, int Y, int E, bool ALIGNED>
 __global__ void __launch_bounds__(RW_THREADS) k_combine_sorted(const void* __restrict__ ys, int64_t ldys, int rows, const float* __restrict__ w,
                                                               const int* __restrict__ pos, int K, int H, int blocks, void* __restrict__ y,
                                                               int64_t ldy) {
-    const int t = blockIdx.x / blocks, c = ((blockIdx.x % blocks) * blockDim.x + threadIdx.x) * E;
-    if (c >= H) return;
-    float s[E] = {};
-    for (int k0 = 0; k0 < K; k0 += RW_GROUP) {
-        Pack<YS, E> v[RW_GROUP];
-        bool in[RW_GROUP];
+    const int t = blockIdx.x / blocks, i = (blockIdx.x % blocks) * blockDim.x + threadIdx.x, full = H / E;
+    const auto sum = [&](int c, auto size) {
+        constexpr int N = decltype(size)::value;
+        float s[N] = {};
+        for (int k0 = 0; k0 < K; k0 += RW_GROUP) {
+            Pack<YS, N> v[RW_GROUP];
+            bool in[RW_GROUP];
 #pragma unroll
-        for (int k = 0; k < RW_GROUP; ++k) {
-            const int p = k0 + k < K ? pos[(int64_t) t * K + k0 + k] : -1;
-            in[k] = (unsigned) p < (unsigned) rows;
-            if (in[k]) v[k] = pack_at<YS, E>(ys, p * ldys + c);
-        }
-#pragma unroll
-        for (int k = 0; k < RW_GROUP; ++k)
-            if (in[k]) {
-                const float wk = w ? w[(int64_t) t * K + k0 + k] : 1.f;
-#pragma unroll
-                for (int e = 0; e < E; ++e) s[e] = fmaf(wk, to_float<YS>(v[k].v[e]), s[e]);
+            for (int k = 0; k < RW_GROUP; ++k) {
+                const int p = k0 + k < K ? pos[(int64_t) t * K + k0 + k] : -1;
+                in[k] = (unsigned) p < (unsigned) rows;
+                if (in[k]) v[k] = load_pack<YS, N, ALIGNED>(ys, p * ldys + c);
             }
-    }
-    store_pack<Y, E>(y, t * ldy + c, s);
+#pragma unroll
+            for (int k = 0; k < RW_GROUP; ++k)
+                if (in[k]) {
+                    const float wk = w ? w[(int64_t) t * K + k0 + k] : 1.f;
+#pragma unroll
+                    for (int e = 0; e < N; ++e) s[e] = fmaf(wk, to_float<YS>(v[k].v[e]), s[e]);
+                }
+        }
+        store_pack<Y, N, ALIGNED>(y, t * ldy + c, s);
+    };
+    if (i < full) sum(i * E, std::integral_constant<int, E>());
+    else if (!ALIGNED && i < pieces_of<E>(H)) sum(full * E + i - full, std::integral_constant<int, 1>());
 }
 
 // dys[pos[t][k]] = w[t][k] dy[t], dw[t][k] = sum_h dy[t][h] ys[pos[t][k]][h]: a workgroup a token, a wavefront a pick (the 17th on go to
@@ -255,7 +273,7 @@ __global__ void __launch_bounds__(RW_THREADS) k_combine_sorted(const void* __res
 // rate); 10 picks of 1024 columns 42 us, where four pieces at once leave room for fewer wavefronts: 56.  With all of a token's
 // picks in one thread's registers and their sums joined in LDS 52 and 84.
 constexpr int CB_WAVES = 16, CB_AT = 2;   // pieces of a row requested at once
-template <int YS, int DY, int E>
+template <int YS, int DY, int E, bool ALIGNED>
 __global__ void __launch_bounds__(CB_WAVES * WAVE) k_combine_sorted_backward(const void* __restrict__ dy, int64_t lddy, const void* ys, int64_t ldys,
                                                                             int rows, const float* __restrict__ w, const int* __restrict__ pos,
                                                                             int K, int H, void* dys, int64_t lddys, float* __restrict__ dw) {
@@ -266,21 +284,22 @@ __global__ void __launch_bounds__(CB_WAVES * WAVE) k_combine_sorted_backward(con
         float s = 0.f;
         if ((unsigned) p < (unsigned) rows) {
             const float wk = dys ? w[at] : 0.f;
-            for (int c0 = lane * E; c0 < H; c0 += CB_AT * WAVE * E) {
+            const int full = H / E * E;
+            for (int c0 = lane * E; c0 < full; c0 += CB_AT * WAVE * E) {
                 Pack<DY, E> d[CB_AT];
                 Pack<YS, E> v[CB_AT];
 #pragma unroll
                 for (int u = 0; u < CB_AT; ++u) {
                     const int c = c0 + u * WAVE * E;
-                    if (c < H) {
-                        d[u] = pack_at<DY, E>(dy, t * lddy + c);
-                        if (dw) v[u] = pack_at<YS, E>(ys, p * ldys + c);
+                    if (c < full) {
+                        d[u] = load_pack<DY, E, ALIGNED>(dy, t * lddy + c);
+                        if (dw) v[u] = load_pack<YS, E, ALIGNED>(ys, p * ldys + c);
                     }
                 }
 #pragma unroll
                 for (int u = 0; u < CB_AT; ++u) {
                     const int c = c0 + u * WAVE * E;
-                    if (c >= H) continue;
+                    if (c >= full) continue;
                     float o[E];
 #pragma unroll
                     for (int e = 0; e < E; ++e) {
@@ -288,8 +307,14 @@ __global__ void __launch_bounds__(CB_WAVES * WAVE) k_combine_sorted_backward(con
                         o[e] = wk * g;
                         if (dw) s = fmaf(g, to_float<YS>(v[u].v[e]), s);
                     }
-                    if (dys) store_pack<YS, E>(dys, p * lddys + c, o);
+                    if (dys) store_pack<YS, E, ALIGNED>(dys, p * lddys + c, o);
                 }
+            }
+            if (!ALIGNED && full + lane < H) {   // the values behind the pieces
+                const int c = full + lane;
+                const float g = to_float<DY>(load_pack<DY, 1, false>(dy, t * lddy + c).v[0]), o[1] = {wk * g};
+                if (dw) s = fmaf(g, to_float<YS>(load_pack<YS, 1, false>(ys, p * ldys + c).v[0]), s);
+                if (dys) store_pack<YS, 1, false>(dys, p * lddys + c, o);
             }
             s = group_sum<WAVE>(s);
         }
@@ -347,13 +372,12 @@ void combine_sorted(uint32_t ys_type, const void* ys, int64_t ldys, int rows, co
         by_type(y_type, [&](auto b) {
             constexpr int YS = decltype(a)::value, Y = decltype(b)::value, E = wide_of(YS);
             const int yb = E * out_size(Y) < 16 ? E * out_size(Y) : 16;
-            if (H % E == 0 && wide(ys, ldys, out_size(YS), 16) && wide(y, ldy, out_size(Y), yb)) {
-                const RowSplit r = row_split(H / E);
-                k_combine_sorted<YS, Y, E><<<grid_rows(T, r.blocks, r.threads), r.threads, 0, st>>>(ys, ldys, rows, w, pos, K, H, r.blocks, y, ldy);
-            } else {
-                const RowSplit r = row_split(H);
-                k_combine_sorted<YS, Y, 1><<<grid_rows(T, r.blocks, r.threads), r.threads, 0, st>>>(ys, ldys, rows, w, pos, K, H, r.blocks, y, ldy);
-            }
+            const RowSplit r = row_split(pieces_of<E>(H));
+            const unsigned grid = grid_rows(T, r.blocks, r.threads);
+            if (H % E == 0 && wide(ys, ldys, out_size(YS), 16) && wide(y, ldy, out_size(Y), yb))
+                k_combine_sorted<YS, Y, E, true><<<grid, r.threads, 0, st>>>(ys, ldys, rows, w, pos, K, H, r.blocks, y, ldy);
+            else
+                k_combine_sorted<YS, Y, E, false><<<grid, r.threads, 0, st>>>(ys, ldys, rows, w, pos, K, H, r.blocks, y, ldy);
         });
     });
 }
@@ -398,17 +422,17 @@ extern "C" int sfnx_moe_sort_rows(int elem, const void* x, int64_t ldx, int T, i
         check_rows(x, ldx, H, elem, T > 0);
         check_rows(xs, ldxs, H, elem, T > 0 && rows > 0);
         if (T == 0) return;
-        const auto go = [&](auto piece) {
-            typedef decltype(piece) P;
-            const int pieces = (int) ((int64_t) H * elem / sizeof(P));
-            const RowSplit r = row_split(pieces);
-            k_sort_rows<P><<<grid_rows(T, r.blocks, r.threads), r.threads, 0, stream_of(st)>>>((const uint8_t*) x, ldx * elem, K, pieces, r.blocks, pos,
-                                                                                             (uint8_t*) xs, ldxs * elem, rows);
+        const bool aligned = H * elem % 16 == 0 && wide(x, ldx, elem, 16) && wide(xs, ldxs, elem, 16);
+        const auto go = [&](auto size) {
+            constexpr int ELEM = decltype(size)::value;
+            const RowSplit r = row_split(pieces_of<16 / ELEM>(H));
+            const unsigned grid = grid_rows(T, r.blocks, r.threads);
+            const auto kern = aligned ? k_sort_rows<ELEM, true> : k_sort_rows<ELEM, false>;
+            kern<<<grid, r.threads, 0, stream_of(st)>>>((const uint8_t*) x, ldx * elem, K, H, r.blocks, pos, (uint8_t*) xs, ldxs * elem, rows);
         };
-        if (H * elem % 16 == 0 && wide(x, ldx, elem, 16) && wide(xs, ldxs, elem, 16)) go(uint4{});
-        else if (elem == 4) go(uint32_t{});
-        else if (elem == 2) go(uint16_t{});
-        else go(uint8_t{});
+        if (elem == 4) go(std::integral_constant<int, 4>());
+        else if (elem == 2) go(std::integral_constant<int, 2>());
+        else go(std::integral_constant<int, 1>());
     });
 }
 
@@ -446,9 +470,9 @@ extern "C" int sfnx_moe_combine_sorted_backward(uint32_t dy_type, const void* dy
                 constexpr int YS = decltype(a)::value, DY = decltype(b)::value, E = wide_of(YS);
                 const int db = E * out_size(DY) < 16 ? E * out_size(DY) : 16, threads = std::min(K, CB_WAVES) * WAVE;
                 if (H % E == 0 && wide(ys, ldys, out_size(YS), 16) && (!dys || wide(dys, lddys, out_size(YS), 16)) && wide(dy, lddy, out_size(DY), db))
-                    k_combine_sorted_backward<YS, DY, E><<<grid, threads, 0, stream_of(st)>>>(dy, lddy, ys, ldys, rows, topw, pos, K, H, dys, lddys, dw);
+                    k_combine_sorted_backward<YS, DY, E, true><<<grid, threads, 0, stream_of(st)>>>(dy, lddy, ys, ldys, rows, topw, pos, K, H, dys, lddys, dw);
                 else
-                    k_combine_sorted_backward<YS, DY, 1><<<grid, threads, 0, stream_of(st)>>>(dy, lddy, ys, ldys, rows, topw, pos, K, H, dys, lddys, dw);
+                    k_combine_sorted_backward<YS, DY, E, false><<<grid, threads, 0, stream_of(st)>>>(dy, lddy, ys, ldys, rows, topw, pos, K, H, dys, lddys, dw);
             });
         });
     });
