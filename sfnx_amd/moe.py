@@ -549,11 +549,14 @@ class Adapters:
         self.A, self.B, self.scale = A, B, scale   # held: the tables point into them
         if len(A) < 1 or len(A) != len(B):
             raise ValueError("A and B: expected a matrix of each for every adapter")
-        self.n, t = len(A), A[0]
-        if t.dtype not in (torch.float16, torch.bfloat16):
-            raise ValueError(f"A: type {t.dtype}, expected torch.float16 or torch.bfloat16")
-        (self.rank, self.n_in), self.n_out, self.dtype, self.type = t.shape, B[0].shape[0], t.dtype, _TYPE_ID[t.dtype]
-        self.device = t.get_device()
+        a, b = (M if isinstance(M, torch.Tensor) else M[0] for M in (A, B))
+        if a.dtype not in (torch.float16, torch.bfloat16):
+            raise ValueError(f"A: type {a.dtype}, expected torch.float16 or torch.bfloat16")
+        for name, m, M in (("A", a, A), ("B", b, B)):
+            if m.dim() != 2 + (m is M):
+                raise ValueError(f"{name}: {m.dim()} dimensions, expected a matrix for each adapter")
+        self.n, self.dtype, self.type, self.device = len(A), a.dtype, _TYPE_ID[a.dtype], a.get_device()
+        self.rank, self.n_in, self.n_out = a.shape[-2], a.shape[-1], b.shape[-2]
         self._a, self.sa, self._A = self._place("A", A, (self.rank, self.n_in))
         self._b, self.sb, self._B = self._place("B", B, (self.n_out, self.rank))
         if scale is not None:

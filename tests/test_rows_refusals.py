@@ -81,6 +81,8 @@ def test_python_refuses():
         (lambda: moe.moe_combine_sorted(f(8, 8).double(), f(4, 2), i(4, 2), f(4, 8)), "ys: type"),
         (lambda: moe.moe_sort_rows_backward(f(8, 8, t=torch.uint8), i(4, 2), f(4, 8)), "dxs: type"),
         (lambda: moe.Adapters(f(2, 8, 16), f(2, 5, 8)), "A: type"), (lambda: moe.Adapters(f(0, 8, 16), f(0, 5, 8)), "for every adapter"),
+        (lambda: moe.Adapters(f(2, 8, t=torch.bfloat16), f(2, 5, 8, t=torch.bfloat16)), "A: 2 dimensions"),
+        (lambda: moe.Adapters([f(8, 16, t=torch.bfloat16)], [f(8, t=torch.bfloat16)]), "B: 1 dimensions"),
         (lambda: moe.Adapters(f(2, 8, 16, t=torch.bfloat16), f(3, 5, 8, t=torch.bfloat16)), "for every adapter"),
         (lambda: moe.Adapters(f(2, 8, 16, t=torch.bfloat16), f(2, 5, 4, t=torch.bfloat16)), "B: shape|A: not on"),
     ]
