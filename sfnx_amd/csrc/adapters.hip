@@ -30,7 +30,7 @@ struct AdapterArgs {
     int64_t ldo;
     int rows;                 // of x, base and out
     int slices, units;        // of the outputs: slices of `units` units
-    int subs;                 // one launch: tiles of 16 rows a job may have
+    int subs;                 // one launch: workgroups a slice of a job has, which take its tiles of 16 entries in turn
     float* part;              // two launches: parts of s, [parts][rows][rank rounded up to 16, 32, 64 or 128]
     int parts, steps;         // of `steps` steps of 128 input columns each
 };
@@ -176,22 +176,11 @@ template <bool X32, int RT> struct Few {
     static_assert(AW_WAVES * AD_ROWS * P * 4 <= LDS && LDS <= 160 * 1024, "");
 };
 
+// a tile: the n rows (16 at most count) of lanes' jr, the outputs c0 .. c1 - 1
 template <Elem EL, bool X32, int RT, int OT>
-__global__ void __launch_bounds__(AW_THREADS) k_adapter_mm(const AdapterArgs a) {
+__device__ __forceinline__ void few_rows(const AdapterArgs& a, const Lds& L, const uint8_t* Aw, const uint8_t* Bw, float sc, JobRow jr, int n, int c0, int c1) {
     typedef Few<X32, RT> F;
-    extern __shared__ __align__(16) uint8_t lds_[];
-    const Lds L = lds_of(lds_);
-    const int slice = blockIdx.x % a.slices, tile = blockIdx.x / a.slices, j = tile / a.subs, m0 = tile % a.subs * AD_ROWS;
-    const int lane = threadIdx.x % WAVE, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE), r = lane % 16, q = lane / 16;
-    // all of the job at once: the list holds njobs_cap of them
-    const sfnx_bigjob& job = a.jobs[j];
-    const int nj = *a.njobs, n = min(job.n, SFNX_PF_JOB) - m0, w = job.w;
-    const JobRow jr = job_row(job, n + m0, m0 + r, a.rows);
-    if (j >= nj || n <= 0) return;
-    const int c0 = slice * a.units * AD_UNIT, c1 = min(a.n_out, c0 + a.units * AD_UNIT), o = jr.o;
-    if ((unsigned) w >= (unsigned) a.n) return copy_base<OT>(a, o, c0 + wave * AD_UNIT + 8 * q, c1, AW_WAVES * AD_UNIT);
-    const uint8_t *Aw = expert_at(a.A, a.sa, w), *Bw = expert_at(a.B, a.sb, w);
-    const float sc = a.scale ? a.scale[w] : 1.f;
+    const int lane = threadIdx.x % WAVE, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE), r = lane % 16, q = lane / 16, o = jr.o;
     uint8_t* const xl = L.p + wave * F::BYTES;
     uint8_t* const al = xl + AD_ROWS * F::XROW;
     // ---- a unit's base and B: a tile's row r is column u + 8 (r / 4) + 4 t + r % 4, so that lane l's results are the columns u + 8 q ..
@@ -300,6 +289,34 @@ __global__ void __launch_bounds__(AW_THREADS) k_adapter_mm(const AdapterArgs a) 
         }
         if (o >= 0) store_eight<OT>(a.out, o * a.ldo + u + 8 * q, c1 - u - 8 * q, pack<OT>(v));
         g = request(u + AW_WAVES * AD_UNIT);
+    }
+}
+
+template <Elem EL, bool X32, int RT, int OT>
+__global__ void __launch_bounds__(AW_THREADS) k_adapter_mm(const AdapterArgs a) {
+    extern __shared__ __align__(16) uint8_t lds_[];
+    const Lds L = lds_of(lds_);
+    const int slice = blockIdx.x % a.slices, tile = blockIdx.x / a.slices, j = tile / a.subs, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
+    const int r = threadIdx.x % 16, q = threadIdx.x % WAVE / 16;
+    int m0 = tile % a.subs * AD_ROWS;
+    // all of the job at once: the list holds njobs_cap of them
+    const sfnx_bigjob& job = a.jobs[j];
+    const int nj = *a.njobs, n = min(job.n, SFNX_PF_JOB), w = job.w;
+    JobRow jr = job_row(job, n, m0 + r, a.rows);
+    if (j >= nj || n <= m0) return;
+    const int c0 = slice * a.units * AD_UNIT, c1 = min(a.n_out, c0 + a.units * AD_UNIT);
+    const bool some = (unsigned) w < (unsigned) a.n;
+    const uint8_t *Aw = some ? expert_at(a.A, a.sa, w) : nullptr, *Bw = some ? expert_at(a.B, a.sb, w) : nullptr;
+    const float sc = some && a.scale ? a.scale[w] : 1.f;
+    // one tile, but of a job with more entries than x has rows, some of which are none of its rows
+#pragma unroll 1
+    for (;;) {
+        if (some) few_rows<EL, X32, RT, OT>(a, L, Aw, Bw, sc, jr, n - m0, c0, c1);
+        else copy_base<OT>(a, jr.o, c0 + wave * AD_UNIT + 8 * q, c1, AW_WAVES * AD_UNIT);
+        m0 += a.subs * AD_ROWS;
+        if (m0 >= n) return;
+        __syncthreads();   // the tile's s is read
+        jr = job_row(job, n, m0 + r, a.rows);
     }
 }
 
