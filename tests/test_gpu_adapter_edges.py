@@ -1,4 +1,4 @@
-"""adapter_mm on job lists that no grouping makes."""
+"""adapter_mm on job lists that no grouping makes, and s = scale A x: that it keeps 24 bits in both forms, and the ends of its range."""
 import pytest
 import torch
 
@@ -44,3 +44,61 @@ def test_rows_behind_rows_outside(T, R, t, x_t):
         there = base.cuda()
         moe.adapter_mm(moe.Adapters(A.cuda(), B.cuda()), *jobs, x.cuda(), there, there)
         assert torch.equal(there[done.cuda()], out[done.cuda()]) and torch.equal(there[~done.cuda()].cpu(), base[~done])
+
+
+def in_order(T, n):
+    ids = torch.arange(T, dtype=torch.int32) % n
+    g = moe.RowGroups(T, n, in_place=True)
+    moe.group_rows(ids.cuda(), g)
+    return ids, g
+
+
+def spread(T, R, n_in, bits, t, x_t):
+    """x and A whose s = sum of 2^-b over bits, negative in odd ranks and times 2^(row % 3): every term comes from columns of its own, far apart, and is
+    the product of two normal numbers.  All sums of terms are exact in 32 bits, in any order."""
+    A, x = torch.zeros((2, R, n_in)), torch.zeros((T, n_in))
+    for i, b in enumerate(bits):
+        c = (i * (n_in - 1)) // max(1, len(bits) - 1)
+        A[:, :, c] = 2.0 ** -(b // 2) * (1 - 2 * (torch.arange(R) % 2))
+        x[:, c] = 2.0 ** -(b - b // 2) * 2.0 ** (torch.arange(T) % 3)
+    s = sum(2.0 ** -b for b in bits)
+    return x.to(x_t), A.to(t), s * 2.0 ** (torch.arange(T) % 3).double()[:, None] * (1 - 2 * (torch.arange(R) % 2)).double()
+
+
+SHAPES = [(2, 8, 2048), (2, 32, 1024), (2, 40, 2048), (2, 64, 4096), (3, 128, 2048), (70, 64, 136), (1100, 8, 2048), (1100, 32, 256)]
+
+
+@pytest.mark.parametrize("t, x_t", KINDS)
+@pytest.mark.parametrize("T, R, n_in", SHAPES)
+def test_s_keeps_24_bits(T, R, n_in, t, x_t):
+    """s = 1 + 2^-9 + 2^-17 + 2^-23 needs all bits of 32, and comes out times a power of two; with s = 1 + 2^-9 + 2^-12 values of B of 11 bits
+    give products of 23: everything is exact, in both forms"""
+    n_out, t, x_t = 145, TYPES[t], TYPES[x_t]
+    ids, g = in_order(T, 2)
+    scale = torch.tensor([0.5, -4.0])
+    k = torch.arange(n_out) % R
+    for bits, b in (((0, 9, 17, 23), 1.0), ((0, 9, 12), 1 + 2.0 ** -10 if t == torch.float16 else 1 + 2.0 ** -7)):
+        x, A, s = spread(T, R, n_in, bits, t, x_t)
+        B = torch.zeros((2, n_out, R))
+        B[0, torch.arange(n_out), k] = b * 2.0 ** (torch.arange(n_out) % 5 - 2)
+        B[1] = -2 * B[0]
+        out = torch.empty((T, n_out)).cuda()
+        moe.adapter_mm(moe.Adapters(A.cuda(), B.to(t).cuda(), scale.cuda()), g.jobs, g.njobs, g.cap, x.cuda(), None, out)
+        at = ids.long()
+        want = scale[at].double()[:, None] * s[:, k] * B[at[:, None], torch.arange(n_out), k].double()
+        assert torch.equal(out.cpu().double(), want)
+
+
+@pytest.mark.parametrize("t, x_t", KINDS)
+@pytest.mark.parametrize("T, R", [(2, 8), (2, 40), (3, 128), (1100, 16)])
+def test_smallest_values_of_16_bits(T, R, t, x_t):
+    """x, A and B below their types' smallest normal numbers are not taken for zeros"""
+    n_in, n_out, t, x_t = 256, 70, TYPES[t], TYPES[x_t]
+    low, f = {torch.float16: (2.0 ** -23, 8.0), torch.bfloat16: (2.0 ** -130, 2.0 ** 40)}[t]
+    ids, g = in_order(T, 1)
+    for a, u, b in ((low, f, f), (f, low, f), (f, f, low)):
+        A, x, B = torch.zeros((1, R, n_in)), torch.zeros((T, n_in)), torch.zeros((1, n_out, R))
+        A[:, :, 9], x[:, 9], B[:, :, R - 1] = a, u, b
+        out = torch.empty((T, n_out)).cuda()
+        moe.adapter_mm(moe.Adapters(A.to(t).cuda(), B.to(t).cuda()), g.jobs, g.njobs, g.cap, x.to(x_t).cuda(), None, out)
+        assert (out.cpu().double() == low * f * f).all(), (a, u, b)
