@@ -423,8 +423,10 @@ __global__ void __launch_bounds__(A2_THREADS) k_adapter_shrink(const AdapterArgs
 
 // The second: out = base + B s on bf16 matrix instructions, s as three bf16 parts whose sum it is: the upper 8 bits of its 24, the next, the
 // last (truncated, so that none overflows).  Their products with B's values are exact; f16 values of B are two bf16 parts (the product of
-// both lowest, 2^-25 of the whole, is left out).  A part that is 0 times an infinity would be NaN where the product is not: jobs with such
-// an s, and columns with such a B, are computed value by value.  The results pass through LDS, so that base and out go by whole rows' pieces.
+// both lowest, 2^-25 of the whole, is left out).  A part that is 0 times an infinity would be NaN where the product is not, below 2^-110 the
+// last part's bits would lie under bf16's smallest value, and f16's largest is 65536 in its first part, whose product with an s of 2^112 is
+// infinite: jobs with an s outside [2^-102, 2^112) that is not 0 (above, no part is subnormal), and columns with a B that is not finite, are
+// computed value by value.  The results pass through LDS, so that base and out go by whole rows' pieces.
 // 4096 rows, rank 64, 4096 columns, bf16, 67 MB of base and out: 24.6 us, of which 6 pass before the first product (the job, then the parts of s, which
 // every slice sums and splits for itself), and 2.6 for each unit of 128 columns: reads of LDS and products 1.5, the way out 1.
 // the parts of two finite values, packed
@@ -437,6 +439,12 @@ __device__ __forceinline__ void split3(float f, float g, uint32_t (&p)[3]) {
     p[0] = __builtin_amdgcn_perm(b, a, 0x07060302u);
     p[1] = __builtin_amdgcn_perm(d, c, 0x07060302u);
     p[2] = __builtin_amdgcn_perm(y, x, 0x07060302u);
+}
+// how far a size's bits lie above S_LOW's; of those below, but 0, more than any
+constexpr uint32_t S_LOW = (127u - 102) << 23, S_HIGH = (127u + 112) << 23;
+__device__ __forceinline__ uint32_t past_low(float f) {
+    const uint32_t b = abs_bits(f);
+    return b ? b - S_LOW : 0;
 }
 // the largest size of 16-bit values, in each half
 typedef uint16_t ushort2v __attribute__((ext_vector_type(2)));
@@ -617,13 +625,13 @@ __global__ void __launch_bounds__(Expand<RT>::THREADS) k_adapter_expand(const Ad
 #pragma unroll
                 for (int c = 0; c < RK; c += 2) {
                     const float f = s[i][c] * sc, h = s[i][c + 1] * sc;
-                    size = max(size, max(abs_bits(f), abs_bits(h)));
+                    size = max(size, max(past_low(f), past_low(h)));
                     uint32_t p[3];
                     split3(f, h, p);
 #pragma unroll
                     for (int k = 0; k < 3; ++k) *reinterpret_cast<uint32_t*>(sp + (k * SFNX_PF_JOB + 16 * i + m0) * X::SP + rk + c) = p[k];
                 }
-            const int fin = __all(size < 0x7f800000u);
+            const int fin = __all(size < S_HIGH - S_LOW);
             if (lane == 0) reinterpret_cast<int*>(res)[wave * AE_PITCH + AE_COLS] = fin;   // beside the results
             lds_barrier();
 #pragma unroll

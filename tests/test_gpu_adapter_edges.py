@@ -90,6 +90,38 @@ def test_s_keeps_24_bits(T, R, n_in, t, x_t):
 
 
 @pytest.mark.parametrize("t, x_t", KINDS)
+@pytest.mark.parametrize("T, R, n_in", SHAPES)
+@pytest.mark.parametrize("power", [-118, -112, -106, 100])
+def test_small_and_large_s(T, R, n_in, power, t, x_t):
+    """the same where the scale takes s far down or up: its last bits are beyond 16-bit types' smallest values, and still count"""
+    n_out, t, x_t = 145, TYPES[t], TYPES[x_t]
+    ids, g = in_order(T, 2)
+    scale = torch.tensor([2.0 ** power, -2.0 ** power])
+    k = torch.arange(n_out) % R
+    x, A, s = spread(T, R, n_in, (0, 9, 17, 23), t, x_t)
+    B = torch.zeros((2, n_out, R))
+    B[:, torch.arange(n_out), k] = 2.0 ** 15
+    out = torch.empty((T, n_out)).cuda()
+    moe.adapter_mm(moe.Adapters(A.cuda(), B.to(t).cuda(), scale.cuda()), g.jobs, g.njobs, g.cap, x.cuda(), None, out)
+    want = scale[ids.long()].double()[:, None] * s[:, k] * 2.0 ** 15
+    assert torch.equal(out.cpu().double(), want)
+
+
+@pytest.mark.parametrize("T, R", [(2, 8), (2, 40), (3, 128), (1100, 16)])
+def test_products_that_just_fit(T, R):
+    """s = 5.19393e33 times f16's largest value, 65504, is 3.4022e38 and fits 32 bits; 65536 times s would not"""
+    n_in, n_out = 256, 70
+    ids, g = in_order(T, 1)
+    A, B, x = torch.zeros((1, R, n_in)), torch.zeros((1, n_out, R)), torch.zeros((T, n_in))
+    A[0, R - 1, 7], x[:, 7], B[0, :, R - 1] = 1.0, 5.19393e33, 65504.0
+    assert float(x[0, 7]) * 65504 < torch.finfo(torch.float32).max < float(x[0, 7]) * 65536
+    out = torch.empty((T, n_out)).cuda()
+    moe.adapter_mm(moe.Adapters(A.half().cuda(), B.half().cuda()), g.jobs, g.njobs, g.cap, x.cuda(), None, out)
+    want = torch.full((T, n_out), float(x[0, 7]) * 65504, dtype=torch.float64)
+    within(out, want, 2 * STEP * want, torch.float32)   # a product as two, their sum
+
+
+@pytest.mark.parametrize("t, x_t", KINDS)
 @pytest.mark.parametrize("T, R", [(2, 8), (2, 40), (3, 128), (1100, 16)])
 def test_smallest_values_of_16_bits(T, R, t, x_t):
     """x, A and B below their types' smallest normal numbers are not taken for zeros"""
