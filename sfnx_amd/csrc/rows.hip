@@ -49,6 +49,7 @@ __device__ __forceinline__ void block_prefix(int& a, int& b, int (&sums)[2][GR_W
 }
 
 // table: the chunks' counts, or null
+constexpr int GR_FIXED = (2 * GR_WAVES + 1) * 4 + 12;   // LDS beside the 28 bytes a group: sums and all, to the next 16 bytes
 __global__ void __launch_bounds__(GR_THREADS) k_group_rows(const int* __restrict__ ids, int n, int G, int chunk, const int* __restrict__ table,
                                                           int* __restrict__ offsets, int* __restrict__ pos, int* __restrict__ order,
                                                           sfnx_bigjob* __restrict__ jobs, int* __restrict__ njobs, int in_place) {
@@ -408,9 +409,9 @@ extern "C" int sfnx_group_rows(const int* ids, int n, int n_groups, int* offsets
         int* const table = need ? (int*) ws : nullptr;
         if (table) k_group_count<<<blocks, GR_THREADS, n_groups * sizeof(int), stream_of(st)>>>(ids, n, n_groups, chunk, table);
         static std::atomic<uint64_t> asked{0};
-        if (28 * n_groups > 64 * 1024) allow_lds((const void*) k_group_rows, 28 * GR_MAX, asked);
-        k_group_rows<<<blocks, GR_THREADS, 28 * (size_t) n_groups, stream_of(st)>>>(ids, n, n_groups, chunk, table, offsets, pos, order, jobs,
-                                                                                       njobs, in_place);
+        const int lds = 28 * n_groups;
+        if (lds + GR_FIXED > 64 * 1024) allow_lds((const void*) k_group_rows, 28 * GR_MAX, asked);
+        k_group_rows<<<blocks, GR_THREADS, lds, stream_of(st)>>>(ids, n, n_groups, chunk, table, offsets, pos, order, jobs, njobs, in_place);
     });
 }
 
