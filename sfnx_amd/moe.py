@@ -410,6 +410,8 @@ class RowGroups:
     def __init__(self, n: int, n_groups: int, in_place: bool = False, device="cuda"):
         if n < 0 or n_groups < 1:
             raise ValueError("n below 0, or no groups")
+        if max(n, n_groups) > _INT_MAX:
+            raise ValueError(f"{max(n, n_groups)} rows or groups, more than {_INT_MAX}")
         i32 = dict(dtype=torch.int32, device=device)
         self.n, self.n_groups, self.in_place = n, n_groups, in_place
         self.cap = n // PF_JOB + min(n, n_groups) + 1
@@ -457,6 +459,8 @@ def _need_picks(pos, T: int, dev) -> int:
         _need(pos, "pos", _I32)
     if pos.numel() != T * K or (pos.dim() == 2 and pos.shape[0] != T):
         raise ValueError(f"pos: {tuple(pos.shape)}, expected K for each of {T} tokens")
+    if K > _INT_MAX:
+        _too_large("pos", (T, K))
     return K
 
 
@@ -478,7 +482,7 @@ def moe_sort_rows(x, pos, xs) -> None:
         raise ValueError(f"x: type {dt}, xs {xs.dtype}: expected the same, of 1, 2 or 4 bytes")
     s, d, p = x.shape, xs.shape, pos.shape
     if (len(s) == len(d) == len(p) == 2 and s[1] == d[1] and s[0] == p[0] and pos.dtype is torch.int32 and _usual(dev, x, xs, pos)
-            and max(s[0], d[0], s[1]) <= _INT_MAX):
+            and max(s[0], d[0], s[1], p[1]) <= _INT_MAX):
         K, ldx, ldxs = p[1], s[1], d[1]
     else:
         ldx = _need_matrix(x, "x", (dt,), None, dev)
@@ -491,7 +495,7 @@ def moe_sort_rows_backward(dxs, pos, dx) -> None:
     """dx[t] = sum_k dxs[pos[t][k]], the gradient of moe_sort_rows; each of f32, f16 or bf16"""
     dev, s, d, p = _current(), dxs.shape, dx.shape, pos.shape
     if (len(s) == len(d) == len(p) == 2 and s[1] == d[1] and d[0] == p[0] and pos.dtype is torch.int32 and dxs.dtype in _TYPE_ID
-            and dx.dtype in _TYPE_ID and _usual(dev, dxs, dx, pos) and max(s[0], d[0], s[1]) <= _INT_MAX):
+            and dx.dtype in _TYPE_ID and _usual(dev, dxs, dx, pos) and max(s[0], d[0], s[1], p[1]) <= _INT_MAX):
         K, lddxs, lddx = p[1], s[1], d[1]
     else:
         lddxs = _need_matrix(dxs, "dxs", _TYPE_ID, None, dev)
@@ -506,7 +510,7 @@ def moe_combine_sorted(ys, topw, pos, y) -> None:
     dev, s, d, p = _current(), ys.shape, y.shape, pos.shape
     if (len(s) == len(d) == len(p) == 2 and s[1] == d[1] and d[0] == p[0] and p == topw.shape and pos.dtype is torch.int32
             and topw.dtype is torch.float32 and ys.dtype in _TYPE_ID and y.dtype in _TYPE_ID and _usual(dev, ys, y, pos, topw)
-            and max(s[0], d[0], s[1]) <= _INT_MAX):
+            and max(s[0], d[0], s[1], p[1]) <= _INT_MAX):
         K, ldys, ldy = p[1], s[1], d[1]
     else:
         ldys = _need_matrix(ys, "ys", _TYPE_ID, None, dev)
@@ -523,7 +527,7 @@ def moe_combine_sorted_backward(dy, ys, topw, pos, dys, dw) -> None:
     dev, d, s, p = _current(), dy.shape, ys.shape, pos.shape
     if (len(s) == len(d) == len(p) == 2 and s[1] == d[1] and d[0] == p[0] and p == topw.shape and pos.dtype is torch.int32
             and topw.dtype is torch.float32 and ys.dtype in _TYPE_ID and dy.dtype in _TYPE_ID and _usual(dev, dy, ys, pos, topw)
-            and max(s[0], d[0], s[1]) <= _INT_MAX
+            and max(s[0], d[0], s[1], p[1]) <= _INT_MAX
             and (dys is None or (dys.dtype is ys.dtype and dys.shape == s and _usual(dev, dys)))
             and (dw is None or (dw.dtype is torch.float32 and dw.shape == p and _usual(dev, dw)))):
         K = p[1]
@@ -557,6 +561,9 @@ class Adapters:
                 raise ValueError(f"{name}: {m.dim()} dimensions, expected a matrix for each adapter")
         self.n, self.dtype, self.type, self.device = len(A), a.dtype, _TYPE_ID[a.dtype], a.get_device()
         self.rank, self.n_in, self.n_out = a.shape[-2], a.shape[-1], b.shape[-2]
+        for name, sizes in (("A", (self.n, self.rank, self.n_in)), ("B", (self.n_out,))):
+            if max(sizes) > _INT_MAX:
+                _too_large(name, sizes)
         self._a, self.sa, self._A = self._place("A", A, (self.rank, self.n_in))
         self._b, self.sb, self._B = self._place("B", B, (self.n_out, self.rank))
         if scale is not None:
