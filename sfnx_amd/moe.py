@@ -547,10 +547,13 @@ def moe_combine_sorted_backward(dy, ys, topw, pos, dys, dw) -> None:
 class Adapters:
     """Low-rank adapters of one projection, of many requests: A [n][rank][n_in] and B [n][n_out][rank] (f16 or bf16), or lists of n
     matrices that live apart (then reached through tables of their pointers), and scale [n] f32 (None: 1).  rank is a multiple of 8, at
-    most 128: an adapter of another rank is filled up with zeros."""
+    most 128: an adapter of another rank is filled up with zeros.  The matrices given are held and read at each call, so changes of their
+    values count; other matrices, in a list that was given or by an attribute, need other Adapters."""
 
     def __init__(self, A, B, scale: torch.Tensor | None = None):
-        self.A, self.B, self.scale = A, B, scale   # held: the tables point into them
+        A, B = (M if isinstance(M, torch.Tensor) else tuple(M) for M in (A, B))
+        self.A, self.B, self.scale = A, B, scale
+        self._held = A, B, scale   # whose addresses are taken below
         if len(A) < 1 or len(A) != len(B):
             raise ValueError("A and B: expected a matrix of each for every adapter")
         a, b = (M if isinstance(M, torch.Tensor) else M[0] for M in (A, B))

@@ -1,4 +1,7 @@
-"""Sizes that the library's 32-bit integers would cut, on a host without a GPU."""
+"""What Adapters and RowGroups keep for the library's pointers and 32-bit sizes, on a host without a GPU."""
+import gc
+import weakref
+
 import pytest
 import torch
 
@@ -9,6 +12,39 @@ from sfnx_amd import moe
 def anywhere(monkeypatch):
     """tensors are taken where they are"""
     monkeypatch.setattr(moe, "_need", lambda *a, **k: None)
+
+
+def bf(*s):
+    return torch.ones(s, dtype=torch.bfloat16)
+
+
+def test_adapters_hold_what_their_tables_name(anywhere):
+    """a list whose entries are replaced, or cleared, after the tables were made: the matrices live as long as the adapters"""
+    A, B = [bf(8, 16) for _ in range(3)], [bf(5, 8) for _ in range(3)]
+    at = [m.data_ptr() for m in A], [m.data_ptr() for m in B]
+    alive = [weakref.ref(m) for m in A + B]
+    ad = moe.Adapters(A, B)
+    A[1] = bf(8, 16)
+    B.clear()
+    A.pop()
+    gc.collect()
+    assert all(r() is not None for r in alive)
+    assert ad._A.tolist() == at[0] and ad._B.tolist() == at[1]
+    del ad
+    gc.collect()
+    assert alive[1]() is None and alive[2]() is None and alive[3]() is None
+
+
+def test_adapters_hold_what_they_were_made_of(anywhere):
+    """attributes given other tensors, or none: the addresses taken stay those of tensors that live"""
+    A, B, scale = bf(3, 8, 16), bf(3, 5, 8), torch.ones(3)
+    alive = [weakref.ref(m) for m in (A, B, scale)]
+    ad = moe.Adapters(A, B, scale)
+    a, b, s = A.data_ptr(), B.data_ptr(), scale.data_ptr()
+    del A, B, scale
+    ad.A = ad.B = ad.scale = None
+    gc.collect()
+    assert all(r() is not None for r in alive) and (ad._a, ad._b, ad._scale) == (a, b, s)
 
 
 @pytest.mark.parametrize("n, G", [(2 ** 31, 3), (2 ** 32 + 5, 3), (5, 2 ** 31), (5, 2 ** 32 + 3)])
