@@ -251,7 +251,8 @@ int sfnx_group_rows(const int* ids, int n, int n_groups, int* offsets, int* pos,
 size_t sfnx_group_rows_workspace(int n, int n_groups);
 /* xs[pos[t][k]] = x[t] for rows of H values of elem (1, 2 or 4) bytes, pos [T][K] (of sfnx_group_rows), rows of x and xs ldx and ldxs
  * values apart.  Here and below an entry of pos outside [0, rows) is left out (rows: of the sorted side), a sorted row that no entry names
- * is left as it was, and K <= 64, H <= 2^20.  No two entries may be equal, and outputs overlap no input but where it is said. */
+ * is left as it was, and K <= 64, H <= 2^20.  No two entries may be equal, and outputs overlap no input but where it is said.  A launch has fewer
+ * than 2^32 threads: T below 2^22 in the combine's gradient, below 2^32 over a row's threads (16 bytes each) in the others; more is refused. */
 int sfnx_moe_sort_rows(int elem, const void* x, int64_t ldx, int T, int K, int H, const int* pos, void* xs, int64_t ldxs, int rows, void* st);
 /* dx[t] = sum_k dxs[pos[t][k]], summed in 32 bits in k order and rounded once (0 where every entry is left out).  Types SFNX_F32,
  * SFNX_F16 or SFNX_BF16, each side its own. */
@@ -275,8 +276,10 @@ int sfnx_moe_combine_sorted_backward(uint32_t dy_type, const void* dy, int64_t l
  * zeros.  scale [n_adapters] f32, or null (1).  x: f32 or of the adapters' type, rows ldx values apart.  base and out: f32, f16 or
  * bf16, rows ldo values apart; base may be out (added in place) or null (zeros).  A job whose w is no adapter adds nothing: its
  * out rows become base's (group n_adapters serves rows without one; in place they may also be in no job).  Rows of no job are left as
- * they were, and so are rows outside [0, rows) in a job.  A row may be out of one job only.  A_a x and its product with B_a are summed and
- * kept in 32 bits, and rounded once, with base, to out's type.
+ * they were; entries whose y or out is outside [0, rows) are left out, and a job may have more entries than there are rows.  A row may be
+ * out of one entry of one job only.  A_a x and its product with B_a are summed and kept in 32 bits, and rounded once, with base, to out's type.
+ * The same call gives the same bits; the order of a row's sums goes by the row's place in the list, the number of rows and the list's size, so
+ * that beside other rows its last bits may differ.  One row whose s is not finite slows its whole job.
  * rank % 8 == 0, at most 128; n_in % 8 == 0; n_in and n_out at most 2^20; A, B, x and their rows 16-byte aligned.
  * Few rows of small ranks are one launch, others two, which need a workspace of sfnx_adapter_workspace bytes (0: none; never less for more
  * rows), 16-byte aligned, whose contents do not matter; calls that may overlap need one each.  out overlaps neither x nor, unless it is base,

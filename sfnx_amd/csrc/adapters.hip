@@ -162,8 +162,8 @@ template <Elem EL, bool X32> __device__ __forceinline__ float4v shrink_mma(const
 __device__ __forceinline__ uint4 lds16(const uint8_t* p) { return *reinterpret_cast<const uint4*>(p); }
 
 // ------------------------------------------------------------------------------------------------ one launch
-// For few rows and small ranks.  Bound by a chain of reads: the job, its rows of x and A, B's tail, a launch's start (1 row, rank 16, 2048 -> 1024, f32: 5.3 us; 16 rows of
-// 16 adapters, 2048 -> 2048, bf16: 6.1).  Each wavefront copies its own chunks of columns and multiplies them, so that none waits for another
+// For few rows and small ranks.  Bound by a chain of reads: the job, its rows of x and A, B's tail, a launch's start (1 row, rank 16, 2048 -> 1024, f32: 5.2 us; 16 rows of
+// 16 adapters, 2048 -> 2048, bf16: 6.2).  Each wavefront copies its own chunks of columns and multiplies them, so that none waits for another
 // before the sum; base and B are on their way meanwhile.  Loops stay rolled: a launch of few workgroups runs its code once, and fetching it is
 // part of its time (f32 x, 16 ranks, 2048 columns, unrolled to one pass: 12.7 us a launch).
 constexpr int AW_WAVES = 8, AW_THREADS = AW_WAVES * WAVE;
@@ -426,7 +426,8 @@ __global__ void __launch_bounds__(A2_THREADS) k_adapter_shrink(const AdapterArgs
 // both lowest, 2^-25 of the whole, is left out).  A part that is 0 times an infinity would be NaN where the product is not, below 2^-110 the
 // last part's bits would lie under bf16's smallest value, and f16's largest is 65536 in its first part, whose product with an s of 2^112 is
 // infinite: jobs with an s outside [2^-102, 2^112) that is not 0 (above, no part is subnormal), and columns with a B that is not finite, are
-// computed value by value.  The results pass through LDS, so that base and out go by whole rows' pieces.
+// computed value by value, and the call takes as long as such a job does (4096 rows, rank 64, 4096 columns, one value of x infinite: 595 us for 40).
+// The results pass through LDS, so that base and out go by whole rows' pieces.
 // 4096 rows, rank 64, 4096 columns, bf16, 67 MB of base and out: 24.6 us, of which 6 pass before the first product (the job, then the parts of s, which
 // every slice sums and splits for itself), and 2.6 for each unit of 128 columns: reads of LDS and products 1.5, the way out 1.
 // the parts of two finite values, packed
@@ -686,17 +687,18 @@ void split_columns(int64_t jobs, int n_in, int& parts, int& steps) {
 // The form.  One launch computes s in each slice and holds 128 KB of LDS, two have a launch more and pass s through memory.  us in a graph, one
 // and two launches, 4 adapters of a list of 8, 2048 -> 2048 columns, bf16:
 //   rows                 1          16          128         512         1024        2048        4096
-//   rank 16, bf16 x      4.6  7.9   6.3  8.2    7.0  9.4    8.4  10.7   10.1 12.4   17.0 16.7   32.9 21.9
-//   rank 32, bf16 x      6.0  8.3   7.9  8.4    8.1  10.3   9.6  11.6   11.8 13.9   19.7 18.5   37.7 23.2
-//   rank 16, f32 x       5.3  9.1   9.6  9.5    10.7 11.2   11.9 12.2   13.9 14.2   21.6 19.8   40.5 25.6
-//   rank 32, f32 x       6.7  10.3  12.6 10.4   13.7 12.4   15.1 13.6   17.4 16.1   25.9 22.4   48.9 28.7
+//   rank 16, bf16 x      4.7  8.0   6.3  8.2    6.9  9.5    8.3  10.9   10.0 12.3   17.0 16.9   32.5 22.1
+//   rank 32, bf16 x      6.1  8.3   7.6  8.5    7.9  10.4   9.5  11.6   11.7 13.9   19.6 18.7   37.3 23.3
+//   rank 16, f32 x       5.2  9.2   8.7  9.5    9.9  11.3   11.0 12.3   13.2 14.1   20.5 19.9   38.0 25.8
+//   rank 32, f32 x       6.7  10.4  12.1 10.5   13.5 12.4   14.9 13.7   17.2 16.1   25.6 22.5   48.0 28.9
 // A window's rows are mostly one to an adapter, which one launch multiplies as the first column does.  Ranks above 32 are two launches: each slice would
 // read 256 KB of A for itself, of which a compute unit takes in about 35 KB/us.
 bool two_launches(int rows, int rank, bool x32) { return rank > 32 || rows > 1024 || (x32 && rank > 16 && rows > SFNX_MAXT); }
 
 // Jobs that are not full, as launches take them: one for each adapter, and for the rows without; of a long list a chunk's rows are taken to use a
 // quarter.  More are a second round of workgroups, fewer leave compute units idle (4096 rows of 16 of 64 adapters, 2048 -> 2048, rank 32, f32:
-// 38 us, with all 64 counted 71).
+// 38 us, with all 64 counted 71).  Long lists of which few are used leave them idle all the same: 4096 rows of 4 adapters, rank 64, 4096 columns,
+// 39.6 us of a list of 8, 41.0 of 64, 108 of 1000.
 int64_t short_jobs(const AdapterArgs& a) {
     const int most = std::min(a.rows, a.n + 1);
     return a.rows <= 256 ? most : (most + 3) / 4;
