@@ -48,8 +48,8 @@ __device__ __forceinline__ void block_prefix(int& a, int& b, int (&sums)[2][GR_W
     a -= a0, b -= b0;
 }
 
-// table: the chunks' counts, or null
 constexpr int GR_FIXED = (2 * GR_WAVES + 1) * 4 + 12;   // LDS beside the 28 bytes a group: sums and all, to the next 16 bytes
+// table: the chunks' counts, or null
 __global__ void __launch_bounds__(GR_THREADS) k_group_rows(const int* __restrict__ ids, int n, int G, int chunk, const int* __restrict__ table,
                                                           int* __restrict__ offsets, int* __restrict__ pos, int* __restrict__ order,
                                                           sfnx_bigjob* __restrict__ jobs, int* __restrict__ njobs, int in_place) {
